@@ -52,7 +52,7 @@ def hip_source_id(extra_flags=()):
     are built from them.  The compiler's version is NOT part of it: the id must be reproducible on a box that only loads the
     prebuilt libraries (no hipcc call at import); a compiler change rebuilds through force=True / a clean tree."""
     return _digest(hip_sources() + glob.glob(os.path.join(_native.CSRC, "*.h")) + [os.path.join(ROOT, "include", "onedc_hip.h")],
-                   repr(sorted(FILE_FLAGS.items())) + repr(tuple(extra_flags)))
+                   repr(HIP_FLAGS) + repr(sorted(FILE_FLAGS.items())) + repr(tuple(extra_flags)))
 
 
 BUILD_ID_MARKER = b"@(#)onedc-build-id:"
@@ -90,6 +90,10 @@ def build_coder(force=False):
 # on one box: window kernel with GroupNorm on load 128->128 at 768x768 3.47 -> 3.38 ms, 256->128 5.80 -> 5.57; GEGLU
 # 320->2560 422 -> 410 us; d = 80 attention 0.951 -> 0.874 ms; everything else within noise.
 _NO_SLP = ("-fno-slp-vectorize",)
+# Every HIP file: no packed-f32 instructions (v_pk_add / mul / fma_f32).  Some of their forms have given wrong results on MI355X now
+# and then, without an error; the scalar pairs compute the same IEEE values.  (The host pass does not know the feature and says so.)
+HIP_FLAGS = ("--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang",
+             "-packed-fp32-ops")
 # ref_arith.hip reproduces torch-CPU's rounding sequence: a multiply followed by an add must stay two roundings (the chains
 # themselves are explicit fmaf calls)
 FILE_FLAGS = {"attention.hip": ("-fno-honor-nans",) + _NO_SLP, "xattn_block.hip": ("-fno-honor-nans",) + _NO_SLP, "gemm_conv_win.hip": _NO_SLP, "gemm_conv_win4.hip": _NO_SLP, "gemm_conv.hip": _NO_SLP,
@@ -126,7 +130,7 @@ def build_hip(force=False, extra_flags=()):
             # a wrong id means the objects' provenance is unknown (a copied tree keeps no mtimes, an ablation build leaves
             # mtime-fresh objects behind): all of them are compiled again, not only the one that carries the id
             if force or wrong_id or _stale(o, [s] + headers):
-                jobs.append([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c", "-Wno-unused-result",
+                jobs.append([HIPCC, *HIP_FLAGS, "-c",
                              *FILE_FLAGS.get(os.path.basename(s), ()), *defs, *extra_flags,
                              *((f'-DONEDC_BUILD_ID="{sid}"',) if carries_id else ()), "-o", o, s])
             objs.append(o)
@@ -160,8 +164,7 @@ def build_probe(force=False):
     obj = os.path.join(_native.CSRC, "gemm_conv_win4.probe.f16.o")
     others = [s[:-4] + ".f16.o" for s in hip_sources() if os.path.basename(s) != "gemm_conv_win4.hip"]
     if force or _stale(obj, [src] + headers):
-        _run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c", "-Wno-unused-result",
-              *FILE_FLAGS.get("gemm_conv_win4.hip", ()), "-DONEDC_ACT_F16", "-DEXP_W4_TIMELINE", "-o", obj, src])
+        _run([HIPCC, *HIP_FLAGS, "-c", *FILE_FLAGS.get("gemm_conv_win4.hip", ()), "-DONEDC_ACT_F16", "-DEXP_W4_TIMELINE", "-o", obj, src])
     if force or _stale(PROBE_F16_SO, [obj] + others):
         _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", PROBE_F16_SO, obj, *others])
     print(f"[build] {os.path.relpath(PROBE_F16_SO, ROOT)}: diagnostic build (clock probe)", flush=True)

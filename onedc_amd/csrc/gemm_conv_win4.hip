@@ -631,8 +631,8 @@ __global__ __launch_bounds__(256, 2) void conv_win4_kernel(const onedc_conv_para
     typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
     typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
     lds_char *const my = (lds_char *)smem + wave * 16384;
-    // Epilogue arithmetic on channel PAIRS (v_pk_fma_f32 / v_pk_add_f32: no MFMA of this wave is in flight any more, and
-    // a wave finishes 128 outputs per lane): value = alpha * acc + bias + residual; statistics are kept per pair -- (sum,
+    // Epilogue arithmetic on channel PAIRS (a wave finishes 128 outputs per lane; the build has packed f32 instructions off, so a
+    // pair is two scalar instructions): value = alpha * acc + bias + residual; statistics are kept per pair -- (sum,
     // sum of squares) of (v0, v1) and of (v2, v3) -- and folded to quads at the end where the buffer wants quads.  Fixed
     // order, no atomics; the order is this kernel's own (its k order already is).
     f32x2_t s_lo[2][4], q_lo[2][4], s_hi[2][4], q_hi[2][4];

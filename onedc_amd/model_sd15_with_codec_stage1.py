@@ -353,7 +353,7 @@ class DecodePipeline:
     """Throughput mode for a stream of batches: a software pipeline over whole batches.
 
     Stage E (entropy: container parse, prior networks, the four host rANS hops, all latency-bound and
-    GPU-light) of batch n+1 runs on a worker thread with its own high-priority HIP stream while stage S
+    GPU-light) of batch n+1 runs on a worker thread with its own HIP stream while stage S
     (synthesis transform, UNet step, VAE decoder: 97 % of the device time) of earlier batches runs on
     `s_streams` further worker threads, each with its own stream.  Two S streams are the default: the ~700
     kernels of one stage S form a dependent chain, and between two dependent kernels the GPU idles for the
@@ -369,7 +369,8 @@ class DecodePipeline:
         self.z_only = z_only
         self.dev = model.device
         with torch.cuda.device(self.dev):
-            self.stream_e = torch.cuda.Stream(device=self.dev, priority=-1)
+            # (every stream at the default priority: work on streams of different priorities can hang this GPU for good)
+            self.stream_e = torch.cuda.Stream(device=self.dev)
             self.streams_s = [torch.cuda.Stream(device=self.dev) for _ in range(max(1, s_streams))]
         # The VAE decoders of the stage-S streams run one after the other ON THE GPU (each waits for the previous one's
         # end-of-VAE event): two VAE decoders side by side only time-slice the same CUs -- every one of their kernels

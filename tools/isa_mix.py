@@ -46,7 +46,7 @@ def main():
     flags = list(FILE_FLAGS.get(os.path.basename(src), ()))
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
-        cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-DONEDC_ACT_F16", "-S", "--cuda-device-only",
+        cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-DONEDC_ACT_F16", "-S", "--cuda-device-only",
                "-Wno-unused-result", *flags, *extra, "-o", out, src]
         subprocess.run(cmd, check=True, stderr=subprocess.DEVNULL)
         text = open(out).read().split("\n")

@@ -1,7 +1,7 @@
 // issue_mix.hip — what the vector pipe and the matrix pipe of ONE SIMD cost each other, in shader cycles per instruction.
 // The question behind it (flash_attn64): a wave issues 64 v_exp_f32, 32 packs and 56 MFMAs per tile and
 // shares its SIMD with one other wave -- which of those streams add, which hide behind each other?
-//   hipcc --offload-arch=gfx950 -O3 -o tools/micro/issue_mix tools/micro/issue_mix.hip && tools/micro/issue_mix
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/micro/issue_mix tools/micro/issue_mix.hip && tools/micro/issue_mix
 // Every wave runs ITER iterations of one instruction mix on registers only and reads s_memtime around the loop; the host
 // prints shader cycles per iteration and wave for one, two and three waves per SIMD (256, 512 or 768 workgroups of 4 waves on
 // 256 CUs; their LDS request, 128 / 64 / 40 KB, decides how many share a CU).
@@ -19,7 +19,7 @@ constexpr int ITER = 4096;
 // MODE: 0  16 v_exp_f32            1  16 v_fma_f32            2  8 MFMA 16x16x32         3  4 MFMA 32x32x16
 //       4  8 MFMA16 + 16 v_exp     5  8 MFMA16 + 16 v_fma     6  4 MFMA32 + 16 v_exp     7  4 MFMA32 + 16 v_fma
 //       8  16 v_exp + 8 v_cvt_pk_bf16_f32 + 14 MFMA16 (flash_attn64's mix per 16 scores of a lane)
-//       9  16 v_permlane16_swap    10 16 v_exp_f16             11 8 v_pk_fma_f32 (16 values)
+//       9  16 v_permlane16_swap    10 16 v_exp_f16
 template <int MODE>
 __global__ __launch_bounds__(256) void mix_kernel(unsigned long long *cycles, float *out, int seed) {
     extern __shared__ char smem[];
@@ -61,8 +61,6 @@ __global__ __launch_bounds__(256) void mix_kernel(unsigned long long *cycles, fl
             if (MODE == 8 && (i & 1)) asm volatile("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(pk[i >> 1]) : "v"(x[i - 1]), "v"(x[i]));
             if (MODE == 9) asm volatile("v_permlane16_swap_b32 %0, %1" : "+v"(x[i]), "+v"(x[i ^ 1]));
             if (MODE == 10) asm volatile("v_exp_f16 %0, %0" : "+v"(x[i]));
-            if (MODE == 11 && (i & 1))
-                asm volatile("v_pk_fma_f32 %0, %0, %0, %0" : "+v"(*(double *)&x[i - 1]));
         }
     }
     const unsigned long long t1 = __builtin_amdgcn_s_memtime();
@@ -117,7 +115,6 @@ int main() {
     run<0>("16 v_exp_f32", cyc, out);
     run<10>("16 v_exp_f16", cyc, out);
     run<1>("16 v_fma_f32", cyc, out);
-    run<11>("8 v_pk_fma_f32 (16 values)", cyc, out);
     run<9>("16 v_permlane16_swap_b32", cyc, out);
     run<2>("8 v_mfma_f32_16x16x32_bf16", cyc, out);
     run<3>("4 v_mfma_f32_32x32x16_bf16 (the same flops)", cyc, out);

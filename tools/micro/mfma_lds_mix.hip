@@ -6,7 +6,7 @@
 // 32 MFMAs, random f16 / bf16 data, ~1.5 s per case so that the power management settles; TFLOP/s from HIP events, the in-loop
 // clock from s_memtime / s_memrealtime stamps of every wave (MI355X_MICROARCH.md, DVFS give-back item 6; the stamps go to a buffer
 // nothing else reads).
-//   hipcc --offload-arch=gfx950 -O3 -o tools/micro/mfma_lds_mix tools/micro/mfma_lds_mix.hip && tools/micro/mfma_lds_mix
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/micro/mfma_lds_mix tools/micro/mfma_lds_mix.hip && tools/micro/mfma_lds_mix
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cstdint>

@@ -1,6 +1,6 @@
 // mfma_power.hip — does the sustained matrix rate depend on the operands' BITS?  (the bf16 build of the window
 // kernel runs 3 - 6 % faster than the f16 build on the same layers, while on constant operands the f16 instruction is the faster one.)
-//   hipcc --offload-arch=gfx950 -O3 -o tools/micro/mfma_power tools/micro/mfma_power.hip && tools/micro/mfma_power
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/micro/mfma_power tools/micro/mfma_power.hip && tools/micro/mfma_power
 // Register-only loops of v_mfma_f32_16x16x32_f16 / _bf16, 8 waves per SIMD, ~0.5 s per case so that the power management settles;
 // operands: random values (full mantissa), the same values with the low mantissa bits of A, or of A and B, cleared.
 #include <hip/hip_runtime.h>

@@ -1,6 +1,6 @@
 // mfma_rate.hip — what the matrix cores of THIS chip deliver per format, registers only (no LDS, no memory): the ceiling
 // an MXFP8 conv could reach against the 16-bit kernels.
-//   hipcc --offload-arch=gfx950 -O3 -o tools/micro/mfma_rate tools/micro/mfma_rate.hip && tools/micro/mfma_rate
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/micro/mfma_rate tools/micro/mfma_rate.hip && tools/micro/mfma_rate
 // Every wave issues ITER x 16 independent MFMAs (16 accumulator tiles, so no instruction waits for the previous one's
 // result); 8 waves per SIMD hide the issue gaps.  Prints TFLOP/s at the clock the chip holds under that load.
 #include <hip/hip_runtime.h>
