@@ -372,6 +372,95 @@ int onedc_ref_prior_indexes(const float *params, const float *thresholds, int n_
 int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_cs, int x_co, int y_cs, int y_co,
                           void *stream);
 
+/* ---- transformer-block operators for image / video tokens ---------------------------------------------------------------
+ * Norms before and after a block fused with the block's gate and the residual scale: the join between two sub-blocks of a
+ * transformer block in one pass over the residual stream.  Per token row (b, n) of C channels:
+ *   t  = x + alpha * gate[b] * P(f)                         P = identity, or (post) norm(f) * post_w + post_b
+ *   xo = t in the stream's type                             (f, xo NULL: t = x, no join)
+ *   y  = (norm(t) * w + b) * (1 + scale[b]) + shift[b]      (y NULL: no norm behind the join)
+ * norm = LayerNorm (mean and variance) or RMSNorm (mean square) over the C channels, statistics and arithmetic in f32; y is taken
+ * from t BEFORE xo's rounding.  Every vector is f32 and may be NULL (factor 1, summand 0); gate / scale / shift hold one row per
+ * picture, `*_rs` floats apart (0: one row for all pictures, e.g. a learned per-channel residual scale as the gate).
+ * x and xo are 16-bit or (x_f32) f32; f, y are 16-bit or (f_f32, only with x_f32) f32.  Rows are NHWC views: channel stride *_cs,
+ * offset *_co, any values; xo may be x itself.  B * N rows may be 0.  Launches only, no workspace.
+ * Returns -1 for a missing pointer, -2 for sizes or strides, -3 for a combination of options that has no meaning. */
+enum { ONEDC_NORM_LAYER = 0, ONEDC_NORM_RMS = 1 };
+typedef struct onedc_block_norm_params {
+    const void *x; const void *f; void *xo; void *y;
+    const float *post_w; const float *post_b; const float *gate; const float *w; const float *b; const float *scale; const float *shift;
+    int32_t B, N, C;
+    int32_t x_cs, x_co, f_cs, f_co, xo_cs, xo_co, y_cs, y_co;
+    int32_t gate_rs, scale_rs, shift_rs;
+    int32_t kind, post, x_f32, f_f32;
+    float alpha, eps;
+} onedc_block_norm_params;
+int onedc_block_norm(const onedc_block_norm_params *p, void *stream);
+
+/* Its backward pass.  p as in the forward call, but p->x (x_cs, x_co) is the joined stream t as stored (the forward's xo) and p->xo,
+ * p->y are not read.  dy: gradient of y (NULL: none, no norm behind the join); dxo: gradient of xo (NULL: 0; one of the two is
+ * given).  dx = dt: gradient of x; df: gradient of f (both NULL-able).  dy, df have f's type, dxo, dx x's type; dx may be dxo, df may
+ * be dy.  Parameter gradients, f32, each NULL where not wanted: d_post_w, d_post_b, d_w, d_b [C]; d_gate, d_scale, d_shift [C] per
+ * picture, dense -- or one row summed over the pictures where the parameter is one row for all (*_rs == 0).
+ * Sums over rows run in a fixed order (no atomics): partial sums per run of rows in ws, f32 inside a run, f64 across runs.
+ * ws: onedc_block_norm_backward_ws_bytes(p, g) bytes of device scratch, the call's own until it has run (0: none needed).
+ * Statuses as above; -15: ws missing or too small. */
+typedef struct onedc_block_norm_grad {
+    const void *dy; const void *dxo; void *dx; void *df;
+    float *d_post_w; float *d_post_b; float *d_gate; float *d_w; float *d_b; float *d_scale; float *d_shift;
+    void *ws; int64_t ws_bytes;
+    int32_t dy_cs, dy_co, dxo_cs, dxo_co, dx_cs, dx_co, df_cs, df_co;
+} onedc_block_norm_grad;
+int64_t onedc_block_norm_backward_ws_bytes(const onedc_block_norm_params *p, const onedc_block_norm_grad *g);
+int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_block_norm_grad *g, void *stream);
+
+/* Rotary positions over several axes (time, height, width, ...): pair i of every head of token n turns by the angle
+ * pos[n][axis[i]] * freq[i].  Queries and keys in one launch; heads of D dims back to back in rows of *_cs channels at offset *_co.
+ * Pair i is (i, i + pairs) or, neighbours = 1, (2 i, 2 i + 1); dims from 2 * pairs on pass through.  inverse = 1 turns back: the
+ * backward pass of the operator.  turns: f64 [pairs], frequency / 2 pi (the phase is reduced to a fraction of a turn in f64: exact
+ * to 2^-53 of the position whatever its size; sine and cosine in f32).  axis: int32 [pairs], each in [0, axes).  pos: int32 or
+ * (pos_f32) f32 [N][axes], pos_bs elements between pictures (0: the same for all).  x16 or (x_f32) f32 heads.  q / k may be
+ * transformed in place (qo == q with the same strides); kh = 0: no keys.
+ * Returns -1 for a missing pointer, -2 for sizes or strides. */
+typedef struct onedc_rotary_params {
+    const void *q; void *qo; const void *k; void *ko; const void *pos; const double *turns; const int32_t *axis;
+    int32_t B, N, D, pairs, axes, qh, kh;
+    int32_t q_cs, q_co, qo_cs, qo_co, k_cs, k_co, ko_cs, ko_co;
+    int32_t x_f32, pos_f32, neighbours, inverse;
+    int64_t pos_bs;
+} onedc_rotary_params;
+int onedc_rotary_axes(const onedc_rotary_params *p, void *stream);
+
+/* 4-bit microscaled floating point (OCP MX v1.0, MXFP4): blocks of 32 consecutive values of a row share a power of two 2^(s - 127),
+ * values are e2m1 (0 .5 1 1.5 2 3 4 6 and sign).  A matrix of `rows` rows of K values is held as
+ *   codes  [rows][Kp / 2]   two codes a byte, the lower half first        Kp = K rounded up to 128, padding codes are 0
+ *   scales [rows][Kp / 32]  the bytes s; 255: the block is NaN
+ * which is what v_mfma_scale_f32_16x16x128_f8f6f4 takes per lane: 16 bytes of codes and one scale byte.
+ *   quantize   s - 127 = max(floor(log2 amax) - 2, -127); values times 2^-(s - 127) rounded to the nearest code, ties to the even
+ *              code, magnitudes over 6 to 6; a block with a NaN or an infinity becomes NaN.  x: 16-bit or (x_f32) f32 rows of K
+ *              channels, stride x_cs, offset x_co
+ *   dequantize the values, rounded once to y's type
+ * Returns -1 for a missing pointer, -2 for sizes, strides or a code pointer that is not 16-byte aligned (scales: 4-byte). */
+int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream);
+int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y_f32, int y_cs, int y_co, int64_t rows, int K,
+                           void *stream);
+/* Product of two such matrices along K with the epilogues of onedc_conv_gemm:
+ *   y[m][n] = act(alpha * sum_k x[m][k] w[n][k] + bias[n]) + res[m][n]
+ * products exact, sums in f32, one rounding to y's type (16-bit or y_f32).  epi: ONEDC_EPI_LINEAR, _LEAKY (slope), _SILU, or _GEGLU,
+ * where rows of w come in blocks of 16, values in front of their gates, N % 32 == 0, y and res have N / 2 channels.  res has y's type.
+ * x: either (xc, xs) as above, or, xc NULL, raw rows xr (16-bit or xr_f32, stride xr_cs, offset xr_co) that are quantised on the way:
+ * only for M <= ONEDC_MXFP4_ROWS_RAW, without scratch.  M may be 0.
+ * Returns -1 for a missing pointer, -2 for sizes, strides or alignment, -3 for an epilogue it does not know or a GEGLU layer with
+ * N % 32, -4 for raw rows with M > ONEDC_MXFP4_ROWS_RAW. */
+#define ONEDC_MXFP4_ROWS_RAW 16
+typedef struct onedc_mxfp4_params {
+    const void *xc; const void *xs; const void *xr; const void *wc; const void *ws; const float *bias; const void *res; void *y;
+    int64_t M;
+    int32_t N, K;
+    int32_t xr_cs, xr_co, xr_f32, y_cs, y_co, r_cs, r_co, y_f32, epi;
+    float alpha, slope;
+} onedc_mxfp4_params;
+int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream);
+
 /* sinusoidal timestep embedding, flip_sin_to_cos, shift 0 (decoder_unet.py:138): f32 [n][dim] */
 int onedc_timestep_embedding(const float *t, float *emb, int n, int dim, void *stream);
 /* y = a + b (bf16), used where a residual cannot ride on a GEMM epilogue */

@@ -104,6 +104,33 @@ class XAttnParams(C.Structure):
     ]
 
 
+class BlockNormParams(C.Structure):
+    """onedc_block_norm_params of include/onedc_hip.h."""
+    _fields_ = [(n, _P) for n in ("x", "f", "xo", "y", "post_w", "post_b", "gate", "w", "b", "scale", "shift")] + [
+        (n, C.c_int32) for n in ("B", "N", "C", "x_cs", "x_co", "f_cs", "f_co", "xo_cs", "xo_co", "y_cs", "y_co", "gate_rs", "scale_rs",
+                                 "shift_rs", "kind", "post", "x_f32", "f_f32")] + [("alpha", _F), ("eps", _F)]
+
+
+class BlockNormGrad(C.Structure):
+    """onedc_block_norm_grad of include/onedc_hip.h."""
+    _fields_ = [(n, _P) for n in ("dy", "dxo", "dx", "df", "d_post_w", "d_post_b", "d_gate", "d_w", "d_b", "d_scale", "d_shift", "ws")] + [
+        ("ws_bytes", _L)] + [(n, C.c_int32) for n in ("dy_cs", "dy_co", "dxo_cs", "dxo_co", "dx_cs", "dx_co", "df_cs", "df_co")]
+
+
+class RotaryParams(C.Structure):
+    """onedc_rotary_params of include/onedc_hip.h."""
+    _fields_ = [(n, _P) for n in ("q", "qo", "k", "ko", "pos", "turns", "axis")] + [
+        (n, C.c_int32) for n in ("B", "N", "D", "pairs", "axes", "qh", "kh", "q_cs", "q_co", "qo_cs", "qo_co", "k_cs", "k_co", "ko_cs",
+                                 "ko_co", "x_f32", "pos_f32", "neighbours", "inverse")] + [("pos_bs", _L)]
+
+
+class MxFp4Params(C.Structure):
+    """onedc_mxfp4_params of include/onedc_hip.h."""
+    _fields_ = [(n, _P) for n in ("xc", "xs", "xr", "wc", "ws", "bias", "res", "y")] + [("M", _L)] + [
+        (n, C.c_int32) for n in ("N", "K", "xr_cs", "xr_co", "xr_f32", "y_cs", "y_co", "r_cs", "r_co", "y_f32", "epi")] + [
+        ("alpha", _F), ("slope", _F)]
+
+
 SIGNATURES = {
     "onedc_conv_gemm": (_I, [C.POINTER(ConvParams), _P]),
     "onedc_conv_win_takes": (_I, [C.POINTER(ConvParams)]),
@@ -148,6 +175,13 @@ SIGNATURES = {
     "onedc_ref_conv3x3": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
     "onedc_ref_conv3x3_im2col": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P]),
     "onedc_ref_prior_indexes": (_I, [_P, _P, _I, _P, _I, _I, _I, _I, _I, _P]),
+    "onedc_block_norm": (_I, [C.POINTER(BlockNormParams), _P]),
+    "onedc_block_norm_backward": (_I, [C.POINTER(BlockNormParams), C.POINTER(BlockNormGrad), _P]),
+    "onedc_block_norm_backward_ws_bytes": (_L, [C.POINTER(BlockNormParams), C.POINTER(BlockNormGrad)]),
+    "onedc_rotary_axes": (_I, [C.POINTER(RotaryParams), _P]),
+    "onedc_mxfp4_quantize": (_I, [_P, _I, _I, _I, _P, _P, _L, _I, _P]),
+    "onedc_mxfp4_dequantize": (_I, [_P, _P, _P, _I, _I, _I, _L, _I, _P]),
+    "onedc_mxfp4_linear": (_I, [C.POINTER(MxFp4Params), _P]),
     "onedc_add": (_I, [_P, _P, _P, _L, _P]),
     "onedc_hip_version": (C.c_char_p, []),
     "onedc_hip_abi_version": (_I, []),
@@ -719,4 +753,337 @@ def timestep_embedding(t, emb):
 
 def add(a, b, y):
     _ok(lib().onedc_add(a.data_ptr(), b.data_ptr(), y.data_ptr(), y.numel(), stream()), "onedc_add")
+    return y
+
+
+# ---- transformer-block operators for image / video tokens ---------------------------------------------------------------------------
+# Views hold the tokens as pixels: B pictures (clips), H * W tokens each, C channels.  Unlike the wrappers above these check every
+# tensor against what the kernels address before they launch, and say what is wrong.
+
+NORM_LAYER, NORM_RMS = 0, 1
+
+
+def _check_view(what, name, v, like=None, channels=None, dtypes=None):
+    """A View whose rows lie inside its buffer; the same tokens as `like`, `channels` wide, of one of `dtypes`."""
+    n = v.B * v.H * v.W
+    if min(v.B, v.H, v.W) < 0 or v.C < 1 or v.co < 0 or v.co + v.C > v.cs or not v.t.is_contiguous() or (
+            n and (n - 1) * v.cs + v.co + v.C > v.t.numel()):
+        raise KernelError(f"{what}: {name} is a view outside its buffer ({v.B} x {v.H} x {v.W} rows, channels {v.co}..{v.co + v.C} of {v.cs}, "
+                          f"{v.t.numel()} values{'' if v.t.is_contiguous() else ', not contiguous'})")
+    if like is not None and (v.B, v.H * v.W) != (like.B, like.H * like.W):
+        raise KernelError(f"{what}: {name} has {v.B} x {v.H * v.W} rows, not {like.B} x {like.H * like.W}")
+    if channels is not None and v.C != channels:
+        raise KernelError(f"{what}: {name} has {v.C} channels, not {channels}")
+    if dtypes is not None and v.t.dtype not in dtypes:
+        raise KernelError(f"{what}: {name} is {v.t.dtype}, not {' or '.join(str(d) for d in dtypes)} (current format: {act()})")
+
+
+def _check_device(what, *tensors):
+    """Every tensor on the device whose current stream the launch goes to."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type == "cuda" and here is None:
+            here = torch.cuda.current_device()
+        if t.device.type != "cuda" or t.device.index != here:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the launch goes to {'no GPU' if here is None else f'cuda:{here}'} "
+                              "(torch.cuda.device selects it)")
+
+
+def _overlap(a, b):
+    """Whether two views share a value: their address ranges meet, and they are not different channels of rows of one pitch."""
+    ea, eb = a.t.element_size(), b.t.element_size()
+    a0, b0 = a.ptr + a.co * ea, b.ptr + b.co * eb
+    na, nb = a.B * a.H * a.W, b.B * b.H * b.W
+    if not na or not nb or a0 + ((na - 1) * a.cs + a.C) * ea <= b0 or b0 + ((nb - 1) * b.cs + b.C) * eb <= a0:
+        return False
+    pitch = a.cs * ea
+    if pitch != b.cs * eb:
+        return True
+    d = (b0 - a0) % pitch                             # where b's channels begin inside a's rows
+    return d < a.C * ea or d + b.C * eb > pitch
+
+
+def _same(a, b):
+    return a.ptr == b.ptr and a.cs == b.cs and a.co == b.co and a.t.dtype == b.t.dtype
+
+
+def _check_apart(what, name, out, *others):
+    """Nothing that the launch reads or writes elsewhere lies under `out`."""
+    for o in others:
+        if o is not None and _overlap(out, o):
+            raise KernelError(f"{what}: {name} shares memory with another operand")
+
+
+def _check_vector(what, name, t, n):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+        raise KernelError(f"{what}: {name} must be {n} contiguous f32 values, not {tuple(t.shape)} {t.dtype}")
+
+
+def _row_stride(what, name, t, B, Cc):
+    """Floats between the pictures' rows of a [B, C] parameter; 0: one row ([C] or [1, C]) for all pictures."""
+    if t is None:
+        return 0
+    if t.dtype == torch.float32 and t.dim() in (1, 2) and t.shape[-1] == Cc and (Cc == 1 or t.stride(-1) == 1):
+        if t.dim() == 1 or t.shape[0] == 1:
+            return 0
+        if t.shape[0] == B and Cc <= t.stride(0) < 2 ** 31:
+            return t.stride(0)
+    raise KernelError(f"{what}: {name} must be f32 [{Cc}] or [{B}, {Cc}] with dense rows, not {tuple(t.shape)} {t.dtype} strides {t.stride()}")
+
+
+def _block_norm_params(what, x, f, y_dtype, kind, eps, post, post_w, post_b, gate, alpha, w, b, scale, shift, has_y):
+    if kind not in (NORM_LAYER, NORM_RMS):
+        raise KernelError(f"{what}: kind must be NORM_LAYER or NORM_RMS, not {kind!r}")
+    _check_view(what, "x", x, dtypes=(a16(), torch.float32))
+    if x.B * x.H * x.W > 0x7fffffff or x.C > 1 << 20:
+        raise KernelError(f"{what}: {x.B * x.H * x.W} rows of {x.C} channels are more than the kernel indexes")
+    if f is not None:
+        _check_view(what, "f", f, x, x.C, (a16(), torch.float32) if x.f32 else (a16(),))
+        if y_dtype is not None and f.t.dtype != y_dtype:
+            raise KernelError(f"{what}: f is {f.t.dtype}, the normalised side {y_dtype}: one type")
+    elif post or gate is not None:
+        raise KernelError(f"{what}: a post norm or a gate needs f")
+    if (post_w is not None or post_b is not None) and not post:
+        raise KernelError(f"{what}: post_w / post_b need post=True")
+    if not has_y and any(t is not None for t in (w, b, scale, shift)):
+        raise KernelError(f"{what}: w, b, scale and shift belong to the norm behind the join, which this call has not")
+    for name, t in (("post_w", post_w), ("post_b", post_b), ("w", w), ("b", b)):
+        _check_vector(what, name, t, x.C)
+    p = BlockNormParams(x.ptr, None if f is None else f.ptr, None, None, _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale),
+                        _ptr(shift), x.B, x.H * x.W, x.C, x.cs, x.co, 0 if f is None else f.cs, 0 if f is None else f.co, 0, 0, 0, 0,
+                        _row_stride(what, "gate", gate, x.B, x.C), _row_stride(what, "scale", scale, x.B, x.C),
+                        _row_stride(what, "shift", shift, x.B, x.C), kind, int(bool(post)), int(x.f32),
+                        int(f.f32 if f is not None else y_dtype == torch.float32), alpha, eps)
+    return p
+
+
+def block_norm(x, y=None, *, f=None, xo=None, kind=NORM_LAYER, eps=1e-5, post=False, post_w=None, post_b=None, gate=None, alpha=1.0,
+               w=None, b=None, scale=None, shift=None):
+    """The join between two sub-blocks of a transformer block in one launch:
+        t = x + alpha * gate * P(f),  P = norm(f) * post_w + post_b with post=True, else f;  xo = t;
+        y = (norm(t) * w + b) * (1 + scale) + shift
+    without f (and xo): y of x itself; without y: the join alone.  x, xo: Views in the current 16-bit format or f32 (the residual
+    stream); f, y: Views in the current format, or f32 where x is.  xo may be x.  post_w, post_b, w, b: f32 [C]; gate, scale, shift:
+    f32 [B, C] (rows may be slices of one wide modulation tensor) or [C], one row for all pictures.  Returns (xo, y)."""
+    what = "block_norm"
+    if y is None and xo is None:
+        raise KernelError(f"{what}: neither y nor xo: nothing to compute")
+    if (f is None) != (xo is None):
+        raise KernelError(f"{what}: f and xo come together (the branch and the joined stream)")
+    p = _block_norm_params(what, x, f, None if y is None else y.t.dtype, kind, eps, post, post_w, post_b, gate, alpha, w, b, scale, shift,
+                           y is not None)
+    if y is not None:
+        _check_view(what, "y", y, x, x.C, (a16(), torch.float32) if x.f32 else (a16(),))
+        _check_apart(what, "y", y, x, f, xo)
+        p.y, p.y_cs, p.y_co = y.ptr, y.cs, y.co
+    if xo is not None:
+        _check_view(what, "xo", xo, x, x.C, (x.t.dtype,))
+        _check_apart(what, "xo", xo, None if _same(xo, x) else x, f)
+        p.xo, p.xo_cs, p.xo_co = xo.ptr, xo.cs, xo.co
+    _check_device(what, *(v.t for v in (x, f, xo, y) if v is not None), post_w, post_b, gate, w, b, scale, shift)
+    _ok(lib().onedc_block_norm(C.byref(p), stream()), "onedc_block_norm")
+    return xo, y
+
+
+def block_norm_backward(x, dy, dx=None, *, dxo=None, f=None, df=None, kind=NORM_LAYER, eps=1e-5, post=False, post_w=None, post_b=None,
+                        gate=None, alpha=1.0, w=None, b=None, scale=None, shift=None, d_post_w=None, d_post_b=None, d_gate=None, d_w=None,
+                        d_b=None, d_scale=None, d_shift=None):
+    """Backward pass of block_norm.  x: the JOINED stream as block_norm stored it (its xo; its x where there was no f); dy, dxo: the
+    gradients of y and xo, None where the loss does not depend on them.  Writes dx (the gradient of the stream in front of the join), df, and
+    the parameter gradients that are asked for, f32, dense: [C], and [B, C] for gate / scale / shift where those have a row per picture.
+    dx may be dxo, df may be dy.  Sums over rows run in a fixed order: the same bits every time."""
+    what = "block_norm_backward"
+    if dy is None and dxo is None:
+        raise KernelError(f"{what}: neither dy nor dxo: no gradient to pass on")
+    p = _block_norm_params(what, x, f, dy.t.dtype if dy is not None else None if df is None else df.t.dtype, kind, eps, post, post_w, post_b,
+                           gate, alpha, w, b, scale, shift, dy is not None)
+    side = (a16(), torch.float32) if x.f32 else (a16(),)
+    g = BlockNormGrad()
+    if f is None and any(t is not None for t in (df, d_gate, d_post_w, d_post_b)):
+        raise KernelError(f"{what}: df, d_gate, d_post_w and d_post_b need f")
+    for name, v, dtypes in (("dy", dy, side), ("dxo", dxo, (x.t.dtype,)), ("dx", dx, (x.t.dtype,)), ("df", df, side)):
+        if v is not None:
+            _check_view(what, name, v, x, x.C, dtypes)
+            setattr(g, name, v.ptr)
+            setattr(g, name + "_cs", v.cs)
+            setattr(g, name + "_co", v.co)
+    if dx is not None:
+        _check_apart(what, "dx", dx, x, f, dy, df, None if dxo is None or _same(dx, dxo) else dxo)
+    if df is not None:
+        _check_apart(what, "df", df, x, f, dxo, None if dy is None or _same(df, dy) else dy)
+    grads = (("d_post_w", d_post_w, post_w, 0), ("d_post_b", d_post_b, post_b, 0), ("d_gate", d_gate, gate, p.gate_rs), ("d_w", d_w, w, 0),
+             ("d_b", d_b, b, 0), ("d_scale", d_scale, scale, p.scale_rs), ("d_shift", d_shift, shift, p.shift_rs))
+    for name, t, of, rs in grads:
+        if t is not None:
+            if of is None:
+                raise KernelError(f"{what}: {name} of a parameter that the call has not")
+            _check_vector(what, name, t, x.C * (x.B if rs else 1))
+            setattr(g, name, t.data_ptr())
+    _check_device(what, *(v.t for v in (x, f, dy, dxo, dx, df) if v is not None), post_w, post_b, gate, w, b, scale, shift,
+                  *(t for _, t, _, _ in grads))
+    need = lib().onedc_block_norm_backward_ws_bytes(C.byref(p), C.byref(g))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=x.t.device)          # the call's own: two captured graphs never share it
+        g.ws, g.ws_bytes = ws.data_ptr(), need
+    _ok(lib().onedc_block_norm_backward(C.byref(p), C.byref(g), stream()), "onedc_block_norm_backward")
+    return dx, df
+
+
+class RotaryAxes:
+    """The plan of rotary_axes for heads of D dims: sections[a] dims (even) of every head turn with axis a, dims past their sum pass
+    through.  Pair frequencies: theta ** (-2 j / sections[a]) for pair j of axis a, or, shared_spectrum, theta ** (-2 i / sum) for pair i of
+    the whole head, the axes taking their sections of it in order.  theta: one base, or one per axis (not with shared_spectrum).
+    neighbours: pairs are (2 i, 2 i + 1) instead of (i, i + pairs)."""
+
+    def __init__(self, D, sections, theta=10000.0, neighbours=False, shared_spectrum=False, device="cuda:0"):
+        sections = tuple(int(n) for n in sections)
+        if not 1 <= D <= 4096 or not 1 <= len(sections) <= 16 or any(n < 0 or n % 2 for n in sections) or sum(sections) > D:
+            raise KernelError(f"RotaryAxes: sections {sections} are not even parts of a head of {D} dims")
+        bases = tuple(float(t) for t in (theta if isinstance(theta, (tuple, list)) else (theta,) * len(sections)))
+        if len(bases) != len(sections) or any(not t > 0 for t in bases) or (shared_spectrum and len(set(bases)) > 1):
+            raise KernelError(f"RotaryAxes: theta {theta} does not fit {len(sections)} axes")
+        self.D, self.sections, self.neighbours, self.shared_spectrum = D, sections, bool(neighbours), bool(shared_spectrum)
+        self.pairs, self.axes = sum(sections) // 2, len(sections)
+        if shared_spectrum:
+            freq = bases[0] ** (-torch.arange(self.pairs, dtype=torch.float64) / max(self.pairs, 1))
+        else:
+            freq = torch.cat([t ** (-2.0 * torch.arange(n // 2, dtype=torch.float64) / max(n, 1)) for n, t in zip(sections, bases)])
+        axis = torch.cat([torch.full((n // 2,), a, dtype=torch.int32) for a, n in enumerate(sections)])
+        pad = torch.zeros(1, dtype=torch.float64)                             # (never empty: a plan without pairs still has addresses)
+        self.turns = torch.cat([freq / (2.0 * 3.141592653589793), pad]).to(device)
+        self.axis = torch.cat([axis, pad.to(torch.int32)]).to(device)
+
+
+def rotary_axes(plan, pos, q, qo=None, k=None, ko=None, inverse=False):
+    """Turn queries q and keys k (Views of heads * D channels, heads back to back; 16-bit or f32) by their tokens' positions, in one
+    launch.  pos: int32 or f32 [N, axes], or [B, N, axes] with other positions per picture.  qo / ko None: in place.  k may have
+    fewer heads than q, or be None.  inverse: turn back -- the backward pass.  Returns (qo, ko)."""
+    what = "rotary_axes"
+    if k is None and ko is not None:
+        raise KernelError(f"{what}: ko without k")
+    qo = q if qo is None else qo
+    ko = k if ko is None else ko
+    _check_view(what, "q", q, dtypes=(a16(), torch.float32))
+    for name, v, like in (("qo", qo, q), ("k", k, q), ("ko", ko, q)):
+        if v is not None:
+            _check_view(what, name, v, like, None if name == "k" else (q if name == "qo" else k).C, (q.t.dtype,))
+    for name, v in (("q", q), ("k", k)):
+        if v is not None and (v.C % plan.D or v.C // plan.D > 4096):
+            raise KernelError(f"{what}: {name} has {v.C} channels: not 1 to 4096 heads of {plan.D}")
+    N = q.H * q.W
+    if q.B * N > 0x7fffffff:
+        raise KernelError(f"{what}: {q.B * N} rows are more than the kernel indexes")
+    if pos.dtype not in (torch.int32, torch.float32) or not pos.is_contiguous() or tuple(pos.shape) not in (
+            (N, plan.axes), (1, N, plan.axes), (q.B, N, plan.axes)):
+        raise KernelError(f"{what}: pos must be contiguous int32 or f32 [{N}, {plan.axes}] or [{q.B}, {N}, {plan.axes}], not "
+                          f"{tuple(pos.shape)} {pos.dtype}")
+    _check_apart(what, "qo", qo, None if _same(qo, q) else q, k, ko)
+    if k is not None:
+        _check_apart(what, "ko", ko, None if _same(ko, k) else k, q)
+    _check_device(what, q.t, qo.t, *(v.t for v in (k, ko) if v is not None), pos, plan.turns, plan.axis)
+    p = RotaryParams(q.ptr, qo.ptr, None if k is None else k.ptr, None if k is None else ko.ptr, pos.data_ptr(), plan.turns.data_ptr(),
+                     plan.axis.data_ptr(), q.B, N, plan.D, plan.pairs, plan.axes, q.C // plan.D, 0 if k is None else k.C // plan.D, q.cs, q.co,
+                     qo.cs, qo.co, 0 if k is None else k.cs, 0 if k is None else k.co, 0 if k is None else ko.cs, 0 if k is None else ko.co,
+                     int(q.f32), int(pos.dtype == torch.float32), int(plan.neighbours), int(bool(inverse)),
+                     N * plan.axes if pos.dim() == 3 and pos.shape[0] > 1 else 0)
+    _ok(lib().onedc_rotary_axes(C.byref(p), stream()), "onedc_rotary_axes")
+    return qo, ko
+
+
+class MxFp4:
+    """A matrix of `rows` rows of K values in 4-bit microscaled floating point (include/onedc_hip.h): codes uint8 [rows][Kp / 2], scales
+    uint8 [rows][Kp / 32], Kp = K rounded up to 128 with zero codes behind K."""
+    __slots__ = ("codes", "scales", "rows", "K")
+
+    def __init__(self, codes, scales, rows, K):
+        kp = (K + 127) // 128 * 128
+        if K < 1 or rows < 0 or K > 1 << 24 or rows > 0x7fffffff:
+            raise KernelError(f"MxFp4: no matrix of {rows} rows of {K} values")
+        for name, t, n in (("codes", codes, kp // 2), ("scales", scales, kp // 32)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (rows, n) or not t.is_contiguous():
+                raise KernelError(f"MxFp4: {name} must be contiguous uint8 [{rows}, {n}], not {tuple(t.shape)} {t.dtype}")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            raise KernelError("MxFp4: codes must be 16-byte aligned, scales 4-byte")
+        self.codes, self.scales, self.rows, self.K = codes, scales, rows, K
+
+
+def mxfp4_empty(rows, K, device):
+    kp = (K + 127) // 128 * 128
+    return MxFp4(torch.empty(rows, kp // 2, dtype=torch.uint8, device=device), torch.empty(rows, kp // 32, dtype=torch.uint8, device=device),
+                 rows, K)
+
+
+def mxfp4_quantize(x, q=None):
+    """x: View (16-bit or f32), its rows (tokens) quantised along the channels into q (default: a new MxFp4).  A block of 32 with a NaN
+    or an infinity reads back as NaN."""
+    what = "mxfp4_quantize"
+    _check_view(what, "x", x, dtypes=(a16(), torch.float32))
+    rows = x.B * x.H * x.W
+    if q is None:
+        q = mxfp4_empty(rows, x.C, x.t.device)
+    elif (q.rows, q.K) != (rows, x.C):
+        raise KernelError(f"{what}: q holds {q.rows} x {q.K} values, x has {rows} x {x.C}")
+    _check_device(what, x.t, q.codes, q.scales)
+    if rows:
+        _ok(lib().onedc_mxfp4_quantize(x.ptr, int(x.f32), x.cs, x.co, q.codes.data_ptr(), q.scales.data_ptr(), rows, x.C, stream()),
+            "onedc_mxfp4_quantize")
+    return q
+
+
+def mxfp4_dequantize(q, y):
+    """The values that q stands for, into the View y (16-bit, rounded, or f32, exact)."""
+    what = "mxfp4_dequantize"
+    _check_view(what, "y", y, channels=q.K, dtypes=(a16(), torch.float32))
+    if y.B * y.H * y.W != q.rows:
+        raise KernelError(f"{what}: y has {y.B * y.H * y.W} rows, q {q.rows}")
+    _check_device(what, y.t, q.codes, q.scales)
+    if q.rows:
+        _ok(lib().onedc_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), y.ptr, int(y.f32), y.cs, y.co, q.rows, q.K, stream()),
+            "onedc_mxfp4_dequantize")
+    return y
+
+
+MXFP4_ROWS_RAW = 16        # ONEDC_MXFP4_ROWS_RAW of include/onedc_hip.h (tests/test_token_ops.py compares)
+
+
+def mxfp4_linear(x, w, bias, y, *, epi=EPI_LINEAR, slope=0.01, alpha=1.0, res=None):
+    """y = act(alpha * x w^T + bias) + res with both operands in 4 bits.  x: a View (16-bit or f32; quantised on the way -- in the same
+    launch up to MXFP4_ROWS_RAW rows) or an MxFp4; w: MxFp4 of N rows (pack.pack_mxfp4); bias: f32 [N] or None; y, res: Views of one
+    type (16-bit or f32), N channels, N / 2 for EPI_GEGLU (rows of w in blocks of 16, values in front of gates: pack.glu_perm).
+    res may be y."""
+    what = "mxfp4_linear"
+    if epi not in (EPI_LINEAR, EPI_LEAKY, EPI_SILU, EPI_GEGLU):
+        raise KernelError(f"{what}: epilogue {epi!r} is not one of LINEAR, LEAKY, SILU, GEGLU")
+    if epi == EPI_GEGLU and w.rows % 32:
+        raise KernelError(f"{what}: a gated layer needs whole blocks of 16 values and 16 gates, not {w.rows} rows")
+    held = isinstance(x, MxFp4)
+    rows, kx = (x.rows, x.K) if held else (x.B * x.H * x.W, x.C)
+    if not held:
+        _check_view(what, "x", x, dtypes=(a16(), torch.float32))
+    if kx != w.K:
+        raise KernelError(f"{what}: x has {kx} values a row, w {w.K}")
+    out = w.rows // 2 if epi == EPI_GEGLU else w.rows
+    if out < 1 or w.rows > 1 << 24:
+        raise KernelError(f"{what}: no layer of {w.rows} outputs")
+    _check_view(what, "y", y, channels=out, dtypes=(a16(), torch.float32))
+    if y.B * y.H * y.W != rows:
+        raise KernelError(f"{what}: y has {y.B * y.H * y.W} rows, x {rows}")
+    _check_vector(what, "bias", bias, w.rows)
+    if res is not None:
+        _check_view(what, "res", res, y, out, (y.t.dtype,))
+        _check_apart(what, "y", y, None if _same(y, res) else res)
+    if not held:
+        _check_apart(what, "y", y, x)
+    _check_device(what, *((x.codes, x.scales) if held else (x.t,)), w.codes, w.scales, y.t, bias, None if res is None else res.t)
+    if not rows:
+        return y
+    if not held and rows > MXFP4_ROWS_RAW:
+        x, held = mxfp4_quantize(x), True
+    p = MxFp4Params(x.codes.data_ptr() if held else None, x.scales.data_ptr() if held else None, None if held else x.ptr, w.codes.data_ptr(),
+                    w.scales.data_ptr(), _ptr(bias), None if res is None else res.ptr, y.ptr, rows, w.rows, w.K, 0 if held else x.cs,
+                    0 if held else x.co, 0 if held else int(x.f32), y.cs, y.co, 0 if res is None else res.cs, 0 if res is None else res.co,
+                    int(y.f32), epi, alpha, slope)
+    _ok(lib().onedc_mxfp4_linear(C.byref(p), stream()), "onedc_mxfp4_linear")
     return y

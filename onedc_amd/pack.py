@@ -49,6 +49,15 @@ def pack_matrix(w2d, device, row_perm=None, dtype=None):
     return _pad_rows(w2d.contiguous()).to(dtype).to(device).contiguous()
 
 
+def pack_mxfp4(w2d, device, row_perm=None):
+    """[rows][K] f32 -> kernels.MxFp4 on `device`, the weight operand of kernels.mxfp4_linear (no row padding: the kernel knows N)."""
+    from . import kernels
+    if row_perm is not None:
+        w2d = w2d[row_perm]
+    w = w2d.float().contiguous().to(device)
+    return kernels.mxfp4_quantize(kernels.View(w, 1, 1, w.shape[0], w.shape[1]))
+
+
 SPLIT16_SCALE = 2048.0          # 2^11: the low half of a split operand is stored times this (csrc/gemm_conv.hip, SPLIT)
 
 
