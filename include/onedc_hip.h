@@ -439,7 +439,8 @@ int onedc_rotary_axes(const onedc_rotary_params *p, void *stream);
  *              code, magnitudes over 6 to 6; a block with a NaN or an infinity becomes NaN.  x: 16-bit or (x_f32) f32 rows of K
  *              channels, stride x_cs, offset x_co
  *   dequantize the values, rounded once to y's type
- * Returns -1 for a missing pointer, -2 for sizes, strides or a code pointer that is not 16-byte aligned (scales: 4-byte). */
+ * Returns -1 for a missing pointer, -2 for sizes (K up to ONEDC_MXFP4_MAX_K), strides or a code
+ * pointer that is not 16-byte aligned (scales: 4-byte). */
 int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream);
 int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y_f32, int y_cs, int y_co, int64_t rows, int K,
                            void *stream);
@@ -452,6 +453,7 @@ int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y
  * Returns -1 for a missing pointer, -2 for sizes, strides or alignment, -3 for an epilogue it does not know or a GEGLU layer with
  * N % 32, -4 for raw rows with M > ONEDC_MXFP4_ROWS_RAW. */
 #define ONEDC_MXFP4_ROWS_RAW 16
+#define ONEDC_MXFP4_MAX_K (1 << 22)
 typedef struct onedc_mxfp4_params {
     const void *xc; const void *xs; const void *xr; const void *wc; const void *ws; const float *bias; const void *res; void *y;
     int64_t M;

@@ -999,7 +999,7 @@ class MxFp4:
 
     def __init__(self, codes, scales, rows, K):
         kp = (K + 127) // 128 * 128
-        if K < 1 or rows < 0 or K > 1 << 24 or rows > 0x7fffffff:
+        if not 1 <= K <= 1 << 22 or not 0 <= rows <= 0x7fffffff:
             raise KernelError(f"MxFp4: no matrix of {rows} rows of {K} values")
         for name, t, n in (("codes", codes, kp // 2), ("scales", scales, kp // 32)):
             if t.dtype != torch.uint8 or tuple(t.shape) != (rows, n) or not t.is_contiguous():
