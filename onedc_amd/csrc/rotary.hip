@@ -4,47 +4,155 @@
 //
 // The angle is kept in turns: phase = pos * turns[i] in f64, minus its nearest whole number, so that positions of any size lose
 // nothing; sine and cosine of the remaining half turn in f32.
+//
+// Bound by HBM: q and k are read and written once, 3 operations an element.  What has to stay off that path are the angles: a
+// workgroup computes the sines and cosines of its T tokens once, into LDS, and all heads of those tokens read them from there (neighbouring
+// lanes hold neighbouring heads, so most of a wave's LDS reads are one address).
+#include "conv_common.h"
 #include "elem.h"
 
 namespace {
 
-// cosine and sine of the angle of pair i at token n of picture b
-__device__ __forceinline__ float2 phase(const onedc_rotary_params &p, int64_t b, int n, int i) {
-    const int64_t at = b * p.pos_bs + (int64_t)n * p.axes + p.axis[i];
-    const double pos = p.pos_f32 ? (double)((const float *)p.pos)[at] : (double)((const int32_t *)p.pos)[at];
-    const double t = pos * p.turns[i];
-    float s, c;
-    sincospif(2.f * (float)(t - rint(t)), &s, &c);
-    return make_float2(c, p.inverse ? -s : s);
-}
+constexpr int NT = 256;
+constexpr int MAX_TABLE = 8192;           // pairs of sine and cosine in LDS: 64 KB
 
-// one thread per (token, head, pair or passed-through dim)
+// VEC values at p as f32
+template <bool F32, int VEC>
+struct Piece {
+    typedef typename Elem<F32>::T T;
+    typedef __attribute__((ext_vector_type(VEC))) T V;
+    V v;
+    __device__ __forceinline__ void load(const T *p) { v = *(const V *)p; }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (F32) return v[i];
+        else return a2f(v[i]);
+    }
+    __device__ __forceinline__ void set(int i, float a, float b) {       // values i, i + 1
+        if constexpr (F32) {
+            v[i] = a;
+            v[i + 1] = b;
+        } else {
+            const uint32_t w = pack_a2(a, b);
+            v[i] = (T)(w & 0xffffu);
+            v[i + 1] = (T)(w >> 16);
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const { *(V *)p = v; }
+};
 template <bool F32>
-__global__ __launch_bounds__(256) void rotary_kernel(onedc_rotary_params p) {
-    typedef Elem<F32> E;
-    const int heads = p.qh + p.kh, per = p.D - p.pairs;
-    const int64_t total = (int64_t)p.B * p.N * heads * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t th = i / per;
-        const int j = (int)(i - th * per);
-        const int64_t row = th / heads;
-        const int h = (int)(th - row * heads);
+struct Piece<F32, 1> {
+    typedef typename Elem<F32>::T T;
+    T v;
+    __device__ __forceinline__ void load(const T *p) { v = *p; }
+    __device__ __forceinline__ float get(int) const { return Elem<F32>::get(&v); }
+    __device__ __forceinline__ void set1(float a) { Elem<F32>::put(&v, a); }
+    __device__ __forceinline__ void store(T *p) const { *p = v; }
+};
+
+// A token's heads are cut into units of VEC values: `turn` units a head that turn (two pieces each with pairs of halves, one with pairs of
+// neighbours), then the pieces that pass through.
+struct Units {
+    int turn, per, T;                     // turning units and all units of a head; tokens of a workgroup
+    OnedcFastDiv by_unit, by_head, by_pair;
+};
+
+template <bool F32, int VEC, bool NEIGHBOURS>
+__global__ __launch_bounds__(NT) void rotary_kernel(onedc_rotary_params p, Units u) {
+    typedef typename Elem<F32>::T T;
+    extern __shared__ __attribute__((aligned(16))) float table[];         // [T][pairs] cosines, then sines
+    const int64_t row0 = (int64_t)blockIdx.x * u.T;
+    const int64_t rows = (int64_t)p.B * p.N;
+    const int tokens = (int)(rows - row0 < u.T ? rows - row0 : u.T);
+    float *const cosines = table, *const sines = table + u.T * p.pairs;
+
+    for (int i = threadIdx.x; i < tokens * p.pairs; i += NT) {
+        const int t = u.by_pair.div(i), j = i - t * p.pairs;
+        const int64_t row = row0 + t, b = row / p.N;
+        const int64_t at = b * p.pos_bs + (row - b * p.N) * p.axes + p.axis[j];
+        const double pos = p.pos_f32 ? (double)((const float *)p.pos)[at] : (double)((const int32_t *)p.pos)[at];
+        const double turn = pos * p.turns[j];
+        float s, c;
+        sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
+        cosines[i] = c;
+        sines[i] = p.inverse ? -s : s;
+    }
+    __syncthreads();
+
+    const int heads = p.qh + p.kh, total = tokens * heads * u.per;
+    for (int i = threadIdx.x; i < total; i += NT) {
+        const int th = u.by_unit.div(i), unit = i - th * u.per;
+        const int t = u.by_head.div(th), h = th - t * heads;
+        const int64_t row = row0 + t;
         const bool isq = h < p.qh;
-        const typename E::T *src = isq ? (const typename E::T *)p.q + row * p.q_cs + p.q_co + h * p.D
-                                       : (const typename E::T *)p.k + row * p.k_cs + p.k_co + (h - p.qh) * p.D;
-        typename E::T *dst = isq ? (typename E::T *)p.qo + row * p.qo_cs + p.qo_co + h * p.D
-                                 : (typename E::T *)p.ko + row * p.ko_cs + p.ko_co + (h - p.qh) * p.D;
-        if (j >= p.pairs) {
-            dst[p.pairs + j] = src[p.pairs + j];
+        const T *src = isq ? (const T *)p.q + row * p.q_cs + p.q_co + h * p.D : (const T *)p.k + row * p.k_cs + p.k_co + (h - p.qh) * p.D;
+        T *dst = isq ? (T *)p.qo + row * p.qo_cs + p.qo_co + h * p.D : (T *)p.ko + row * p.ko_cs + p.ko_co + (h - p.qh) * p.D;
+        if (unit >= u.turn) {
+            const int at = 2 * p.pairs + (unit - u.turn) * VEC;
+            Piece<F32, VEC> v;
+            v.load(src + at);
+            v.store(dst + at);
             continue;
         }
-        const int64_t b = row / p.N;
-        const float2 cs = phase(p, b, (int)(row - b * p.N), j);
-        const int ia = p.neighbours ? 2 * j : j, ib = p.neighbours ? 2 * j + 1 : j + p.pairs;
-        const float a = E::get(src + ia), v = E::get(src + ib);
-        E::put(dst + ia, a * cs.x - v * cs.y);
-        E::put(dst + ib, v * cs.x + a * cs.y);
+        if constexpr (VEC == 1) {                                        // one pair
+            const float c = cosines[t * p.pairs + unit], s = sines[t * p.pairs + unit];
+            const int ia = NEIGHBOURS ? 2 * unit : unit, ib = NEIGHBOURS ? 2 * unit + 1 : unit + p.pairs;
+            Piece<F32, 1> a, b;
+            a.load(src + ia), b.load(src + ib);
+            const float x = a.get(0), y = b.get(0);
+            a.set1(x * c - y * s), b.set1(y * c + x * s);
+            a.store(dst + ia), b.store(dst + ib);
+        } else if constexpr (NEIGHBOURS) {                                // VEC / 2 pairs
+            typedef __attribute__((ext_vector_type(VEC / 2))) float C;
+            const C c = *(const C *)(cosines + t * p.pairs + unit * (VEC / 2)), s = *(const C *)(sines + t * p.pairs + unit * (VEC / 2));
+            Piece<F32, VEC> v;
+            v.load(src + unit * VEC);
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+                const float x = v.get(2 * j), y = v.get(2 * j + 1);
+                v.set(2 * j, x * c[j] - y * s[j], y * c[j] + x * s[j]);
+            }
+            v.store(dst + unit * VEC);
+        } else {                                                          // VEC pairs
+            typedef __attribute__((ext_vector_type(4))) float C;           // (four at a time: the table is 16-byte aligned)
+            C c[VEC / 4], s[VEC / 4];
+#pragma unroll
+            for (int j = 0; j < VEC / 4; ++j) {
+                c[j] = *(const C *)(cosines + t * p.pairs + unit * VEC + 4 * j);
+                s[j] = *(const C *)(sines + t * p.pairs + unit * VEC + 4 * j);
+            }
+            Piece<F32, VEC> a, b;
+            a.load(src + unit * VEC), b.load(src + unit * VEC + p.pairs);
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) {
+                const float x0 = a.get(j), x1 = a.get(j + 1), y0 = b.get(j), y1 = b.get(j + 1);
+                const float c0 = c[j / 4][j % 4], c1 = c[j / 4][j % 4 + 1], s0 = s[j / 4][j % 4], s1 = s[j / 4][j % 4 + 1];
+                a.set(j, x0 * c0 - y0 * s0, x1 * c1 - y1 * s1);
+                b.set(j, y0 * c0 + x0 * s0, y1 * c1 + x1 * s1);
+            }
+            a.store(dst + unit * VEC), b.store(dst + unit * VEC + p.pairs);
+        }
     }
+}
+
+template <bool F32, int VEC>
+int launch(const onedc_rotary_params *p, void *stream) {
+    Units u;
+    u.turn = VEC == 1 ? p->pairs : p->neighbours ? 2 * p->pairs / VEC : p->pairs / VEC;
+    u.per = u.turn + (p->D - 2 * p->pairs) / VEC;
+    // tokens a workgroup: up to 2048 units (8 a thread), fewer where that leaves under two workgroups a CU
+    const int64_t rows = (int64_t)p->B * p->N;
+    const int heads = p->qh + p->kh;
+    int64_t T = 2048 / ((int64_t)heads * u.per) + 1, most = (rows + 511) / 512;
+    if (T > most) T = most;
+    if (p->pairs && T > MAX_TABLE / p->pairs) T = MAX_TABLE / p->pairs;
+    u.T = (int)(T < 1 ? 1 : T);
+    u.by_unit = OnedcFastDiv(u.per), u.by_head = OnedcFastDiv(heads), u.by_pair = OnedcFastDiv(p->pairs ? p->pairs : 1);
+    const dim3 grid((unsigned)((rows + u.T - 1) / u.T));
+    const size_t lds = (size_t)u.T * p->pairs * 8 + 16;
+    if (p->neighbours) hipLaunchKernelGGL((rotary_kernel<F32, VEC, true>), grid, dim3(NT), lds, as_stream(stream), *p, u);
+    else hipLaunchKernelGGL((rotary_kernel<F32, VEC, false>), grid, dim3(NT), lds, as_stream(stream), *p, u);
+    ONEDC_LAUNCH_CHECK();
+    return 0;
 }
 
 }  // namespace
@@ -57,12 +165,16 @@ extern "C" int onedc_rotary_axes(const onedc_rotary_params *p, void *stream) {
     const int cq = p->qh * p->D, ck = p->kh * p->D;
     if (p->q_co < 0 || p->q_cs - cq < p->q_co || p->qo_co < 0 || p->qo_cs - cq < p->qo_co) return -2;
     if (p->kh && (p->k_co < 0 || p->k_cs - ck < p->k_co || p->ko_co < 0 || p->ko_cs - ck < p->ko_co)) return -2;
-    const int64_t total = (int64_t)p->B * p->N * (p->qh + p->kh) * (p->D - p->pairs);
-    if (!total) return 0;
-    const int64_t blocks = (total + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
-    if (p->x_f32) hipLaunchKernelGGL(rotary_kernel<true>, grid, dim3(256), 0, as_stream(stream), *p);
-    else hipLaunchKernelGGL(rotary_kernel<false>, grid, dim3(256), 0, as_stream(stream), *p);
-    ONEDC_LAUNCH_CHECK();
-    return 0;
+    if (!p->B || !p->N) return 0;
+    // the widest piece that divides a head's parts and every row's beginning: 16 bytes, 8 bytes, or single values
+    const int part = p->neighbours ? 2 * p->pairs : p->pairs, size = p->x_f32 ? 4 : 2;
+    int bits = part | (p->D - 2 * p->pairs) | p->D | p->q_cs | p->q_co | p->qo_cs | p->qo_co;
+    uintptr_t at = (uintptr_t)p->q | (uintptr_t)p->qo;
+    if (p->kh) {
+        bits |= p->k_cs | p->k_co | p->ko_cs | p->ko_co;
+        at |= (uintptr_t)p->k | (uintptr_t)p->ko;
+    }
+    const auto fits = [&](int vec) { return bits % vec == 0 && at % (unsigned)(vec * size) == 0; };
+    if (p->x_f32) return fits(4) ? launch<true, 4>(p, stream) : launch<true, 1>(p, stream);
+    return fits(8) ? launch<false, 8>(p, stream) : fits(4) ? launch<false, 4>(p, stream) : launch<false, 1>(p, stream);
 }
