@@ -8,19 +8,22 @@
 //   df = the same step through norm(f) on alpha * gate * post_w * dt, or alpha * gate * dt without the post norm
 // and every parameter gradient follows from four sums over the rows of a picture: S1 = sum dy, S2 = sum dy * norm(t),
 // T1 = sum dt, T2 = sum dt * norm(f) (f itself without the post norm).
+#include <type_traits>
+
 #include "elem.h"
 
 namespace {
 
 constexpr int NT = 256;
 
-// ---- rows in registers: up to MAX_C channels -------------------------------------------------------------------------------------------
+// ---- rows in registers: up to 16384 channels (backward: 8192) --------------------------------------------------------------------------
 // Bound by HBM: x and f are read once, xo and y written once (backward: four read, two written).  A row belongs to L neighbouring lanes
-// (8 .. 64, or the whole workgroup), which hold it as IT pieces of eight channels each: piece i of lane l begins at channel 8 (i L + l).
-// Statistics are two passes over registers -- mean, then squared deviations -- and log2 L exchanges between lanes.  A workgroup
-// takes a run of rows of one picture, so that the vectors per picture (gate, scale, shift) and per channel are combined once, in LDS:
+// (8 .. 64, or a workgroup of 256, 512 or 1024), which hold it as IT pieces of eight channels each: piece i of lane l begins at channel
+// 8 (i L + l).  Statistics are two passes over registers -- mean, then squared deviations -- and log2 L exchanges between lanes.  A
+// workgroup takes a run of rows of one picture, so that the vectors per picture (gate, scale, shift) and per channel are combined once:
 //   A = alpha gate post_w, Ab = alpha gate post_b (join);  W = w (1 + scale), S = b (1 + scale) + shift (norm behind it)
-// and the next rows' loads are in flight while a row is computed.
+// into LDS where several rows of a wave share them, into registers where a thread owns its channels.  The next row's loads are in
+// flight while a row is computed.
 
 // sum over the L neighbouring lanes of v's row, the same bits in each of them
 template <int O>
@@ -37,17 +40,21 @@ __device__ __forceinline__ float lanes_sum(float v, int L) {
     return v;
 }
 // ... or over the workgroup; red: two floats a wave, alternated so that one barrier a sum is enough
+template <int NTH>
 struct RowSum {
     float *red;
     int L, turn;
     __device__ __forceinline__ float operator()(float v) {
         if (L <= 64) return lanes_sum(v, L);
         v = lanes_sum(v, 64);
-        float *r = red + turn * (NT / 64);
+        float *r = red + turn * (NTH / 64);
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
         __syncthreads();
-        return (r[0] + r[1]) + (r[2] + r[3]);
+        float s = r[0];
+#pragma unroll
+        for (int i = 1; i < NTH / 64; ++i) s += r[i];
+        return s;
     }
 };
 
@@ -102,37 +109,56 @@ __device__ __forceinline__ void put8(void *base, int64_t at, const float (&v)[8]
 
 struct Plan {
     int L, run_rows, runs;                // lanes a row; rows of a run, runs of a picture
-    int has;                              // 1: A, 2: Ab, 4: W, 8: S are in LDS (in this order, C8 floats each)
+    int has;                              // which combined vectors there are
 };
 enum { HAS_A = 1, HAS_AB = 2, HAS_W = 4, HAS_S = 8 };
 
 __device__ __forceinline__ float at(const float *v, int64_t i, float none) { return v ? v[i] : none; }
+__device__ __forceinline__ float combined(const onedc_block_norm_params &p, int which, int64_t b, int c) {
+    if (which == HAS_A || which == HAS_AB) {
+        const float g = p.alpha * at(p.gate, b * p.gate_rs + c, 1.f);
+        return which == HAS_A ? g * at(p.post_w, c, 1.f) : g * at(p.post_b, c, 0.f);
+    }
+    const float s = 1.f + at(p.scale, b * p.scale_rs + c, 0.f);
+    return which == HAS_W ? s * at(p.w, c, 1.f) : __builtin_fmaf(s, at(p.b, c, 0.f), at(p.shift, b * p.shift_rs + c, 0.f));
+}
 
-// the combined vectors of picture b
-__device__ __forceinline__ void combine(const onedc_block_norm_params &p, int has, int64_t b, float *lds, int C8) {
-    float *A = lds, *Ab = A + (has & HAS_A ? C8 : 0), *W = Ab + (has & HAS_AB ? C8 : 0), *S = W + (has & HAS_W ? C8 : 0);
-    for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
-        if (has & (HAS_A | HAS_AB)) {
-            const float g = p.alpha * at(p.gate, b * p.gate_rs + c, 1.f);
-            if (has & HAS_A) A[c] = g * at(p.post_w, c, 1.f);
-            if (has & HAS_AB) Ab[c] = g * at(p.post_b, c, 0.f);
-        }
-        if (has & (HAS_W | HAS_S)) {
-            const float s = 1.f + at(p.scale, b * p.scale_rs + c, 0.f);
-            if (has & HAS_W) W[c] = s * at(p.w, c, 1.f);
-            if (has & HAS_S) S[c] = s * at(p.b, c, 0.f) + at(p.shift, b * p.shift_rs + c, 0.f);
+// One combined vector of a picture: in LDS (SHARED), or this thread's channels of it in registers
+template <int IT, bool SHARED, int WHICH>
+struct Vector {
+    float v[SHARED ? 1 : IT][8];
+    const float *lds;
+    bool on;
+    // lds: where the next vector begins
+    __device__ __forceinline__ void make(const onedc_block_norm_params &p, int has, int64_t b, int c0, int step, float *&at_lds) {
+        on = has & WHICH;
+        if (!on) return;
+        if constexpr (SHARED) {
+            for (int c = threadIdx.x; c < p.C; c += blockDim.x) at_lds[c] = combined(p, WHICH, b, c);
+            lds = at_lds;
+            at_lds += (p.C + 7) & ~7;
+        } else {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = combined(p, WHICH, b, min(c0 + i * step + j, p.C - 1));
         }
     }
-}
-__device__ __forceinline__ void take8(const float *v, int c, float (&o)[8]) {
-    const f32x4 a = *(const f32x4 *)(v + c), b = *(const f32x4 *)(v + c + 4);
+    __device__ __forceinline__ void get(int i, int c, float (&o)[8]) const {
+        if constexpr (SHARED) {
+            const f32x4 a = *(const f32x4 *)(lds + c), b = *(const f32x4 *)(lds + c + 4);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = a[j], o[4 + j] = b[j];
-}
+            for (int j = 0; j < 4; ++j) o[j] = a[j], o[4 + j] = b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = v[i][j];
+        }
+    }
+};
 
 // v -> (v - mean) * r in place; values behind C stay 0.  Returns r.
-template <bool TAIL, int IT>
-__device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, int C, int kind, float eps, RowSum &sum) {
+template <bool TAIL, int IT, int NTH>
+__device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, int C, int kind, float eps, RowSum<NTH> &sum) {
     if (kind == ONEDC_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
@@ -158,15 +184,22 @@ __device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, 
     return r;
 }
 
-template <int IT, bool X32, bool F32, bool TAIL>
-__global__ __launch_bounds__(NT, IT > 2 ? 3 : 4) void block_norm_rows_kernel(onedc_block_norm_params p, Plan pl) {
+// NTH 256: rows of up to 64 lanes (SHARED), or one row a workgroup
+template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL>
+__global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_norm_rows_kernel(onedc_block_norm_params p, Plan pl) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    const int C8 = (p.C + 7) & ~7;
     const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
-    combine(p, pl.has, b, lds + 2 * (NT / 64), C8);
-    const float *A = lds + 2 * (NT / 64), *Ab = A + (pl.has & HAS_A ? C8 : 0), *W = Ab + (pl.has & HAS_AB ? C8 : 0), *S = W + (pl.has & HAS_W ? C8 : 0);
-    RowSum sum = {lds, pl.L, 0};
-    const int lane = threadIdx.x & (pl.L - 1), step = 8 * pl.L, c0 = lane * 8, each = NT / pl.L;
+    const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
+    float *at_lds = lds + 2 * (NTH / 64);
+    Vector<IT, SHARED, HAS_A> A;
+    Vector<IT, SHARED, HAS_AB> Ab;
+    Vector<IT, SHARED, HAS_W> W;
+    Vector<IT, SHARED, HAS_S> S;
+    A.make(p, pl.has, b, c0, step, at_lds);
+    Ab.make(p, pl.has, b, c0, step, at_lds);
+    W.make(p, pl.has, b, c0, step, at_lds);
+    S.make(p, pl.has, b, c0, step, at_lds);
+    RowSum<NTH> sum = {lds, L, 0};
     const int n1 = min(p.N, (run + 1) * pl.run_rows);
     const int64_t row0 = (int64_t)b * p.N;
     Eight<X32> x[IT];
@@ -180,13 +213,13 @@ __global__ __launch_bounds__(NT, IT > 2 ? 3 : 4) void block_norm_rows_kernel(one
             if (p.f) f[i].template load<TAIL>(p.f, row * p.f_cs + p.f_co + c, left);
         }
     };
-    int n = run * pl.run_rows + threadIdx.x / pl.L;
+    int n = run * pl.run_rows + threadIdx.x / L;
     load(n);
     __syncthreads();
     int cl = c0;
     // (every thread makes every turn: sums over a workgroup have barriers)
     for (int left_rows = n1 - run * pl.run_rows; left_rows > 0; left_rows -= each, n += each) {
-        if (IT > 2) asm volatile("" : "+v"(cl));        // (else the compiler keeps all of a thread's LDS vectors in registers, and spills)
+        if (SHARED && IT > 1) asm volatile("" : "+v"(cl));        // (else the compiler keeps all of a thread's LDS vectors in registers, and spills)
         float t[IT][8];
 #pragma unroll
         for (int i = 0; i < IT; ++i)
@@ -205,13 +238,13 @@ __global__ __launch_bounds__(NT, IT > 2 ? 3 : 4) void block_norm_rows_kernel(one
                 const int c = c0 + i * step;
                 if (c < p.C) {
                     float a[8], ab[8];
-                    if (pl.has & HAS_A) take8(A, cl + i * step, a);
-                    if (pl.has & HAS_AB) take8(Ab, cl + i * step, ab);
+                    if (A.on) A.get(i, cl + i * step, a);
+                    if (Ab.on) Ab.get(i, cl + i * step, ab);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        t[i][j] = __builtin_fmaf(pl.has & HAS_A ? a[j] : p.alpha, v[i][j], t[i][j]);
-                        if (pl.has & HAS_AB) t[i][j] += ab[j];
-                        if (TAIL && c + j >= p.C) t[i][j] = 0.f;                       // (LDS behind C is not written)
+                        t[i][j] = __builtin_fmaf(A.on ? a[j] : p.alpha, v[i][j], t[i][j]);
+                        if (Ab.on) t[i][j] += ab[j];
+                        if (TAIL && c + j >= p.C) t[i][j] = 0.f;               // (the vectors end at C)
                     }
                     if (n < n1) put8<X32, TAIL>(p.xo, (row0 + n) * p.xo_cs + p.xo_co + c, t[i], p.C - c);
                 }
@@ -225,21 +258,193 @@ __global__ __launch_bounds__(NT, IT > 2 ? 3 : 4) void block_norm_rows_kernel(one
             for (int i = 0; i < IT; ++i) {
                 const int c = c0 + i * step;
                 if (c < p.C && n < n1) {
-                    float w[8], s[8];
-                    if (pl.has & HAS_W) {
-                        take8(W, cl + i * step, w);
+                    float w[8];
+                    if (W.on) {
+                        W.get(i, cl + i * step, w);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) t[i][j] *= w[j];
                     }
-                    if (pl.has & HAS_S) {
-                        take8(S, cl + i * step, s);
+                    if (S.on) {
+                        S.get(i, cl + i * step, w);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) t[i][j] += s[j];
+                        for (int j = 0; j < 8; ++j) t[i][j] += w[j];
                     }
                     put8<F32, TAIL>(p.y, (row0 + n) * p.y_cs + p.y_co + c, t[i], p.C - c);
                 }
             }
         }
+    }
+}
+
+// Backward: dx and df of a row; a thread keeps the four sums of its channels over its run of rows, the lane groups of a workgroup add
+// theirs in order, and part[run of a picture][4][C] goes to the next kernel.
+template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL>
+__global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backward_kernel(onedc_block_norm_params p, onedc_block_norm_grad g,
+                                                                                         Plan pl, float *part) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
+    const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
+    float *at_lds = lds + 2 * (NTH / 64);
+    Vector<IT, SHARED, HAS_A> A;
+    Vector<IT, SHARED, HAS_W> W;
+    A.make(p, pl.has, b, c0, step, at_lds);
+    W.make(p, pl.has, b, c0, step, at_lds);
+    RowSum<NTH> sum = {lds, L, 0};
+    const int n1 = min(p.N, (run + 1) * pl.run_rows);
+    const int64_t row0 = (int64_t)b * p.N;
+    // (raw until they are needed, and replaced by the next row's at once: rows of two pieces a lane fit 256 registers so)
+    Eight<X32> rt[IT], rd[IT];
+    Eight<F32> rf[IT], ry[IT];
+    auto load = [&](auto &to, const void *from, int cs, int co, int n) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = c0 + i * step;
+            to[i].template load<TAIL>(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0);
+        }
+    };
+    float s1[IT][8], s2[IT][8], t1[IT][8], t2[IT][8];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s1[i][j] = s2[i][j] = t1[i][j] = t2[i][j] = 0.f;
+    int n = run * pl.run_rows + threadIdx.x / L;
+    if (g.dy) {
+        load(rt, p.x, p.x_cs, p.x_co, n);
+        load(ry, g.dy, g.dy_cs, g.dy_co, n);
+    }
+    if (g.dxo) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n);
+    if (p.f) load(rf, p.f, p.f_cs, p.f_co, n);
+    __syncthreads();
+    int cl = c0;
+    for (int left_rows = n1 - run * pl.run_rows; left_rows > 0; left_rows -= each, n += each) {
+        if (SHARED) asm volatile("" : "+v"(cl));
+        const bool more = left_rows > each;
+        float d[IT][8], f[IT][8];
+        if (g.dy) {
+            float h[IT][8], u[IT][8];
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] = rt[i].get(j), u[i][j] = ry[i].get(j);
+            if (more) {
+                load(rt, p.x, p.x_cs, p.x_co, n + each);
+                load(ry, g.dy, g.dy_cs, g.dy_co, n + each);
+            }
+            const float r = normalise<TAIL>(h, c0, step, p.C, p.kind, p.eps, sum);
+            float su = 0.f, sh = 0.f;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                float w[8];
+                const int c = c0 + i * step;
+                if (W.on && c < p.C) W.get(i, cl + i * step, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (n < n1) {
+                        s1[i][j] += u[i][j];
+                        s2[i][j] = __builtin_fmaf(u[i][j], h[i][j], s2[i][j]);
+                    }
+                    if (W.on) u[i][j] = c + (TAIL ? j : 0) < p.C ? u[i][j] * w[j] : 0.f;
+                    su += u[i][j];
+                    sh = __builtin_fmaf(u[i][j], h[i][j], sh);
+                }
+            }
+            const float mu = p.kind == ONEDC_NORM_LAYER ? sum(su) / p.C : 0.f, mh = sum(sh) / p.C;
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[i][j] = c0 + i * step + (TAIL ? j : 0) < p.C ? r * (u[i][j] - mu - h[i][j] * mh) : 0.f;
+        }
+        if (g.dxo) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[i][j] = g.dy ? d[i][j] + rd[i].get(j) : rd[i].get(j);
+            if (more) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n + each);
+        }
+        if (g.dx && n < n1) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                if (c0 + i * step < p.C) put8<X32, TAIL>(g.dx, (row0 + n) * g.dx_cs + g.dx_co + c0 + i * step, d[i], p.C - c0 - i * step);
+        }
+        if (p.f) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[i][j] = rf[i].get(j);
+            if (more) load(rf, p.f, p.f_cs, p.f_co, n + each);
+        } else {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
+        }
+        float r = 1.f;
+        if (p.post) r = normalise<TAIL>(f, c0, step, p.C, p.kind, p.eps, sum);
+        float sv = 0.f, sf = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            float a[8];
+            const int c = c0 + i * step;
+            if (A.on && c < p.C) A.get(i, cl + i * step, a);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (n < n1) {
+                    t1[i][j] += d[i][j];
+                    t2[i][j] = __builtin_fmaf(d[i][j], f[i][j], t2[i][j]);
+                }
+                d[i][j] *= A.on ? (c + (TAIL ? j : 0) < p.C ? a[j] : 0.f) : p.alpha;
+                sv += d[i][j];
+                sf = __builtin_fmaf(d[i][j], f[i][j], sf);
+            }
+        }
+        if (!g.df) continue;
+        if (p.post) {
+            const float mv = p.kind == ONEDC_NORM_LAYER ? sum(sv) / p.C : 0.f, mf = sum(sf) / p.C;
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - mv - f[i][j] * mf);
+        }
+        if (n < n1) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                if (c0 + i * step < p.C) put8<F32, TAIL>(g.df, (row0 + n) * g.df_cs + g.df_co + c0 + i * step, d[i], p.C - c0 - i * step);
+        }
+    }
+    if (!part) return;
+    float *out = part + (int64_t)blockIdx.x * 4 * p.C;
+    if constexpr (!SHARED) {                         // the thread's channels are nobody else's
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = c0 + i * step + j;
+                if (c < p.C) out[c] = s1[i][j], out[p.C + c] = s2[i][j], out[2 * p.C + c] = t1[i][j], out[3 * p.C + c] = t2[i][j];
+            }
+    } else {
+        const int C8 = (p.C + 7) & ~7, group = threadIdx.x / L;
+        float *acc = lds + 2 * (NTH / 64);           // over the vectors
+        for (int k = 0; k < each; ++k) {
+            __syncthreads();
+            if (group != k) continue;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int c = c0 + i * step;
+                if (c >= p.C) continue;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float(&v)[8] = q == 0 ? s1[i] : q == 1 ? s2[i] : q == 2 ? t1[i] : t2[i];
+                    f32x4 *to = (f32x4 *)(acc + q * C8 + c);
+                    f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+                    if (k) lo += to[0], hi += to[1];
+                    to[0] = lo, to[1] = hi;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            for (int c = threadIdx.x; c < p.C; c += NTH) out[q * p.C + c] = acc[q * C8 + c];
     }
 }
 
@@ -384,36 +589,76 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
     }
 }
 
-// The parameter gradients of one column from the runs' sums
-__global__ void block_norm_params_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const float *part, int runs) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= p.C) return;
-    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f), alpha = p.alpha;
-    double dw = 0, db = 0, dpw = 0, dpb = 0, dgate = 0, dscale = 0, dshift = 0;
-    for (int b = 0; b < p.B; ++b) {
-        double s[4] = {0, 0, 0, 0};
-        for (int r = 0; r < runs; ++r)
-            for (int k = 0; k < 4; ++k) s[k] += part[(((int64_t)b * runs + r) * 4 + k) * p.C + c];
-        const double sc = 1.0 + at(p.scale, (int64_t)b * p.scale_rs + c, 0.f), ga = alpha * at(p.gate, (int64_t)b * p.gate_rs + c, 1.f);
-        dw += sc * s[1];
-        db += sc * s[0];
-        dpw += ga * s[3];
-        dpb += ga * s[2];
-        const double gt = alpha * (pw * s[3] + pb * s[2]), gs = w * s[1] + bb * s[0];
-        if (g.d_gate && p.gate_rs) g.d_gate[(int64_t)b * p.C + c] = (float)gt;
-        if (g.d_scale && p.scale_rs) g.d_scale[(int64_t)b * p.C + c] = (float)gs;
-        if (g.d_shift && p.shift_rs) g.d_shift[(int64_t)b * p.C + c] = (float)s[0];
-        dgate += gt;
-        dscale += gs;
-        dshift += s[0];
+// The parameter gradients.  One picture: 64 channels x 4 quarters of the runs a workgroup, added in order in f64; what has a row per
+// picture is finished here, the picture's sums go on (or, the only picture, everything is finished here).
+struct Sums {
+    double s[4];                          // S1, S2, T1, T2
+};
+__device__ __forceinline__ void finish_picture(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int64_t b, int c, const Sums &s) {
+    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
+    if (g.d_gate && p.gate_rs) g.d_gate[b * p.C + c] = (float)(p.alpha * (pw * s.s[3] + pb * s.s[2]));
+    if (g.d_scale && p.scale_rs) g.d_scale[b * p.C + c] = (float)(w * s.s[1] + bb * s.s[0]);
+    if (g.d_shift && p.shift_rs) g.d_shift[b * p.C + c] = (float)s.s[0];
+}
+// sums over the pictures: plain, and weighted by the picture's gate and scale
+struct Totals {
+    double gate, scale, shift, w, b, post_w, post_b;
+};
+__device__ __forceinline__ void add_picture(const onedc_block_norm_params &p, int64_t b, int c, const Sums &s, Totals &t) {
+    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
+    const double sc = 1.0 + at(p.scale, b * p.scale_rs + c, 0.f), ga = p.alpha * (double)at(p.gate, b * p.gate_rs + c, 1.f);
+    t.gate += p.alpha * (pw * s.s[3] + pb * s.s[2]);
+    t.scale += w * s.s[1] + bb * s.s[0];
+    t.shift += s.s[0];
+    t.w += sc * s.s[1];
+    t.b += sc * s.s[0];
+    t.post_w += ga * s.s[3];
+    t.post_b += ga * s.s[2];
+}
+__device__ __forceinline__ void finish_all(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int c, const Totals &t) {
+    if (g.d_gate && !p.gate_rs) g.d_gate[c] = (float)t.gate;
+    if (g.d_scale && !p.scale_rs) g.d_scale[c] = (float)t.scale;
+    if (g.d_shift && !p.shift_rs) g.d_shift[c] = (float)t.shift;
+    if (g.d_w) g.d_w[c] = (float)t.w;
+    if (g.d_b) g.d_b[c] = (float)t.b;
+    if (g.d_post_w) g.d_post_w[c] = (float)t.post_w;
+    if (g.d_post_b) g.d_post_b[c] = (float)t.post_b;
+}
+
+__global__ __launch_bounds__(NT) void block_norm_picture_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const float *part, Sums *pictures,
+                                                                int runs) {
+    __shared__ Sums red[4][64];
+    const int columns = (p.C + 63) / 64;
+    const int64_t b = blockIdx.x / columns;
+    const int c = (int)(blockIdx.x - b * columns) * 64 + (threadIdx.x & 63), quarter = threadIdx.x >> 6;
+    Sums s = {{0, 0, 0, 0}};
+    if (c < p.C)
+#pragma unroll 4
+        for (int r = quarter; r < runs; r += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s.s[k] += part[((b * runs + r) * 4 + k) * p.C + c];
+    red[quarter][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (quarter || c >= p.C) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s.s[k] = (red[0][threadIdx.x].s[k] + red[1][threadIdx.x].s[k]) + (red[2][threadIdx.x].s[k] + red[3][threadIdx.x].s[k]);
+    finish_picture(p, g, b, c, s);
+    if (pictures) {
+        pictures[b * p.C + c] = s;
+    } else if (p.B == 1) {
+        Totals t = {0, 0, 0, 0, 0, 0, 0};
+        add_picture(p, 0, c, s, t);
+        finish_all(p, g, c, t);
     }
-    if (g.d_gate && !p.gate_rs) g.d_gate[c] = (float)dgate;
-    if (g.d_scale && !p.scale_rs) g.d_scale[c] = (float)dscale;
-    if (g.d_shift && !p.shift_rs) g.d_shift[c] = (float)dshift;
-    if (g.d_w) g.d_w[c] = (float)dw;
-    if (g.d_b) g.d_b[c] = (float)db;
-    if (g.d_post_w) g.d_post_w[c] = (float)dpw;
-    if (g.d_post_b) g.d_post_b[c] = (float)dpb;
+}
+// the sums over the pictures, in order
+__global__ __launch_bounds__(64) void block_norm_all_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const Sums *pictures) {
+    const int c = blockIdx.x * 64 + threadIdx.x;
+    if (c >= p.C) return;
+    Totals t = {0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (int b = 0; b < p.B; ++b) add_picture(p, b, c, pictures[(int64_t)b * p.C + c], t);
+    finish_all(p, g, c, t);
 }
 
 int check_view(const void *p, int cs, int co, int C) { return !p || (cs >= C && co >= 0 && co <= cs - C) ? 0 : -2; }
@@ -432,38 +677,104 @@ int check_common(const onedc_block_norm_params *p) {
     return 0;
 }
 
-struct Runs {
-    int runs, rows;        // runs of `rows` token rows per picture
-};
-Runs backward_runs(const onedc_block_norm_params *p) {
-    const int want = p->B > 0 ? (512 + p->B - 1) / p->B : 1;
-    Runs r;
-    r.rows = (p->N + want - 1) / want;
-    if (r.rows < 1) r.rows = 1;
-    r.runs = (p->N + r.rows - 1) / r.rows;
-    if (r.runs < 1) r.runs = 1;
-    return r;
+bool wants_sums(const onedc_block_norm_grad *g) {
+    return g->d_post_w || g->d_post_b || g->d_gate || g->d_w || g->d_b || g->d_scale || g->d_shift;
+}
+bool wants_all(const onedc_block_norm_params *p, const onedc_block_norm_grad *g) {
+    return g->d_post_w || g->d_post_b || g->d_w || g->d_b || (g->d_gate && !p->gate_rs) || (g->d_scale && !p->scale_rs) || (g->d_shift && !p->shift_rs);
+}
+// Without a parameter per picture the pictures are one.
+onedc_block_norm_params joined_pictures(const onedc_block_norm_params *p) {
+    onedc_block_norm_params q = *p;
+    if (!p->gate_rs && !p->scale_rs && !p->shift_rs) {
+        q.N = p->B * p->N;
+        q.B = q.N ? 1 : 0;
+    }
+    return q;
 }
 
-// Rows in registers: as few lanes a row as hold it in IT pieces of eight, so that few of them idle and exchanges stay short.  false: too wide.
-bool row_plan(const onedc_block_norm_params *p, int most_it, int64_t most_lds, int has, int arrays, int want_runs, Plan *pl, int *it) {
-    const int pieces = (p->C + 7) / 8;
-    pl->has = has;
-    for (pl->L = 8; pl->L <= NT; pl->L = pl->L == 64 ? NT : 2 * pl->L)
-        if (pieces <= most_it * pl->L) break;
-    if (pl->L > NT || (int64_t)arrays * ((p->C + 7) & ~7) * 4 + 64 > most_lds) return false;
-    *it = (pieces + pl->L - 1) / pl->L;
-    // whole turns of the workgroup (NT / L rows each) a run
-    const int each = NT / pl->L, turns = (p->N + each - 1) / each;
-    int want = (want_runs + p->B - 1) / p->B;
+// How rows lie in lanes, by the row's width alone.  Two pieces a lane, in as few lanes as that takes: 4.4 TB/s at 320 channels and 5.4 at
+// 640 against 4.2 / 3.0 with one piece (twice the lanes, half of them idle) and, three pieces, 4.3 / 5.0; five pieces spill.  Three where two
+// of 64 lanes end (1280 channels: 4.3 against 3.8 for one row a workgroup), but not with a ragged end, whose code takes their registers.
+// Wider rows belong to a workgroup each, one piece a thread (two from 8192 channels on, forward).
+struct Shape {
+    int threads, it, most;                // threads a workgroup; pieces a lane; 0: the row is too wide for registers
+    bool shared;                          // several rows a workgroup
+};
+Shape row_shape(int C, int widest, bool back, int *L) {
+    const int pieces = (C + 7) / 8;
+    Shape s = {NT, 0, widest, true};
+    for (*L = 8; *L <= 64; *L *= 2)
+        if (pieces <= 2 * *L) {
+            s.it = pieces <= *L ? 1 : 2;
+            return s;
+        }
+    *L = 64;
+    if (pieces <= 192 && C % 8 == 0 && !back) {
+        s.it = 3;
+        return s;
+    }
+    s.shared = false;
+    for (s.threads = 256; s.threads <= 1024; s.threads *= 2)
+        if (pieces <= s.threads) {
+            s.it = 1;
+            break;
+        }
+    if (!s.it && C <= widest) s.threads = 1024, s.it = 2;
+    *L = s.threads;
+    return s;
+}
+// a run: whole turns of a workgroup; about `want` runs altogether
+void cut_runs(const onedc_block_norm_params &p, int each, int want, Plan *pl) {
+    const int turns = (p.N + each - 1) / each;
+    want = (want + p.B - 1) / p.B;
     want = want < 1 ? 1 : want > turns ? turns : want;
     pl->run_rows = (turns + want - 1) / want * each;
-    pl->runs = (p->N + pl->run_rows - 1) / pl->run_rows;
+    pl->runs = (p.N + pl->run_rows - 1) / pl->run_rows;
+}
+constexpr int WIDEST = 16384, WIDEST_BACK = 8192;
+constexpr int SIMPLE_RUNS = 512;
+
+// shape and runs of a backward pass; false: the simple kernel (it cuts runs of its own)
+bool backward_plan(const onedc_block_norm_params &p, Shape *s, Plan *pl) {
+    *s = row_shape(p.C, WIDEST_BACK, true, &pl->L);
+    if (!s->it) {
+        cut_runs(p, 1, SIMPLE_RUNS, pl);
+        return false;
+    }
+    cut_runs(p, s->threads / pl->L, s->shared ? 1024 : s->threads == 256 ? 1024 : 512, pl);
+    pl->has = (p.f && (p.gate || p.post_w) ? HAS_A : 0) | (p.w || p.scale ? HAS_W : 0);
     return true;
 }
 
-bool wants_sums(const onedc_block_norm_grad *g) {
-    return g->d_post_w || g->d_post_b || g->d_gate || g->d_w || g->d_b || g->d_scale || g->d_shift;
+// one instance of a kernel template for every shape, type and end of a row
+template <class Call>
+void by_shape(const Shape &s, bool x32, bool f32, bool tail, Call &&call) {
+    auto types = [&](auto nth, auto shared, auto it) {
+        auto ends = [&](auto x, auto f) {
+            if (tail) call(nth, shared, it, x, f, std::true_type());
+            else call(nth, shared, it, x, f, std::false_type());
+        };
+        if (f32) ends(std::true_type(), std::true_type());
+        else if (x32) ends(std::true_type(), std::false_type());
+        else ends(std::false_type(), std::false_type());
+    };
+    typedef std::integral_constant<int, 1> I1;
+    typedef std::integral_constant<int, 2> I2;
+    typedef std::integral_constant<int, 3> I3;
+    if (s.shared) {
+        if (s.it == 1) types(std::integral_constant<int, NT>(), std::true_type(), I1());
+        else if (s.it == 2) types(std::integral_constant<int, NT>(), std::true_type(), I2());
+        else types(std::integral_constant<int, NT>(), std::true_type(), I3());
+    } else if (s.threads == 256) {
+        types(std::integral_constant<int, 256>(), std::false_type(), I1());
+    } else if (s.threads == 512) {
+        types(std::integral_constant<int, 512>(), std::false_type(), I1());
+    } else if (s.it == 1) {
+        types(std::integral_constant<int, 1024>(), std::false_type(), I1());
+    } else {
+        types(std::integral_constant<int, 1024>(), std::false_type(), I2());
+    }
 }
 
 }  // namespace
@@ -479,30 +790,20 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
     if (check_view(p->xo, p->xo_cs, p->xo_co, p->C) || check_view(p->y, p->y_cs, p->y_co, p->C)) return -2;
     if (!p->f != !p->xo) return -3;
     if (!p->y && (p->w || p->b || p->scale || p->shift)) return -3;
-    int has = 0;
-    if (p->f && (p->gate || p->post_w)) has |= HAS_A;
-    if (p->f && p->post_b) has |= HAS_AB;
-    if (p->y && (p->w || p->scale)) has |= HAS_W;
-    if (p->y && (p->b || p->shift)) has |= HAS_S;
+    const onedc_block_norm_params q = joined_pictures(p);
     Plan pl;
-    int it;
-    onedc_block_norm_params q = *p;
-    if (!p->gate_rs && !p->scale_rs && !p->shift_rs && rows <= 0x7fffffff) q.B = 1, q.N = (int)rows;     // one picture, as far as this goes
-    if (row_plan(&q, 5, 128 << 10, has, __builtin_popcount(has), 1024, &pl, &it)) {
-        const size_t lds = 64 + (size_t)__builtin_popcount(has) * ((p->C + 7) & ~7) * 4;
+    const Shape shape = row_shape(p->C, WIDEST, false, &pl.L);
+    if (shape.it) {
+        pl.has = (p->f && (p->gate || p->post_w) ? HAS_A : 0) | (p->f && p->post_b ? HAS_AB : 0) | (p->y && (p->w || p->scale) ? HAS_W : 0) |
+                 (p->y && (p->b || p->shift) ? HAS_S : 0);
+        cut_runs(q, shape.threads / pl.L, shape.threads > 256 ? 512 : 1024, &pl);
+        const size_t lds = shape.threads / 64 * 8 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * ((p->C + 7) & ~7) * 4 : 0);
         const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
-        const bool tail = p->C & 7;
-#define BN_ROWS(IT, X, F, TAIL)                                                                                           \
-    do {                                                                                                                  \
-        static OnedcLdsAttrOnce once;                                                                                     \
-        once.ensure({{(const void *)block_norm_rows_kernel<IT, X, F, TAIL>, 128 << 10}});                                 \
-        hipLaunchKernelGGL((block_norm_rows_kernel<IT, X, F, TAIL>), grid, dim3(NT), lds, as_stream(stream), q, pl);      \
-    } while (0)
-#define BN_ROWS_TAIL(IT, X, F) do { if (tail) BN_ROWS(IT, X, F, true); else BN_ROWS(IT, X, F, false); } while (0)
-#define BN_ROWS_IT(X, F) do { if (it <= 2) BN_ROWS_TAIL(2, X, F); else BN_ROWS_TAIL(5, X, F); } while (0)
-        if (p->f_f32) BN_ROWS_IT(true, true);
-        else if (p->x_f32) BN_ROWS_IT(true, false);
-        else BN_ROWS_IT(false, false);
+        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail) {
+            constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
+            constexpr bool SH = decltype(shared)::value, X = decltype(x32)::value, F = decltype(f32)::value, TL = decltype(tail)::value;
+            hipLaunchKernelGGL((block_norm_rows_kernel<NTH, SH, IT, X, F, TL>), grid, dim3(NTH), lds, as_stream(stream), q, pl);
+        });
         ONEDC_LAUNCH_CHECK();
         return 0;
     }
@@ -517,8 +818,13 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
 }
 
 int64_t onedc_block_norm_backward_ws_bytes(const onedc_block_norm_params *p, const onedc_block_norm_grad *g) {
-    if (check_common(p) || !g || !wants_sums(g)) return 0;
-    return (int64_t)p->B * backward_runs(p).runs * 4 * p->C * sizeof(float);
+    if (check_common(p) || !g || !wants_sums(g) || !p->B || !p->N) return 0;
+    const onedc_block_norm_params q = joined_pictures(p);
+    Shape s;
+    Plan pl;
+    backward_plan(q, &s, &pl);
+    // the pictures' sums in front of the runs' (8-byte aligned)
+    return (q.B > 1 && wants_all(p, g) ? (int64_t)q.B * p->C * sizeof(Sums) : 0) + (int64_t)q.B * pl.runs * 4 * p->C * sizeof(float);
 }
 
 int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_block_norm_grad *g, void *stream) {
@@ -540,22 +846,52 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     const bool sums = wants_sums(g);
     const int64_t need = onedc_block_norm_backward_ws_bytes(p, g);
     if (need && (!g->ws || g->ws_bytes < need)) return -15;
-    const Runs r = backward_runs(p);
-    float *part = sums ? (float *)g->ws : nullptr;
-    if (any) {
-        const dim3 grid((unsigned)(p->B * r.runs));
-        if (p->f_f32)
-            hipLaunchKernelGGL((block_norm_backward_kernel<true, true>), grid, dim3(NT), 0, as_stream(stream), *p, *g, part, r.runs, r.rows);
-        else if (p->x_f32)
-            hipLaunchKernelGGL((block_norm_backward_kernel<true, false>), grid, dim3(NT), 0, as_stream(stream), *p, *g, part, r.runs, r.rows);
-        else
-            hipLaunchKernelGGL((block_norm_backward_kernel<false, false>), grid, dim3(NT), 0, as_stream(stream), *p, *g, part, r.runs, r.rows);
-        ONEDC_LAUNCH_CHECK();
+    if (!any) {
+        if (sums) {                                  // no rows: every sum is 0
+            onedc_block_norm_params none = *p;
+            if (p->B) {
+                hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)p->B * ((p->C + 63) / 64))), dim3(NT), 0, as_stream(stream),
+                                   none, *g, (const float *)nullptr, (Sums *)nullptr, 0);
+                ONEDC_LAUNCH_CHECK();
+            }
+            none.B = 0;
+            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 63) / 64), dim3(64), 0, as_stream(stream), none, *g, (const Sums *)nullptr);
+            ONEDC_LAUNCH_CHECK();
+        }
+        return 0;
     }
+    const onedc_block_norm_params q = joined_pictures(p);
+    Shape shape;
+    Plan pl;
+    const bool rows = backward_plan(q, &shape, &pl);
+    Sums *pictures = sums && q.B > 1 && wants_all(p, g) ? (Sums *)g->ws : nullptr;
+    float *part = sums ? (float *)((char *)g->ws + (pictures ? (int64_t)q.B * p->C * sizeof(Sums) : 0)) : nullptr;
+    const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
+    if (rows) {
+        const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most, then the sums)
+        const size_t lds = shape.threads / 64 * 8 + scratch;
+        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail) {
+            constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
+            constexpr bool SH = decltype(shared)::value, X = decltype(x32)::value, F = decltype(f32)::value, TL = decltype(tail)::value;
+            if constexpr (IT == 1 || (SH && IT == 2))
+                hipLaunchKernelGGL((block_norm_rows_backward_kernel<NTH, SH, IT, X, F, TL>), grid, dim3(NTH), lds, as_stream(stream), q, *g, pl, part);
+        });
+    } else if (p->f_f32) {
+        hipLaunchKernelGGL((block_norm_backward_kernel<true, true>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+    } else if (p->x_f32) {
+        hipLaunchKernelGGL((block_norm_backward_kernel<true, false>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+    } else {
+        hipLaunchKernelGGL((block_norm_backward_kernel<false, false>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+    }
+    ONEDC_LAUNCH_CHECK();
     if (sums) {
-        hipLaunchKernelGGL(block_norm_params_kernel, dim3((p->C + 255) / 256), dim3(256), 0, as_stream(stream), *p, *g, part,
-                           p->N > 0 ? r.runs : 0);
+        hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)q.B * ((p->C + 63) / 64))), dim3(NT), 0, as_stream(stream), q, *g, part,
+                           pictures, pl.runs);
         ONEDC_LAUNCH_CHECK();
+        if (pictures) {
+            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 63) / 64), dim3(64), 0, as_stream(stream), q, *g, (const Sums *)pictures);
+            ONEDC_LAUNCH_CHECK();
+        }
     }
     return 0;
 }

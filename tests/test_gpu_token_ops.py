@@ -166,6 +166,10 @@ CASES = [
     (5, 1, 100, "layer", False, "each", "each", True, -2.0),
     (2, 131, 72, "rms", False, "each", None, True, 1.0),
     (1, 17, 2048, "layer", False, "one", "one", True, 1.0),
+    (2, 6, 1536, "rms", True, "each", "each", True, 1.0),
+    (1, 5, 2500, "layer", False, "one", None, True, 1.0),
+    (1, 2, 5001, "rms", True, "each", "each", True, 1.0),
+    (70000, 1, 8, "layer", False, "each", "each", False, 1.0),
 ]
 
 
@@ -224,6 +228,29 @@ def test_block_norm_has_nothing_to_do_for_no_rows(fmt):
     dw = torch.full((64,), 3.0, device=DEV)
     K.block_norm_backward(x, y, View(torch.empty(0, dtype=fmt, device=DEV), 0, 1, 4, 64), w=torch.ones(64, device=DEV), d_w=dw)
     assert float(dw.abs().max()) == 0.0
+    none = View(torch.empty(0, dtype=fmt, device=DEV), 3, 1, 0, 64)              # three pictures without a token: gradients of their gates too
+    for B in (1, 3):
+        none.B = B
+        dg, dw, gate = torch.full((B, 64), 3.0, device=DEV), torch.full((64,), 3.0, device=DEV), torch.ones(B, 64, device=DEV)
+        K.block_norm_backward(none, none, f=none, gate=gate, w=torch.ones(64, device=DEV), d_gate=dg, d_w=dw)
+        assert float(dg.abs().max()) == 0.0 and float(dw.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("Cc", [64, 320, 1280, 2048])
+def test_block_norm_with_no_epsilon(Cc, fmt):
+    """eps = 0 and a row count that leaves lanes of the last turn without a row: nothing of theirs reaches the sums."""
+    B, N = 1, 5
+    g = gen(30)
+    a = options(g, B, Cc, K.NORM_LAYER, True, "each", "each", True)
+    x, f, dy = (rand(g, B, N, Cc).to(fmt) for _ in range(3))
+    p, dx, df = on_gpu(a), empty(B, N, Cc, fmt), empty(B, N, Cc, fmt)
+    out = {"d_" + n: torch.empty(p[n].shape, device=DEV) for n in ("post_w", "post_b", "gate", "w", "b", "scale", "shift")}
+    K.block_norm_backward(tokens(x), tokens(dy), dx, f=tokens(f), df=df, eps=0.0, **p, **out)
+    ref = grads64(x.double(), f.double(), dy.double(), None, in64(a), 0.0)
+    for name, got in {"dx": back(dx), "df": back(df), **out}.items():
+        # terms of order 10 in 16-bit outputs and sums of five of them
+        got, want = got.cpu().double(), ref[name]
+        assert float((got.reshape(want.shape) - want).norm() / want.norm()) < (2 * half_step(fmt) if name in ("dx", "df") else 2e-5), name
 
 
 def test_block_norm_addresses_past_32_bits():
