@@ -30,31 +30,48 @@ template <int O>
 __device__ __forceinline__ float dpp_add(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), O, 0xf, 0xf, true));
 }
-__device__ __forceinline__ float lanes_sum(float v, int L) {
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
+__device__ __forceinline__ float lanes_sum(float v, int L) {      // (L is wave-uniform; without branches the exchanges of two sums overlap)
     v = dpp_add<0xb1>(v);                            // lane ^ 1
     v = dpp_add<0x4e>(v);                            // lane ^ 2
     v = dpp_add<0x141>(v);                           // mirrored within 8
-    if (L > 8) v = dpp_add<0x140>(v);                // mirrored within 16
-    if (L > 16) v += __shfl_xor(v, 16);
-    if (L > 32) v += __shfl_xor(v, 32);
-    return v;
+    const float w = dpp_add<0x140>(v);               // mirrored within 16
+    v = L > 8 ? w : v;
+    const u32x2_t a = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    v = L > 16 ? __uint_as_float(a[0]) + __uint_as_float(a[1]) : v;
+    const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return L > 32 ? __uint_as_float(b[0]) + __uint_as_float(b[1]) : v;
 }
 // ... or over the workgroup; red: two floats a wave, alternated so that one barrier a sum is enough
-template <int NTH>
+template <int NTH, bool SHARED>
 struct RowSum {
     float *red;
     int L, turn;
-    __device__ __forceinline__ float operator()(float v) {
-        if (L <= 64) return lanes_sum(v, L);
-        v = lanes_sum(v, 64);
-        float *r = red + turn * (NTH / 64);
+    float C, inv_C;
+    __device__ __forceinline__ float2 operator()(float v, float w) {
+        if constexpr (SHARED) return make_float2(lanes_sum(v, L), lanes_sum(w, L));
+        v = lanes_sum(v, 64), w = lanes_sum(w, 64);
+        float2 *r = (float2 *)red + turn * (NTH / 64);
         turn ^= 1;
-        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = make_float2(v, w);
         __syncthreads();
-        float s = r[0];
+        float2 s = r[0];
 #pragma unroll
-        for (int i = 1; i < NTH / 64; ++i) s += r[i];
+        for (int i = 1; i < NTH / 64; ++i) s.x += r[i].x, s.y += r[i].y;
         return s;
+    }
+    // v / C, rounded once but for a rare last bit
+    __device__ __forceinline__ float over_C(float v) const {
+        const float q = v * inv_C;
+        return __builtin_fmaf(__builtin_fmaf(-q, C, v), inv_C, q);
+    }
+    __device__ __forceinline__ float mean(float v) {
+        if constexpr (SHARED) return over_C(lanes_sum(v, L));
+        return over_C((*this)(v, 0.f).x);
+    }
+    __device__ __forceinline__ float2 means(float v, float w) {
+        const float2 s = (*this)(v, w);
+        return make_float2(over_C(s.x), over_C(s.y));
     }
 };
 
@@ -128,15 +145,17 @@ template <int IT, bool SHARED, int WHICH>
 struct Vector {
     float v[SHARED ? 1 : IT][8];
     const float *lds;
+    int last;
     bool on;
     // lds: where the next vector begins
-    __device__ __forceinline__ void make(const onedc_block_norm_params &p, int has, int64_t b, int c0, int step, float *&at_lds) {
-        on = has & WHICH;
+    __device__ __forceinline__ void make(const onedc_block_norm_params &p, bool on_, int64_t b, int c0, int step, float *&at_lds) {
+        on = on_;
         if (!on) return;
         if constexpr (SHARED) {
-            for (int c = threadIdx.x; c < p.C; c += blockDim.x) at_lds[c] = combined(p, WHICH, b, c);
+            last = ((p.C + 7) & ~7) - 8;
+            for (int c = threadIdx.x; c < last + 8; c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
             lds = at_lds;
-            at_lds += (p.C + 7) & ~7;
+            at_lds += last + 8;
         } else {
 #pragma unroll
             for (int i = 0; i < IT; ++i)
@@ -144,8 +163,10 @@ struct Vector {
                 for (int j = 0; j < 8; ++j) v[i][j] = combined(p, WHICH, b, min(c0 + i * step + j, p.C - 1));
         }
     }
+    // eight of them from channel c on; a piece behind the row gets the last ones (finite: it multiplies zeros)
     __device__ __forceinline__ void get(int i, int c, float (&o)[8]) const {
         if constexpr (SHARED) {
+            c = min(c, last);
             const f32x4 a = *(const f32x4 *)(lds + c), b = *(const f32x4 *)(lds + c + 4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] = a[j], o[4 + j] = b[j];
@@ -157,26 +178,28 @@ struct Vector {
 };
 
 // v -> (v - mean) * r in place; values behind C stay 0.  Returns r.
-template <bool TAIL, int IT, int NTH>
-__device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, int C, int kind, float eps, RowSum<NTH> &sum) {
+template <bool TAIL, int IT, class Sum>
+__device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, int C, int kind, float eps, Sum &sum) {
     if (kind == ONEDC_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < IT; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += v[i][j];
-        const float m = sum(s) / C;
+        const float m = sum.mean(s);
 #pragma unroll
-        for (int i = 0; i < IT; ++i)
+        for (int i = 0; i < IT; ++i) {
+            const float mi = c0 + i * step < C ? m : 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = c0 + i * step + (TAIL ? j : 0) < C ? v[i][j] - m : 0.f;
+            for (int j = 0; j < 8; ++j) v[i][j] = TAIL && c0 + i * step + j >= C ? 0.f : v[i][j] - mi;
+        }
     }
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) q = __builtin_fmaf(v[i][j], v[i][j], q);
-    const float r = rsqrtf(sum(q) / C + eps);
+    const float r = rsqrtf(sum.mean(q) + eps);
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
@@ -184,93 +207,93 @@ __device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, 
     return r;
 }
 
+// What a call has, known to the compiler for the join between two sub-blocks in full (its branches cost the generic form a third of its
+// time); GENERIC asks the arguments.
+enum { GENERIC = 0, JOIN = 1, JOIN_POST = 2 };
+
 // NTH 256: rows of up to 64 lanes (SHARED), or one row a workgroup
-template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL>
+template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL, int OPT>
 __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_norm_rows_kernel(onedc_block_norm_params p, Plan pl) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
+    const bool has_f = OPT || p.f, has_y = OPT || p.y, post = OPT ? OPT == JOIN_POST : p.post;
     const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
     const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
-    float *at_lds = lds + 2 * (NTH / 64);
+    float *at_lds = lds + 4 * (NTH / 64);
     Vector<IT, SHARED, HAS_A> A;
     Vector<IT, SHARED, HAS_AB> Ab;
     Vector<IT, SHARED, HAS_W> W;
     Vector<IT, SHARED, HAS_S> S;
-    A.make(p, pl.has, b, c0, step, at_lds);
-    Ab.make(p, pl.has, b, c0, step, at_lds);
-    W.make(p, pl.has, b, c0, step, at_lds);
-    S.make(p, pl.has, b, c0, step, at_lds);
-    RowSum<NTH> sum = {lds, L, 0};
+    A.make(p, OPT || pl.has & HAS_A, b, c0, step, at_lds);
+    Ab.make(p, !OPT && pl.has & HAS_AB, b, c0, step, at_lds);
+    W.make(p, OPT || pl.has & HAS_W, b, c0, step, at_lds);
+    S.make(p, OPT || pl.has & HAS_S, b, c0, step, at_lds);
+    RowSum<NTH, SHARED> sum = {lds, L, 0, (float)p.C, 1.f / (float)p.C};
     const int n1 = min(p.N, (run + 1) * pl.run_rows);
     const int64_t row0 = (int64_t)b * p.N;
     Eight<X32> x[IT];
     Eight<F32> f[IT];
-    auto load = [&](int n) {
-        const int64_t row = row0 + n;
+    auto load = [&](auto &to, const void *from, int cs, int co, int n) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = c0 + i * step, left = n < n1 ? p.C - c : 0;
-            x[i].template load<TAIL>(p.x, row * p.x_cs + p.x_co + c, left);
-            if (p.f) f[i].template load<TAIL>(p.f, row * p.f_cs + p.f_co + c, left);
+            const int c = c0 + i * step;
+            to[i].template load<TAIL>(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0);
         }
     };
     int n = run * pl.run_rows + threadIdx.x / L;
-    load(n);
+    load(x, p.x, p.x_cs, p.x_co, n);
+    if (has_f) load(f, p.f, p.f_cs, p.f_co, n);
     __syncthreads();
     int cl = c0;
     // (every thread makes every turn: sums over a workgroup have barriers)
     for (int left_rows = n1 - run * pl.run_rows; left_rows > 0; left_rows -= each, n += each) {
         if (SHARED && IT > 1) asm volatile("" : "+v"(cl));        // (else the compiler keeps all of a thread's LDS vectors in registers, and spills)
+        const bool more = left_rows > each;
         float t[IT][8];
 #pragma unroll
         for (int i = 0; i < IT; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[i][j] = x[i].get(j);
-        if (p.f) {
+        if (more) load(x, p.x, p.x_cs, p.x_co, n + each);
+        if (has_f) {
             float v[IT][8];
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[i][j] = f[i].get(j);
-            if (left_rows > each) load(n + each);
-            if (p.post) normalise<TAIL>(v, c0, step, p.C, p.kind, p.eps, sum);
+            if (more) load(f, p.f, p.f_cs, p.f_co, n + each);
+            if (post) normalise<TAIL>(v, c0, step, p.C, p.kind, p.eps, sum);
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
                 const int c = c0 + i * step;
-                if (c < p.C) {
-                    float a[8], ab[8];
-                    if (A.on) A.get(i, cl + i * step, a);
-                    if (Ab.on) Ab.get(i, cl + i * step, ab);
+                float a[8];
+                if (A.on) A.get(i, cl + i * step, a);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        t[i][j] = __builtin_fmaf(A.on ? a[j] : p.alpha, v[i][j], t[i][j]);
-                        if (Ab.on) t[i][j] += ab[j];
-                        if (TAIL && c + j >= p.C) t[i][j] = 0.f;               // (the vectors end at C)
-                    }
-                    if (n < n1) put8<X32, TAIL>(p.xo, (row0 + n) * p.xo_cs + p.xo_co + c, t[i], p.C - c);
+                for (int j = 0; j < 8; ++j) t[i][j] = __builtin_fmaf(A.on ? a[j] : p.alpha, v[i][j], t[i][j]);
+                if (Ab.on) {
+                    Ab.get(i, cl + i * step, a);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[i][j] += c + (TAIL ? j : 0) < p.C ? a[j] : 0.f;
                 }
+                if (c < p.C && n < n1) put8<X32, TAIL>(p.xo, (row0 + n) * p.xo_cs + p.xo_co + c, t[i], p.C - c);
             }
-        } else if (left_rows > each) {
-            load(n + each);
         }
-        if (p.y) {
+        if (has_y) {
             normalise<TAIL>(t, c0, step, p.C, p.kind, p.eps, sum);
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
                 const int c = c0 + i * step;
-                if (c < p.C && n < n1) {
-                    float w[8];
-                    if (W.on) {
-                        W.get(i, cl + i * step, w);
+                float w[8];
+                if (W.on) {
+                    W.get(i, cl + i * step, w);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) t[i][j] *= w[j];
-                    }
-                    if (S.on) {
-                        S.get(i, cl + i * step, w);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) t[i][j] += w[j];
-                    }
-                    put8<F32, TAIL>(p.y, (row0 + n) * p.y_cs + p.y_co + c, t[i], p.C - c);
+                    for (int j = 0; j < 8; ++j) t[i][j] *= w[j];
                 }
+                if (S.on) {
+                    S.get(i, cl + i * step, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[i][j] += w[j];
+                }
+                if (c < p.C && n < n1) put8<F32, TAIL>(p.y, (row0 + n) * p.y_cs + p.y_co + c, t[i], p.C - c);
             }
         }
     }
@@ -278,18 +301,20 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_nor
 
 // Backward: dx and df of a row; a thread keeps the four sums of its channels over its run of rows, the lane groups of a workgroup add
 // theirs in order, and part[run of a picture][4][C] goes to the next kernel.
-template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL>
-__global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backward_kernel(onedc_block_norm_params p, onedc_block_norm_grad g,
-                                                                                         Plan pl, float *part) {
+template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL, int OPT>
+__global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_norm_rows_backward_kernel(onedc_block_norm_params p,
+                                                                                                       onedc_block_norm_grad g, Plan pl, float *part) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
+    const bool has_f = OPT || p.f, has_dy = OPT || g.dy, has_dxo = OPT || g.dxo, has_dx = OPT || g.dx, has_df = OPT || g.df;
+    const bool post = OPT ? OPT == JOIN_POST : p.post;
     const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
     const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
-    float *at_lds = lds + 2 * (NTH / 64);
+    float *at_lds = lds + 4 * (NTH / 64);
     Vector<IT, SHARED, HAS_A> A;
     Vector<IT, SHARED, HAS_W> W;
-    A.make(p, pl.has, b, c0, step, at_lds);
-    W.make(p, pl.has, b, c0, step, at_lds);
-    RowSum<NTH> sum = {lds, L, 0};
+    A.make(p, OPT || pl.has & HAS_A, b, c0, step, at_lds);
+    W.make(p, OPT || pl.has & HAS_W, b, c0, step, at_lds);
+    RowSum<NTH, SHARED> sum = {lds, L, 0, (float)p.C, 1.f / (float)p.C};
     const int n1 = min(p.N, (run + 1) * pl.run_rows);
     const int64_t row0 = (int64_t)b * p.N;
     // (raw until they are needed, and replaced by the next row's at once: rows of two pieces a lane fit 256 registers so)
@@ -308,19 +333,20 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backwa
 #pragma unroll
         for (int j = 0; j < 8; ++j) s1[i][j] = s2[i][j] = t1[i][j] = t2[i][j] = 0.f;
     int n = run * pl.run_rows + threadIdx.x / L;
-    if (g.dy) {
+    if (has_dy) {
         load(rt, p.x, p.x_cs, p.x_co, n);
         load(ry, g.dy, g.dy_cs, g.dy_co, n);
     }
-    if (g.dxo) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n);
-    if (p.f) load(rf, p.f, p.f_cs, p.f_co, n);
+    if (has_dxo) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n);
+    if (has_f) load(rf, p.f, p.f_cs, p.f_co, n);
     __syncthreads();
     int cl = c0;
     for (int left_rows = n1 - run * pl.run_rows; left_rows > 0; left_rows -= each, n += each) {
         if (SHARED) asm volatile("" : "+v"(cl));
         const bool more = left_rows > each;
+        const float eps = n < n1 ? p.eps : 1.f;          // (a lane group without a row has zeros: they must not meet an infinite r in the sums)
         float d[IT][8], f[IT][8];
-        if (g.dy) {
+        if (has_dy) {
             float h[IT][8], u[IT][8];
 #pragma unroll
             for (int i = 0; i < IT; ++i)
@@ -330,43 +356,45 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backwa
                 load(rt, p.x, p.x_cs, p.x_co, n + each);
                 load(ry, g.dy, g.dy_cs, g.dy_co, n + each);
             }
-            const float r = normalise<TAIL>(h, c0, step, p.C, p.kind, p.eps, sum);
+            const float r = normalise<TAIL>(h, c0, step, p.C, p.kind, eps, sum);
             float su = 0.f, sh = 0.f;
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
                 float w[8];
-                const int c = c0 + i * step;
-                if (W.on && c < p.C) W.get(i, cl + i * step, w);
+                if (W.on) W.get(i, cl + i * step, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (n < n1) {
-                        s1[i][j] += u[i][j];
-                        s2[i][j] = __builtin_fmaf(u[i][j], h[i][j], s2[i][j]);
-                    }
-                    if (W.on) u[i][j] = c + (TAIL ? j : 0) < p.C ? u[i][j] * w[j] : 0.f;
+                    s1[i][j] += u[i][j];
+                    s2[i][j] = __builtin_fmaf(u[i][j], h[i][j], s2[i][j]);
+                    if (W.on) u[i][j] *= w[j];
                     su += u[i][j];
                     sh = __builtin_fmaf(u[i][j], h[i][j], sh);
                 }
             }
-            const float mu = p.kind == ONEDC_NORM_LAYER ? sum(su) / p.C : 0.f, mh = sum(sh) / p.C;
+            const float2 m = sum.means(su, sh);
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                const float mu = p.kind == ONEDC_NORM_LAYER && c0 + i * step < p.C ? m.x : 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[i][j] = c0 + i * step + (TAIL ? j : 0) < p.C ? r * (u[i][j] - mu - h[i][j] * mh) : 0.f;
+                for (int j = 0; j < 8; ++j) {
+                    d[i][j] = r * (u[i][j] - mu - h[i][j] * m.y);
+                    if (TAIL && c0 + i * step + j >= p.C) d[i][j] = 0.f;
+                }
+            }
         }
-        if (g.dxo) {
+        if (has_dxo) {
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[i][j] = g.dy ? d[i][j] + rd[i].get(j) : rd[i].get(j);
+                for (int j = 0; j < 8; ++j) d[i][j] = has_dy ? d[i][j] + rd[i].get(j) : rd[i].get(j);
             if (more) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n + each);
         }
-        if (g.dx && n < n1) {
+        if (has_dx && n < n1) {
 #pragma unroll
             for (int i = 0; i < IT; ++i)
                 if (c0 + i * step < p.C) put8<X32, TAIL>(g.dx, (row0 + n) * g.dx_cs + g.dx_co + c0 + i * step, d[i], p.C - c0 - i * step);
         }
-        if (p.f) {
+        if (has_f) {
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
@@ -379,31 +407,30 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backwa
                 for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
         }
         float r = 1.f;
-        if (p.post) r = normalise<TAIL>(f, c0, step, p.C, p.kind, p.eps, sum);
+        if (post) r = normalise<TAIL>(f, c0, step, p.C, p.kind, eps, sum);
         float sv = 0.f, sf = 0.f;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             float a[8];
-            const int c = c0 + i * step;
-            if (A.on && c < p.C) A.get(i, cl + i * step, a);
+            if (A.on) A.get(i, cl + i * step, a);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (n < n1) {
-                    t1[i][j] += d[i][j];
-                    t2[i][j] = __builtin_fmaf(d[i][j], f[i][j], t2[i][j]);
-                }
-                d[i][j] *= A.on ? (c + (TAIL ? j : 0) < p.C ? a[j] : 0.f) : p.alpha;
+                t1[i][j] += d[i][j];
+                t2[i][j] = __builtin_fmaf(d[i][j], f[i][j], t2[i][j]);
+                d[i][j] *= A.on ? a[j] : p.alpha;
                 sv += d[i][j];
                 sf = __builtin_fmaf(d[i][j], f[i][j], sf);
             }
         }
-        if (!g.df) continue;
-        if (p.post) {
-            const float mv = p.kind == ONEDC_NORM_LAYER ? sum(sv) / p.C : 0.f, mf = sum(sf) / p.C;
+        if (!has_df) continue;
+        if (post) {
+            const float2 m = sum.means(sv, sf);
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                const float mv = p.kind == ONEDC_NORM_LAYER ? m.x : 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - mv - f[i][j] * mf);
+                for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - mv - f[i][j] * m.y);
+            }
         }
         if (n < n1) {
 #pragma unroll
@@ -423,7 +450,7 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : 2) void block_norm_rows_backwa
             }
     } else {
         const int C8 = (p.C + 7) & ~7, group = threadIdx.x / L;
-        float *acc = lds + 2 * (NTH / 64);           // over the vectors
+        float *acc = lds + 4 * (NTH / 64);           // over the vectors
         for (int k = 0; k < each; ++k) {
             __syncthreads();
             if (group != k) continue;
@@ -589,76 +616,67 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
     }
 }
 
-// The parameter gradients.  One picture: 64 channels x 4 quarters of the runs a workgroup, added in order in f64; what has a row per
-// picture is finished here, the picture's sums go on (or, the only picture, everything is finished here).
-struct Sums {
-    double s[4];                          // S1, S2, T1, T2
-};
-__device__ __forceinline__ void finish_picture(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int64_t b, int c, const Sums &s) {
-    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
-    if (g.d_gate && p.gate_rs) g.d_gate[b * p.C + c] = (float)(p.alpha * (pw * s.s[3] + pb * s.s[2]));
-    if (g.d_scale && p.scale_rs) g.d_scale[b * p.C + c] = (float)(w * s.s[1] + bb * s.s[0]);
-    if (g.d_shift && p.shift_rs) g.d_shift[b * p.C + c] = (float)s.s[0];
-}
-// sums over the pictures: plain, and weighted by the picture's gate and scale
-struct Totals {
-    double gate, scale, shift, w, b, post_w, post_b;
-};
-__device__ __forceinline__ void add_picture(const onedc_block_norm_params &p, int64_t b, int c, const Sums &s, Totals &t) {
-    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
-    const double sc = 1.0 + at(p.scale, b * p.scale_rs + c, 0.f), ga = p.alpha * (double)at(p.gate, b * p.gate_rs + c, 1.f);
-    t.gate += p.alpha * (pw * s.s[3] + pb * s.s[2]);
-    t.scale += w * s.s[1] + bb * s.s[0];
-    t.shift += s.s[0];
-    t.w += sc * s.s[1];
-    t.b += sc * s.s[0];
-    t.post_w += ga * s.s[3];
-    t.post_b += ga * s.s[2];
-}
-__device__ __forceinline__ void finish_all(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int c, const Totals &t) {
-    if (g.d_gate && !p.gate_rs) g.d_gate[c] = (float)t.gate;
-    if (g.d_scale && !p.scale_rs) g.d_scale[c] = (float)t.scale;
-    if (g.d_shift && !p.shift_rs) g.d_shift[c] = (float)t.shift;
-    if (g.d_w) g.d_w[c] = (float)t.w;
-    if (g.d_b) g.d_b[c] = (float)t.b;
-    if (g.d_post_w) g.d_post_w[c] = (float)t.post_w;
-    if (g.d_post_b) g.d_post_b[c] = (float)t.post_b;
+// The parameter gradients, in f64 and in a fixed order.  First a picture: 64 channels x 4 quarters of its runs a workgroup.  What has a row
+// per picture is finished here; the picture's parts of what is summed over the pictures go on, parts[picture][7][C].
+enum { P_GATE, P_SCALE, P_SHIFT, P_W, P_B, P_POST_W, P_POST_B, PARTS };
+__device__ __forceinline__ void finish(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int c, const double (&t)[PARTS]) {
+    if (g.d_gate && !p.gate_rs) g.d_gate[c] = (float)t[P_GATE];
+    if (g.d_scale && !p.scale_rs) g.d_scale[c] = (float)t[P_SCALE];
+    if (g.d_shift && !p.shift_rs) g.d_shift[c] = (float)t[P_SHIFT];
+    if (g.d_w) g.d_w[c] = (float)t[P_W];
+    if (g.d_b) g.d_b[c] = (float)t[P_B];
+    if (g.d_post_w) g.d_post_w[c] = (float)t[P_POST_W];
+    if (g.d_post_b) g.d_post_b[c] = (float)t[P_POST_B];
 }
 
-__global__ __launch_bounds__(NT) void block_norm_picture_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const float *part, Sums *pictures,
+__global__ __launch_bounds__(NT) void block_norm_picture_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const float *part, double *parts,
                                                                 int runs) {
-    __shared__ Sums red[4][64];
-    const int columns = (p.C + 63) / 64;
+    __shared__ double red[4][4][64];
+    const int columns = (p.C + 63) / 64, lane = threadIdx.x & 63;
     const int64_t b = blockIdx.x / columns;
-    const int c = (int)(blockIdx.x - b * columns) * 64 + (threadIdx.x & 63), quarter = threadIdx.x >> 6;
-    Sums s = {{0, 0, 0, 0}};
+    const int c = (int)(blockIdx.x - b * columns) * 64 + lane, quarter = threadIdx.x >> 6;
+    double s[4] = {0, 0, 0, 0};
     if (c < p.C)
 #pragma unroll 4
         for (int r = quarter; r < runs; r += 4)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s.s[k] += part[((b * runs + r) * 4 + k) * p.C + c];
-    red[quarter][threadIdx.x & 63] = s;
+            for (int k = 0; k < 4; ++k) s[k] += part[((b * runs + r) * 4 + k) * p.C + c];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) red[quarter][k][lane] = s[k];
     __syncthreads();
     if (quarter || c >= p.C) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s.s[k] = (red[0][threadIdx.x].s[k] + red[1][threadIdx.x].s[k]) + (red[2][threadIdx.x].s[k] + red[3][threadIdx.x].s[k]);
-    finish_picture(p, g, b, c, s);
-    if (pictures) {
-        pictures[b * p.C + c] = s;
+    for (int k = 0; k < 4; ++k) s[k] = (red[0][k][lane] + red[1][k][lane]) + (red[2][k][lane] + red[3][k][lane]);      // S1, S2, T1, T2
+    const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
+    const double sc = 1.0 + at(p.scale, b * p.scale_rs + c, 0.f), ga = p.alpha * (double)at(p.gate, b * p.gate_rs + c, 1.f);
+    const double t[PARTS] = {p.alpha * (pw * s[3] + pb * s[2]), w * s[1] + bb * s[0], s[0], sc * s[1], sc * s[0], ga * s[3], ga * s[2]};
+    if (g.d_gate && p.gate_rs) g.d_gate[b * p.C + c] = (float)t[P_GATE];
+    if (g.d_scale && p.scale_rs) g.d_scale[b * p.C + c] = (float)t[P_SCALE];
+    if (g.d_shift && p.shift_rs) g.d_shift[b * p.C + c] = (float)t[P_SHIFT];
+    if (parts) {
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) parts[(b * PARTS + k) * p.C + c] = t[k];
     } else if (p.B == 1) {
-        Totals t = {0, 0, 0, 0, 0, 0, 0};
-        add_picture(p, 0, c, s, t);
-        finish_all(p, g, c, t);
+        finish(p, g, c, t);
     }
 }
-// the sums over the pictures, in order
-__global__ __launch_bounds__(64) void block_norm_all_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const Sums *pictures) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= p.C) return;
-    Totals t = {0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-    for (int b = 0; b < p.B; ++b) add_picture(p, b, c, pictures[(int64_t)b * p.C + c], t);
-    finish_all(p, g, c, t);
+// then the pictures: 16 channels x 16 shares of them a workgroup
+__global__ __launch_bounds__(NT) void block_norm_all_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const double *parts) {
+    __shared__ double red[16][PARTS][16];
+    const int lane = threadIdx.x & 15, share = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
+    double t[PARTS] = {0, 0, 0, 0, 0, 0, 0};
+    if (c < p.C)
+        for (int64_t b = share; b < p.B; b += 16)
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) t[k] += parts[(b * PARTS + k) * p.C + c];
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) red[share][k][lane] = t[k];
+    __syncthreads();
+    if (share || c >= p.C) return;
+    for (int i = 1; i < 16; ++i)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) t[k] += red[i][k][lane];
+    finish(p, g, c, t);
 }
 
 int check_view(const void *p, int cs, int co, int C) { return !p || (cs >= C && co >= 0 && co <= cs - C) ? 0 : -2; }
@@ -747,13 +765,15 @@ bool backward_plan(const onedc_block_norm_params &p, Shape *s, Plan *pl) {
     return true;
 }
 
-// one instance of a kernel template for every shape, type and end of a row
+// one instance of a kernel template for every shape, type and end of a row, and what the call has (rows with a ragged end: GENERIC)
 template <class Call>
-void by_shape(const Shape &s, bool x32, bool f32, bool tail, Call &&call) {
+void by_shape(const Shape &s, bool x32, bool f32, bool tail, int opt, Call &&call) {
     auto types = [&](auto nth, auto shared, auto it) {
         auto ends = [&](auto x, auto f) {
-            if (tail) call(nth, shared, it, x, f, std::true_type());
-            else call(nth, shared, it, x, f, std::false_type());
+            if (tail) call(nth, shared, it, x, f, std::true_type(), std::integral_constant<int, GENERIC>());
+            else if (opt == JOIN) call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, JOIN>());
+            else if (opt == JOIN_POST) call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, JOIN_POST>());
+            else call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, GENERIC>());
         };
         if (f32) ends(std::true_type(), std::true_type());
         else if (x32) ends(std::true_type(), std::false_type());
@@ -797,12 +817,15 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
         pl.has = (p->f && (p->gate || p->post_w) ? HAS_A : 0) | (p->f && p->post_b ? HAS_AB : 0) | (p->y && (p->w || p->scale) ? HAS_W : 0) |
                  (p->y && (p->b || p->shift) ? HAS_S : 0);
         cut_runs(q, shape.threads / pl.L, shape.threads > 256 ? 512 : 1024, &pl);
-        const size_t lds = shape.threads / 64 * 8 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * ((p->C + 7) & ~7) * 4 : 0);
+        const int opt = !p->f || !p->y || p->post_b ? GENERIC : p->post ? JOIN_POST : JOIN;
+        if (opt && !(p->C & 7)) pl.has = HAS_A | HAS_W | HAS_S;
+        const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * ((p->C + 7) & ~7) * 4 : 0);
         const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
-        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail) {
+        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
             constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
             constexpr bool SH = decltype(shared)::value, X = decltype(x32)::value, F = decltype(f32)::value, TL = decltype(tail)::value;
-            hipLaunchKernelGGL((block_norm_rows_kernel<NTH, SH, IT, X, F, TL>), grid, dim3(NTH), lds, as_stream(stream), q, pl);
+            constexpr int OPT = decltype(what)::value;
+            hipLaunchKernelGGL((block_norm_rows_kernel<NTH, SH, IT, X, F, TL, OPT>), grid, dim3(NTH), lds, as_stream(stream), q, pl);
         });
         ONEDC_LAUNCH_CHECK();
         return 0;
@@ -824,7 +847,7 @@ int64_t onedc_block_norm_backward_ws_bytes(const onedc_block_norm_params *p, con
     Plan pl;
     backward_plan(q, &s, &pl);
     // the pictures' sums in front of the runs' (8-byte aligned)
-    return (q.B > 1 && wants_all(p, g) ? (int64_t)q.B * p->C * sizeof(Sums) : 0) + (int64_t)q.B * pl.runs * 4 * p->C * sizeof(float);
+    return (q.B > 1 && wants_all(p, g) ? (int64_t)q.B * p->C * PARTS * sizeof(double) : 0) + (int64_t)q.B * pl.runs * 4 * p->C * sizeof(float);
 }
 
 int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_block_norm_grad *g, void *stream) {
@@ -851,11 +874,11 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
             onedc_block_norm_params none = *p;
             if (p->B) {
                 hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)p->B * ((p->C + 63) / 64))), dim3(NT), 0, as_stream(stream),
-                                   none, *g, (const float *)nullptr, (Sums *)nullptr, 0);
+                                   none, *g, (const float *)nullptr, (double *)nullptr, 0);
                 ONEDC_LAUNCH_CHECK();
             }
             none.B = 0;
-            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 63) / 64), dim3(64), 0, as_stream(stream), none, *g, (const Sums *)nullptr);
+            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 15) / 16), dim3(NT), 0, as_stream(stream), none, *g, (const double *)nullptr);
             ONEDC_LAUNCH_CHECK();
         }
         return 0;
@@ -864,17 +887,19 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     Shape shape;
     Plan pl;
     const bool rows = backward_plan(q, &shape, &pl);
-    Sums *pictures = sums && q.B > 1 && wants_all(p, g) ? (Sums *)g->ws : nullptr;
-    float *part = sums ? (float *)((char *)g->ws + (pictures ? (int64_t)q.B * p->C * sizeof(Sums) : 0)) : nullptr;
+    double *pictures = sums && q.B > 1 && wants_all(p, g) ? (double *)g->ws : nullptr;
+    float *part = sums ? (float *)((char *)g->ws + (pictures ? (int64_t)q.B * p->C * PARTS * sizeof(double) : 0)) : nullptr;
     const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
     if (rows) {
         const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most, then the sums)
-        const size_t lds = shape.threads / 64 * 8 + scratch;
-        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail) {
+        const size_t lds = shape.threads / 64 * 16 + scratch;
+        const int opt = !p->f || !g->dy || !g->dxo || !g->dx || !g->df ? GENERIC : p->post ? JOIN_POST : JOIN;
+        by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
             constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
             constexpr bool SH = decltype(shared)::value, X = decltype(x32)::value, F = decltype(f32)::value, TL = decltype(tail)::value;
+            constexpr int OPT = decltype(what)::value;
             if constexpr (IT == 1 || (SH && IT == 2))
-                hipLaunchKernelGGL((block_norm_rows_backward_kernel<NTH, SH, IT, X, F, TL>), grid, dim3(NTH), lds, as_stream(stream), q, *g, pl, part);
+                hipLaunchKernelGGL((block_norm_rows_backward_kernel<NTH, SH, IT, X, F, TL, OPT>), grid, dim3(NTH), lds, as_stream(stream), q, *g, pl, part);
         });
     } else if (p->f_f32) {
         hipLaunchKernelGGL((block_norm_backward_kernel<true, true>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
@@ -889,7 +914,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
                            pictures, pl.runs);
         ONEDC_LAUNCH_CHECK();
         if (pictures) {
-            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 63) / 64), dim3(64), 0, as_stream(stream), q, *g, (const Sums *)pictures);
+            hipLaunchKernelGGL(block_norm_all_kernel, dim3((p->C + 15) / 16), dim3(NT), 0, as_stream(stream), q, *g, (const double *)pictures);
             ONEDC_LAUNCH_CHECK();
         }
     }
