@@ -248,7 +248,13 @@ def _ok(rc, name):
         raise KernelError(f"{name} failed with status {rc}")
 
 
+# the raw handle without a Stream object around it where torch has that call (2.7 us less a launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream():
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -763,56 +769,50 @@ def add(a, b, y):
 NORM_LAYER, NORM_RMS = 0, 1
 
 
-def _check_view(what, name, v, like=None, channels=None, dtypes=None):
-    """A View whose rows lie inside its buffer; the same tokens as `like`, `channels` wide, of one of `dtypes`."""
-    n = v.B * v.H * v.W
-    if min(v.B, v.H, v.W) < 0 or v.C < 1 or v.co < 0 or v.co + v.C > v.cs or not v.t.is_contiguous() or (
-            n and (n - 1) * v.cs + v.co + v.C > v.t.numel()):
-        raise KernelError(f"{what}: {name} is a view outside its buffer ({v.B} x {v.H} x {v.W} rows, channels {v.co}..{v.co + v.C} of {v.cs}, "
-                          f"{v.t.numel()} values{'' if v.t.is_contiguous() else ', not contiguous'})")
-    if like is not None and (v.B, v.H * v.W) != (like.B, like.H * like.W):
+def _span(what, name, v, n, channels, dtypes):
+    """Checks a View of n rows against its buffer and what the call needs of it (`channels` wide or None, one of `dtypes`) and returns where it
+    lies: (first byte, end, bytes between rows, bytes of a row, buffer)."""
+    t, cs, co, c = v.t, v.cs, v.co, v.C
+    if v.B * v.H * v.W != n:
+        raise KernelError(f"{what}: {name} has {v.B * v.H * v.W} rows, not {n}")
+    if c < 1 or co < 0 or co + c > cs or not t.is_contiguous() or (n and (n - 1) * cs + co + c > t.numel()):
+        raise KernelError(f"{what}: {name} is a view outside its buffer ({n} rows, channels {co}..{co + c} of {cs}, {t.numel()} values"
+                          f"{'' if t.is_contiguous() else ', not contiguous'})")
+    if channels is not None and c != channels:
+        raise KernelError(f"{what}: {name} has {c} channels, not {channels}")
+    if t.dtype not in dtypes:
+        raise KernelError(f"{what}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)} (current format: {act()})")
+    es = 4 if t.dtype == torch.float32 else 2
+    base = t.data_ptr()
+    lo = base + co * es
+    return lo, (lo + ((n - 1) * cs + c) * es if n else lo), cs * es, c * es, base
+
+
+def _check_pictures(what, name, v, like):
+    if (v.B, v.H * v.W) != (like.B, like.H * like.W):
         raise KernelError(f"{what}: {name} has {v.B} x {v.H * v.W} rows, not {like.B} x {like.H * like.W}")
-    if channels is not None and v.C != channels:
-        raise KernelError(f"{what}: {name} has {v.C} channels, not {channels}")
-    if dtypes is not None and v.t.dtype not in dtypes:
-        raise KernelError(f"{what}: {name} is {v.t.dtype}, not {' or '.join(str(d) for d in dtypes)} (current format: {act()})")
 
 
-def _check_device(what, *tensors):
+def _check_device(what, tensors):
     """Every tensor on the device whose current stream the launch goes to."""
     here = None
     for t in tensors:
-        if t is None:
-            continue
-        if t.device.type == "cuda" and here is None:
-            here = torch.cuda.current_device()
-        if t.device.type != "cuda" or t.device.index != here:
-            raise KernelError(f"{what}: a tensor is on {t.device}, the launch goes to {'no GPU' if here is None else f'cuda:{here}'} "
-                              "(torch.cuda.device selects it)")
+        if t is not None:
+            if here is None and t.is_cuda:
+                here = torch.cuda.current_device()
+            if t.get_device() != here:
+                raise KernelError(f"{what}: a tensor is on {t.device}, the launch goes to {'no GPU' if here is None else f'cuda:{here}'} "
+                                  "(torch.cuda.device selects it)")
 
 
-def _overlap(a, b):
-    """Whether two views share a value: their address ranges meet, and they are not different channels of rows of one pitch."""
-    ea, eb = a.t.element_size(), b.t.element_size()
-    a0, b0 = a.ptr + a.co * ea, b.ptr + b.co * eb
-    na, nb = a.B * a.H * a.W, b.B * b.H * b.W
-    if not na or not nb or a0 + ((na - 1) * a.cs + a.C) * ea <= b0 or b0 + ((nb - 1) * b.cs + b.C) * eb <= a0:
-        return False
-    pitch = a.cs * ea
-    if pitch != b.cs * eb:
-        return True
-    d = (b0 - a0) % pitch                             # where b's channels begin inside a's rows
-    return d < a.C * ea or d + b.C * eb > pitch
-
-
-def _same(a, b):
-    return a.ptr == b.ptr and a.cs == b.cs and a.co == b.co and a.t.dtype == b.t.dtype
-
-
-def _check_apart(what, name, out, *others):
-    """Nothing that the launch reads or writes elsewhere lies under `out`."""
+def _check_apart(what, name, out, others):
+    """Nothing that the launch reads or writes elsewhere lies under `out`: address ranges do not meet, or they are different channels of
+    rows of one pitch."""
     for o in others:
-        if o is not None and _overlap(out, o):
+        if o is None or out[1] <= o[0] or o[1] <= out[0] or out[0] == out[1] or o[0] == o[1]:
+            continue
+        d = (o[0] - out[0]) % out[2]                  # where the other's channels begin inside out's rows
+        if out[2] != o[2] or d < out[3] or d + o[3] > out[2]:
             raise KernelError(f"{what}: {name} shares memory with another operand")
 
 
@@ -833,30 +833,33 @@ def _row_stride(what, name, t, B, Cc):
     raise KernelError(f"{what}: {name} must be f32 [{Cc}] or [{B}, {Cc}] with dense rows, not {tuple(t.shape)} {t.dtype} strides {t.stride()}")
 
 
-def _block_norm_params(what, x, f, y_dtype, kind, eps, post, post_w, post_b, gate, alpha, w, b, scale, shift, has_y):
+def _block_norm_args(what, x, f, has_y, side, kind, post, post_w, post_b, gate, w, b, scale, shift):
+    """What forward and backward check alike: (rows, span of x, span of f or None, row strides of gate, scale, shift, types of f's side)."""
     if kind not in (NORM_LAYER, NORM_RMS):
         raise KernelError(f"{what}: kind must be NORM_LAYER or NORM_RMS, not {kind!r}")
-    _check_view(what, "x", x, dtypes=(a16(), torch.float32))
-    if x.B * x.H * x.W > 0x7fffffff or x.C > 1 << 20:
-        raise KernelError(f"{what}: {x.B * x.H * x.W} rows of {x.C} channels are more than the kernel indexes")
+    n, Cc, f32 = x.B * x.H * x.W, x.C, torch.float32
+    sx = _span(what, "x", x, n, None, (a16(), f32))
+    if n > 0x7fffffff or Cc > 1 << 20:
+        raise KernelError(f"{what}: {n} rows of {Cc} channels are more than the kernel indexes")
+    types = (a16(), f32) if x.t.dtype == f32 else (a16(),)
+    sf = None
     if f is not None:
-        _check_view(what, "f", f, x, x.C, (a16(), torch.float32) if x.f32 else (a16(),))
-        if y_dtype is not None and f.t.dtype != y_dtype:
-            raise KernelError(f"{what}: f is {f.t.dtype}, the normalised side {y_dtype}: one type")
+        _check_pictures(what, "f", f, x)
+        sf = _span(what, "f", f, n, Cc, types)
+        types = (f.t.dtype,)
+        if side is not None and side != f.t.dtype:
+            raise KernelError(f"{what}: f is {f.t.dtype}, the normalised side {side}: one type")
     elif post or gate is not None:
         raise KernelError(f"{what}: a post norm or a gate needs f")
-    if (post_w is not None or post_b is not None) and not post:
+    if not post and (post_w is not None or post_b is not None):
         raise KernelError(f"{what}: post_w / post_b need post=True")
-    if not has_y and any(t is not None for t in (w, b, scale, shift)):
+    if not has_y and (w is not None or b is not None or scale is not None or shift is not None):
         raise KernelError(f"{what}: w, b, scale and shift belong to the norm behind the join, which this call has not")
     for name, t in (("post_w", post_w), ("post_b", post_b), ("w", w), ("b", b)):
-        _check_vector(what, name, t, x.C)
-    p = BlockNormParams(x.ptr, None if f is None else f.ptr, None, None, _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale),
-                        _ptr(shift), x.B, x.H * x.W, x.C, x.cs, x.co, 0 if f is None else f.cs, 0 if f is None else f.co, 0, 0, 0, 0,
-                        _row_stride(what, "gate", gate, x.B, x.C), _row_stride(what, "scale", scale, x.B, x.C),
-                        _row_stride(what, "shift", shift, x.B, x.C), kind, int(bool(post)), int(x.f32),
-                        int(f.f32 if f is not None else y_dtype == torch.float32), alpha, eps)
-    return p
+        if t is not None:
+            _check_vector(what, name, t, Cc)
+    return (n, sx, sf, _row_stride(what, "gate", gate, x.B, Cc), _row_stride(what, "scale", scale, x.B, Cc),
+            _row_stride(what, "shift", shift, x.B, Cc), types)
 
 
 def block_norm(x, y=None, *, f=None, xo=None, kind=NORM_LAYER, eps=1e-5, post=False, post_w=None, post_b=None, gate=None, alpha=1.0,
@@ -872,17 +875,23 @@ def block_norm(x, y=None, *, f=None, xo=None, kind=NORM_LAYER, eps=1e-5, post=Fa
         raise KernelError(f"{what}: neither y nor xo: nothing to compute")
     if (f is None) != (xo is None):
         raise KernelError(f"{what}: f and xo come together (the branch and the joined stream)")
-    p = _block_norm_params(what, x, f, None if y is None else y.t.dtype, kind, eps, post, post_w, post_b, gate, alpha, w, b, scale, shift,
-                           y is not None)
-    if y is not None:
-        _check_view(what, "y", y, x, x.C, (a16(), torch.float32) if x.f32 else (a16(),))
-        _check_apart(what, "y", y, x, f, xo)
-        p.y, p.y_cs, p.y_co = y.ptr, y.cs, y.co
+    n, sx, sf, gate_rs, scale_rs, shift_rs, types = _block_norm_args(what, x, f, y is not None, None if y is None else y.t.dtype, kind, post,
+                                                                    post_w, post_b, gate, w, b, scale, shift)
+    sy = so = None
     if xo is not None:
-        _check_view(what, "xo", xo, x, x.C, (x.t.dtype,))
-        _check_apart(what, "xo", xo, None if _same(xo, x) else x, f)
-        p.xo, p.xo_cs, p.xo_co = xo.ptr, xo.cs, xo.co
-    _check_device(what, *(v.t for v in (x, f, xo, y) if v is not None), post_w, post_b, gate, w, b, scale, shift)
+        _check_pictures(what, "xo", xo, x)
+        so = _span(what, "xo", xo, n, x.C, (x.t.dtype,))
+        _check_apart(what, "xo", so, (None if so == sx else sx, sf))
+    if y is not None:
+        _check_pictures(what, "y", y, x)
+        sy = _span(what, "y", y, n, x.C, types)
+        _check_apart(what, "y", sy, (sx, sf, so))
+    _check_device(what, (x.t, None if f is None else f.t, None if xo is None else xo.t, None if y is None else y.t, post_w, post_b, gate, w, b,
+                         scale, shift))
+    p = BlockNormParams(sx[4], sf and sf[4], so and so[4], sy and sy[4], _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale),
+                        _ptr(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, xo.cs if so else 0, xo.co if so else 0,
+                        y.cs if sy else 0, y.co if sy else 0, gate_rs, scale_rs, shift_rs, kind, int(bool(post)), int(x.t.dtype == torch.float32),
+                        int((f or y).t.dtype == torch.float32), alpha, eps)
     _ok(lib().onedc_block_norm(C.byref(p), stream()), "onedc_block_norm")
     return xo, y
 
@@ -893,36 +902,41 @@ def block_norm_backward(x, dy, dx=None, *, dxo=None, f=None, df=None, kind=NORM_
     """Backward pass of block_norm.  x: the JOINED stream as block_norm stored it (its xo; its x where there was no f); dy, dxo: the
     gradients of y and xo, None where the loss does not depend on them.  Writes dx (the gradient of the stream in front of the join), df, and
     the parameter gradients that are asked for, f32, dense: [C], and [B, C] for gate / scale / shift where those have a row per picture.
-    dx may be dxo, df may be dy.  Sums over rows run in a fixed order: the same bits every time."""
+    dx may be dxo, df may be dy.  Sums over rows run in a fixed order: the same bits every time.  Returns (dx, df)."""
     what = "block_norm_backward"
     if dy is None and dxo is None:
         raise KernelError(f"{what}: neither dy nor dxo: no gradient to pass on")
-    p = _block_norm_params(what, x, f, dy.t.dtype if dy is not None else None if df is None else df.t.dtype, kind, eps, post, post_w, post_b,
-                           gate, alpha, w, b, scale, shift, dy is not None)
-    side = (a16(), torch.float32) if x.f32 else (a16(),)
-    g = BlockNormGrad()
-    if f is None and any(t is not None for t in (df, d_gate, d_post_w, d_post_b)):
+    if f is None and (df is not None or d_gate is not None or d_post_w is not None or d_post_b is not None):
         raise KernelError(f"{what}: df, d_gate, d_post_w and d_post_b need f")
-    for name, v, dtypes in (("dy", dy, side), ("dxo", dxo, (x.t.dtype,)), ("dx", dx, (x.t.dtype,)), ("df", df, side)):
+    n, sx, sf, gate_rs, scale_rs, shift_rs, types = _block_norm_args(
+        what, x, f, dy is not None, dy.t.dtype if dy is not None else None if df is None else df.t.dtype, kind, post, post_w, post_b, gate, w, b,
+        scale, shift)
+    spans = {}
+    for name, v, of in (("dy", dy, types), ("dxo", dxo, (x.t.dtype,)), ("dx", dx, (x.t.dtype,)), ("df", df, types)):
         if v is not None:
-            _check_view(what, name, v, x, x.C, dtypes)
-            setattr(g, name, v.ptr)
-            setattr(g, name + "_cs", v.cs)
-            setattr(g, name + "_co", v.co)
+            _check_pictures(what, name, v, x)
+            spans[name] = _span(what, name, v, n, x.C, of)
+    sy, so, sdx, sdf = (spans.get(name) for name in ("dy", "dxo", "dx", "df"))
     if dx is not None:
-        _check_apart(what, "dx", dx, x, f, dy, df, None if dxo is None or _same(dx, dxo) else dxo)
+        _check_apart(what, "dx", sdx, (sx, sf, sy, sdf, None if sdx == so else so))
     if df is not None:
-        _check_apart(what, "df", df, x, f, dxo, None if dy is None or _same(df, dy) else dy)
-    grads = (("d_post_w", d_post_w, post_w, 0), ("d_post_b", d_post_b, post_b, 0), ("d_gate", d_gate, gate, p.gate_rs), ("d_w", d_w, w, 0),
-             ("d_b", d_b, b, 0), ("d_scale", d_scale, scale, p.scale_rs), ("d_shift", d_shift, shift, p.shift_rs))
-    for name, t, of, rs in grads:
+        _check_apart(what, "df", sdf, (sx, sf, so, None if sdf == sy else sy))
+    for name, t, of, rows in (("d_post_w", d_post_w, post_w, 1), ("d_post_b", d_post_b, post_b, 1), ("d_gate", d_gate, gate, x.B if gate_rs else 1),
+                              ("d_w", d_w, w, 1), ("d_b", d_b, b, 1), ("d_scale", d_scale, scale, x.B if scale_rs else 1),
+                              ("d_shift", d_shift, shift, x.B if shift_rs else 1)):
         if t is not None:
             if of is None:
                 raise KernelError(f"{what}: {name} of a parameter that the call has not")
-            _check_vector(what, name, t, x.C * (x.B if rs else 1))
-            setattr(g, name, t.data_ptr())
-    _check_device(what, *(v.t for v in (x, f, dy, dxo, dx, df) if v is not None), post_w, post_b, gate, w, b, scale, shift,
-                  *(t for _, t, _, _ in grads))
+            _check_vector(what, name, t, x.C * rows)
+    _check_device(what, [v.t for v in (x, f, dy, dxo, dx, df) if v is not None] +
+                  [post_w, post_b, gate, w, b, scale, shift, d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift])
+    side = f or dy
+    p = BlockNormParams(sx[4], sf and sf[4], None, None, _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale), _ptr(shift), x.B,
+                        x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, 0, 0, 0, 0, gate_rs, scale_rs, shift_rs, kind,
+                        int(bool(post)), int(x.t.dtype == torch.float32), int(side is not None and side.t.dtype == torch.float32), alpha, eps)
+    g = BlockNormGrad(sy and sy[4], so and so[4], sdx and sdx[4], sdf and sdf[4], _ptr(d_post_w), _ptr(d_post_b), _ptr(d_gate), _ptr(d_w),
+                      _ptr(d_b), _ptr(d_scale), _ptr(d_shift), None, 0, dy.cs if sy else 0, dy.co if sy else 0, dxo.cs if so else 0,
+                      dxo.co if so else 0, dx.cs if sdx else 0, dx.co if sdx else 0, df.cs if sdf else 0, df.co if sdf else 0)
     need = lib().onedc_block_norm_backward_ws_bytes(C.byref(p), C.byref(g))
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=x.t.device)          # the call's own: two captured graphs never share it
@@ -963,31 +977,44 @@ def rotary_axes(plan, pos, q, qo=None, k=None, ko=None, inverse=False):
     what = "rotary_axes"
     if k is None and ko is not None:
         raise KernelError(f"{what}: ko without k")
-    qo = q if qo is None else qo
-    ko = k if ko is None else ko
-    _check_view(what, "q", q, dtypes=(a16(), torch.float32))
-    for name, v, like in (("qo", qo, q), ("k", k, q), ("ko", ko, q)):
-        if v is not None:
-            _check_view(what, name, v, like, None if name == "k" else (q if name == "qo" else k).C, (q.t.dtype,))
-    for name, v in (("q", q), ("k", k)):
-        if v is not None and (v.C % plan.D or v.C // plan.D > 4096):
-            raise KernelError(f"{what}: {name} has {v.C} channels: not 1 to 4096 heads of {plan.D}")
-    N = q.H * q.W
-    if q.B * N > 0x7fffffff:
-        raise KernelError(f"{what}: {q.B * N} rows are more than the kernel indexes")
-    if pos.dtype not in (torch.int32, torch.float32) or not pos.is_contiguous() or tuple(pos.shape) not in (
-            (N, plan.axes), (1, N, plan.axes), (q.B, N, plan.axes)):
-        raise KernelError(f"{what}: pos must be contiguous int32 or f32 [{N}, {plan.axes}] or [{q.B}, {N}, {plan.axes}], not "
-                          f"{tuple(pos.shape)} {pos.dtype}")
-    _check_apart(what, "qo", qo, None if _same(qo, q) else q, k, ko)
+    n, N, D = q.B * q.H * q.W, q.H * q.W, plan.D
+    sq = _span(what, "q", q, n, None, (a16(), torch.float32))
+    dtype = (q.t.dtype,)
+    sk = sko = None
     if k is not None:
-        _check_apart(what, "ko", ko, None if _same(ko, k) else k, q)
-    _check_device(what, q.t, qo.t, *(v.t for v in (k, ko) if v is not None), pos, plan.turns, plan.axis)
-    p = RotaryParams(q.ptr, qo.ptr, None if k is None else k.ptr, None if k is None else ko.ptr, pos.data_ptr(), plan.turns.data_ptr(),
-                     plan.axis.data_ptr(), q.B, N, plan.D, plan.pairs, plan.axes, q.C // plan.D, 0 if k is None else k.C // plan.D, q.cs, q.co,
-                     qo.cs, qo.co, 0 if k is None else k.cs, 0 if k is None else k.co, 0 if k is None else ko.cs, 0 if k is None else ko.co,
-                     int(q.f32), int(pos.dtype == torch.float32), int(plan.neighbours), int(bool(inverse)),
-                     N * plan.axes if pos.dim() == 3 and pos.shape[0] > 1 else 0)
+        _check_pictures(what, "k", k, q)
+        sk = sko = _span(what, "k", k, n, None, dtype)
+        if ko is None:
+            ko = k
+        else:
+            _check_pictures(what, "ko", ko, q)
+            sko = _span(what, "ko", ko, n, k.C, dtype)
+            _check_apart(what, "ko", sko, (None if sko == sk else sk, sq))
+    if qo is None:
+        qo, sqo = q, sq
+    else:
+        _check_pictures(what, "qo", qo, q)
+        sqo = _span(what, "qo", qo, n, q.C, dtype)
+    _check_apart(what, "qo", sqo, (None if sqo == sq else sq, sk, sko))
+    _check_apart(what, "q", sq, (sko,))
+    qh, kh = q.C // D, 0 if k is None else k.C // D
+    for name, v, h in (("q", q, qh), ("k", k, kh)):
+        if v is not None and (v.C != h * D or h > 4096):
+            raise KernelError(f"{what}: {name} has {v.C} channels: not 1 to 4096 heads of {D}")
+    if n > 0x7fffffff:
+        raise KernelError(f"{what}: {n} rows are more than the kernel indexes")
+    shape = tuple(pos.shape)
+    if pos.dtype not in (torch.int32, torch.float32) or not pos.is_contiguous() or (
+            shape != (N, plan.axes) and shape != (q.B, N, plan.axes) and shape != (1, N, plan.axes)):
+        raise KernelError(f"{what}: pos must be contiguous int32 or f32 [{N}, {plan.axes}] or [{q.B}, {N}, {plan.axes}], not "
+                          f"{shape} {pos.dtype}")
+    _check_device(what, (q.t, qo.t, None if k is None else k.t, None if k is None else ko.t, pos, plan.turns, plan.axis))
+    if not n:
+        return qo, ko
+    p = RotaryParams(sq[4], sqo[4], sk and sk[4], sko and sko[4], pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), q.B, N, D, plan.pairs,
+                     plan.axes, qh, kh, q.cs, q.co, qo.cs, qo.co, k.cs if kh else 0, k.co if kh else 0, ko.cs if kh else 0, ko.co if kh else 0,
+                     int(q.t.dtype == torch.float32), int(pos.dtype == torch.float32), int(plan.neighbours), int(bool(inverse)),
+                     N * plan.axes if len(shape) == 3 and shape[0] > 1 else 0)
     _ok(lib().onedc_rotary_axes(C.byref(p), stream()), "onedc_rotary_axes")
     return qo, ko
 
@@ -1019,29 +1046,27 @@ def mxfp4_quantize(x, q=None):
     """x: View (16-bit or f32), its rows (tokens) quantised along the channels into q (default: a new MxFp4).  A block of 32 with a NaN
     or an infinity reads back as NaN."""
     what = "mxfp4_quantize"
-    _check_view(what, "x", x, dtypes=(a16(), torch.float32))
     rows = x.B * x.H * x.W
+    sx = _span(what, "x", x, rows, None, (a16(), torch.float32))
     if q is None:
         q = mxfp4_empty(rows, x.C, x.t.device)
     elif (q.rows, q.K) != (rows, x.C):
         raise KernelError(f"{what}: q holds {q.rows} x {q.K} values, x has {rows} x {x.C}")
-    _check_device(what, x.t, q.codes, q.scales)
+    _check_device(what, (x.t, q.codes, q.scales))
     if rows:
-        _ok(lib().onedc_mxfp4_quantize(x.ptr, int(x.f32), x.cs, x.co, q.codes.data_ptr(), q.scales.data_ptr(), rows, x.C, stream()),
-            "onedc_mxfp4_quantize")
+        _ok(lib().onedc_mxfp4_quantize(sx[4], int(x.t.dtype == torch.float32), x.cs, x.co, q.codes.data_ptr(), q.scales.data_ptr(), rows, x.C,
+                                       stream()), "onedc_mxfp4_quantize")
     return q
 
 
 def mxfp4_dequantize(q, y):
     """The values that q stands for, into the View y (16-bit, rounded, or f32, exact)."""
     what = "mxfp4_dequantize"
-    _check_view(what, "y", y, channels=q.K, dtypes=(a16(), torch.float32))
-    if y.B * y.H * y.W != q.rows:
-        raise KernelError(f"{what}: y has {y.B * y.H * y.W} rows, q {q.rows}")
-    _check_device(what, y.t, q.codes, q.scales)
+    sy = _span(what, "y", y, q.rows, q.K, (a16(), torch.float32))
+    _check_device(what, (y.t, q.codes, q.scales))
     if q.rows:
-        _ok(lib().onedc_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), y.ptr, int(y.f32), y.cs, y.co, q.rows, q.K, stream()),
-            "onedc_mxfp4_dequantize")
+        _ok(lib().onedc_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), sy[4], int(y.t.dtype == torch.float32), y.cs, y.co, q.rows, q.K,
+                                         stream()), "onedc_mxfp4_dequantize")
     return y
 
 
@@ -1058,32 +1083,32 @@ def mxfp4_linear(x, w, bias, y, *, epi=EPI_LINEAR, slope=0.01, alpha=1.0, res=No
         raise KernelError(f"{what}: epilogue {epi!r} is not one of LINEAR, LEAKY, SILU, GEGLU")
     if epi == EPI_GEGLU and w.rows % 32:
         raise KernelError(f"{what}: a gated layer needs whole blocks of 16 values and 16 gates, not {w.rows} rows")
-    held = isinstance(x, MxFp4)
-    rows, kx = (x.rows, x.K) if held else (x.B * x.H * x.W, x.C)
-    if not held:
-        _check_view(what, "x", x, dtypes=(a16(), torch.float32))
+    held, f32 = isinstance(x, MxFp4), torch.float32
+    sx = None
+    if held:
+        rows, kx = x.rows, x.K
+    else:
+        rows, kx = x.B * x.H * x.W, x.C
+        sx = _span(what, "x", x, rows, None, (a16(), f32))
     if kx != w.K:
         raise KernelError(f"{what}: x has {kx} values a row, w {w.K}")
     out = w.rows // 2 if epi == EPI_GEGLU else w.rows
     if out < 1 or w.rows > 1 << 24:
         raise KernelError(f"{what}: no layer of {w.rows} outputs")
-    _check_view(what, "y", y, channels=out, dtypes=(a16(), torch.float32))
-    if y.B * y.H * y.W != rows:
-        raise KernelError(f"{what}: y has {y.B * y.H * y.W} rows, x {rows}")
+    sy = _span(what, "y", y, rows, out, (a16(), f32))
     _check_vector(what, "bias", bias, w.rows)
+    sr = None
     if res is not None:
-        _check_view(what, "res", res, y, out, (y.t.dtype,))
-        _check_apart(what, "y", y, None if _same(y, res) else res)
-    if not held:
-        _check_apart(what, "y", y, x)
-    _check_device(what, *((x.codes, x.scales) if held else (x.t,)), w.codes, w.scales, y.t, bias, None if res is None else res.t)
+        sr = _span(what, "res", res, rows, out, (y.t.dtype,))
+    _check_apart(what, "y", sy, (sx, None if sr == sy else sr))
+    _check_device(what, (x.codes if held else x.t, x.scales if held else None, w.codes, w.scales, y.t, bias, None if res is None else res.t))
     if not rows:
         return y
     if not held and rows > MXFP4_ROWS_RAW:
         x, held = mxfp4_quantize(x), True
-    p = MxFp4Params(x.codes.data_ptr() if held else None, x.scales.data_ptr() if held else None, None if held else x.ptr, w.codes.data_ptr(),
-                    w.scales.data_ptr(), _ptr(bias), None if res is None else res.ptr, y.ptr, rows, w.rows, w.K, 0 if held else x.cs,
-                    0 if held else x.co, 0 if held else int(x.f32), y.cs, y.co, 0 if res is None else res.cs, 0 if res is None else res.co,
-                    int(y.f32), epi, alpha, slope)
+    p = MxFp4Params(x.codes.data_ptr() if held else None, x.scales.data_ptr() if held else None, None if held else sx[4], w.codes.data_ptr(),
+                    w.scales.data_ptr(), _ptr(bias), sr and sr[4], sy[4], rows, w.rows, w.K, 0 if held else x.cs, 0 if held else x.co,
+                    int(not held and x.t.dtype == f32), y.cs, y.co, res.cs if sr else 0, res.co if sr else 0, int(y.t.dtype == f32), epi, alpha,
+                    slope)
     _ok(lib().onedc_mxfp4_linear(C.byref(p), stream()), "onedc_mxfp4_linear")
     return y
