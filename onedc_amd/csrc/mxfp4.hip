@@ -182,6 +182,14 @@ __device__ __forceinline__ f32x4 mfma_fp4(uint4 a, uint4 b, f32x4 c, uint32_t sa
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, J, (int)sa, J, (int)sb);
 }
 
+// the same over 32 x 32 rows and 64 values: lane l holds row l % 32, values 32 (l / 32) .. + 31
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+template <int J>
+__device__ __forceinline__ f32x16 mfma_fp4_32(uint4 a, uint4 b, f32x16 c, uint32_t sa, uint32_t sb) {
+    const i32x8 va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, vb = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, J, (int)sa, J, (int)sb);
+}
+
 __device__ __forceinline__ float activation(const onedc_mxfp4_params &p, float v) {
     return p.epi == ONEDC_EPI_SILU ? silu_f(v) : p.epi == ONEDC_EPI_LEAKY ? leaky(v, p.slope) : v;
 }
@@ -226,131 +234,121 @@ __device__ __forceinline__ void store8(const onedc_mxfp4_params &p, int64_t m, i
 }
 
 // ---- few rows: the weights' bytes bound it -------------------------------------------------------------------------------------------
-// A workgroup computes 32 weight rows x 16 FM activation rows; its eight waves take every eighth 128-value step of K straight from
-// memory (each weight byte is read once, 64 bytes of 16 rows an instruction) and their sums are added through LDS in wave order.  Raw rows
-// are quantised by the lane that multiplies them, once per workgroup: 70 instructions a step against 2 KB of weights.
-constexpr int SKW = 8;
-template <int FM, bool RAW, bool VEC>
+// A workgroup computes 32 weight rows x 16 activation rows; its sixteen waves take every sixteenth 128-value step of K straight from
+// memory (each weight byte is read once, 64 bytes of 16 rows an instruction; four steps' loads in flight a wave) and their sums are added
+// through LDS in wave order.  Raw rows are quantised by the lane that multiplies them, once a workgroup: 70 instructions a step against
+// 2 KB of weights.
+constexpr int SKW = 16;
+// the 32 values of a lane's block as codes and scale
+template <bool F32, bool VEC>
+struct Block32 {
+    Eight<F32, VEC> v[4];
+    __device__ __forceinline__ void load(const void *x, int64_t at, int left) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j].load(x, at + j * 8, left - j * 8);
+    }
+    __device__ __forceinline__ uint4 codes(uint32_t &s) const {
+        s = block_scale(max(max(v[0].amax_bits(), v[1].amax_bits()), max(v[2].amax_bits(), v[3].amax_bits())));
+        return make_uint4(v[0].codes(s), v[1].codes(s), v[2].codes(s), v[3].codes(s));
+    }
+};
+// RAW 0: codes, 1: 16-bit rows, 2: f32 rows
+template <int RAW, bool VEC>
 __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, int steps, int whole) {
-    __shared__ __attribute__((aligned(16))) float red[SKW][FM][2][16][20];
+    __shared__ __attribute__((aligned(16))) float red[SKW][2][16][20];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kb = lane >> 4;
     const int nt = (p.N + 31) / 32;
     const int n0 = (int)(blockIdx.x % nt) * 32;
-    const int64_t m0 = (int64_t)(blockIdx.x / nt) * (16 * FM);
+    const int64_t m0 = (int64_t)(blockIdx.x / nt) * 16, m = m0 + r < p.M ? m0 + r : p.M - 1;
     const int na = min(n0 + r, p.N - 1), nc = min(n0 + 16 + r, p.N - 1);
     const uint4 *wa = (const uint4 *)p.wc + (int64_t)na * steps * 4 + kb, *wb = (const uint4 *)p.wc + (int64_t)nc * steps * 4 + kb;
     const uint8_t *sa = (const uint8_t *)p.ws + (int64_t)na * steps * 4 + kb, *sb = (const uint8_t *)p.ws + (int64_t)nc * steps * 4 + kb;
-    int64_t m[FM];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) m[i] = m0 + i * 16 + r < p.M ? m0 + i * 16 + r : p.M - 1;
-    f32x4 acc[FM][2];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = FM == 1 ? 4 : 2;               // steps whose loads are in flight together
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    constexpr int U = RAW == 2 ? 2 : 4;              // steps whose loads are in flight together (behind the last: the last again, as zeros)
     for (int s0 = wave; s0 < steps; s0 += SKW * U) {
-        uint4 a[U], c[U], x[FM][U];
-        uint32_t xa[U], xc[U], sx[FM][U];
+        uint4 a[U], c[U], x[U];
+        uint32_t xa[U], xc[U], sx[U];
+        Block32<RAW == 2, VEC> raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = min(s0 + u * SKW, steps - 1);
+            const int s = min(s0 + u * SKW, steps - 1), k0 = s * 128 + kb * 32;
             a[u] = wa[s * 4], c[u] = wb[s * 4];
             xa[u] = sa[s * 4], xc[u] = sb[s * 4];
-            if (!RAW)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    x[i][u] = ((const uint4 *)p.xc)[(m[i] * steps + s) * 4 + kb];
-                    sx[i][u] = ((const uint8_t *)p.xs)[(m[i] * steps + s) * 4 + kb];
-                }
+            if (RAW) {
+                raw[u].load(p.xr, m * p.xr_cs + p.xr_co + k0, s0 + u * SKW < steps ? p.K - k0 : 0);
+            } else {
+                x[u] = ((const uint4 *)p.xc)[(m * steps + s) * 4 + kb];
+                sx[u] = ((const uint8_t *)p.xs)[(m * steps + s) * 4 + kb];
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = s0 + u * SKW;
-            if (s >= steps) break;
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                if (RAW) {
-                    const int k0 = s * 128 + kb * 32;
-                    const int64_t at = m[i] * p.xr_cs + p.xr_co + k0;
-                    uint32_t top = 0;
-                    if (p.xr_f32) {
-                        Eight<true, VEC> v[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j].load(p.xr, at + j * 8, p.K - k0 - j * 8), top = max(top, v[j].amax_bits());
-                        sx[i][u] = block_scale(top);
-                        x[i][u] = make_uint4(v[0].codes(sx[i][u]), v[1].codes(sx[i][u]), v[2].codes(sx[i][u]), v[3].codes(sx[i][u]));
-                    } else {
-                        Eight<false, VEC> v[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j].load(p.xr, at + j * 8, p.K - k0 - j * 8), top = max(top, v[j].amax_bits());
-                        sx[i][u] = block_scale(top);
-                        x[i][u] = make_uint4(v[0].codes(sx[i][u]), v[1].codes(sx[i][u]), v[2].codes(sx[i][u]), v[3].codes(sx[i][u]));
-                    }
-                }
-                acc[i][0] = mfma_fp4<0>(a[u], x[i][u], acc[i][0], xa[u], sx[i][u]);
-                acc[i][1] = mfma_fp4<0>(c[u], x[i][u], acc[i][1], xc[u], sx[i][u]);
-            }
+            if (s0 + u * SKW >= steps) break;
+            if (RAW) x[u] = raw[u].codes(sx[u]);
+            acc[0] = mfma_fp4<0>(a[u], x[u], acc[0], xa[u], sx[u]);
+            acc[1] = mfma_fp4<0>(c[u], x[u], acc[1], xc[u], sx[u]);
         }
     }
     // lane: activation row r, weight rows 4 kb + e of each half
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) *(f32x4 *)&red[wave][i][h][r][kb * 4] = acc[i][h];
+    *(f32x4 *)&red[wave][0][r][kb * 4] = acc[0];
+    *(f32x4 *)&red[wave][1][r][kb * 4] = acc[1];
     __syncthreads();
     const bool glu = p.epi == ONEDC_EPI_GEGLU;
     const int out = glu ? p.N / 2 : p.N, pieces = glu ? 2 : 4;             // eight outputs each
-    for (int t = threadIdx.x; t < 16 * FM * pieces; t += 64 * SKW) {
-        const int row = t / pieces, piece = t - row * pieces;
-        if (m0 + row >= p.M) continue;
-        float v[8];
+    // first one sum a thread (512 of them), then the row's pieces
+    float total = 0.f;
+    const int tr = (threadIdx.x >> 5) & 15, tn = threadIdx.x & 31;
+    if (threadIdx.x < 512) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int n = piece * 8 + j;
-            float a = 0.f, g = 0.f;
-#pragma unroll
-            for (int w = 0; w < SKW; ++w) a += red[w][row >> 4][n >> 4][row & 15][n & 15];
-            if (glu) {
-#pragma unroll
-                for (int w = 0; w < SKW; ++w) g += red[w][row >> 4][1][row & 15][n];
-                v[j] = (p.alpha * a + bias_of(p, n0 + n)) * gelu_f(p.alpha * g + bias_of(p, n0 + 16 + n));
-            } else {
-                v[j] = activation(p, p.alpha * a + bias_of(p, n0 + n));
-            }
-        }
-        const int n = (glu ? n0 / 2 : n0) + piece * 8;
-        if (n < out) store8(p, m0 + row, n, out, v, whole && n + 8 <= out);
+        for (int w = 0; w < SKW; ++w) total += red[w][tn >> 4][tr][tn & 15];
+        total = p.alpha * total + bias_of(p, n0 + tn);
     }
+    __syncthreads();
+    float (*const row32)[36] = (float (*)[36])&red[0][0][0][0];
+    if (threadIdx.x < 512) row32[tr][tn] = total;
+    __syncthreads();
+    const int t = threadIdx.x, row = t / pieces, c = (t - row * pieces) * 8, n = (glu ? n0 / 2 : n0) + c;
+    if (t >= 16 * pieces || m0 + row >= p.M || n >= out) return;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = glu ? row32[row][c + j] * gelu_f(row32[row][16 + c + j]) : activation(p, row32[row][c + j]);
+    store8(p, m0 + row, n, out, v, whole && n + 8 <= out);
 }
 
 // ---- tiles: the matrix cores and what feeds them bound it ---------------------------------------------------------------------------------
-// A workgroup of 2 x 2 waves computes 32 FN weight rows x 32 FM activation rows.  A stage is one 128-value step of both operands, 64 bytes
-// of codes a row, LDS-DMA'd into a ring of NST; the 16-byte chunks of a row are placed at chunk ^ (row / 2 % 4), which puts the eight
-// rows that a fragment read touches together on different banks.  Scales come four steps (16 bytes a row) at a time, one such group ahead;
-// two byte permutes collect a lane's four scales into the word that the matrix instruction picks from.
+// A workgroup of WN x WM waves computes 32 WN FN weight rows x 32 WM FM activation rows.  A stage is KS steps of 128 values of both operands,
+// LDS-DMA'd into a ring of NST: rows of 64 KS bytes whose 16-byte chunks are permuted so that the rows that a fragment read touches
+// together lie on different banks.  Scales come eight steps (32 bytes a row) at a time; byte permutes collect a lane's scales into the
+// words that the matrix instruction picks from.
 // The DMA is written as instructions (it has no destination register): behind the builtin the compiler drains every DMA in flight
 // before each LDS read.
 #define MX_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+// (2 GB at most: a tile's own rows span far less, and offsets from 0xffff0000 on are behind every end)
 __device__ __forceinline__ i32x4 raw_rsrc(const void *base, int64_t bytes) {
     const uint64_t a = (uint64_t)base;
-    return i32x4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(uint32_t)(bytes < 0xfffff000ll ? bytes : 0xfffff000ll), 0x00020000};
+    return i32x4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(bytes < 0x7ffffff0ll ? bytes : 0x7ffffff0ll), 0x00020000};
 }
 // 16 bytes a lane from base + voff + soff to lds + 16 lane; a lane whose voff lies behind the descriptor's end writes zeros
-// (m0 is reserved: nothing else in these kernels reads it)
+// (m0 is reserved: nothing else in these kernels reads it.  No memory clobber: LDS reads may pass it, the waits and barriers order what has to be)
 __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned voff, unsigned soff, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
-template <int FN, int FM, int NST, int OCC>
-__global__ __launch_bounds__(256, OCC) void tile_kernel(onedc_mxfp4_params p, int steps, int tiles_n, int tiles_m, int whole) {
-    constexpr int TN = 32 * FN, TM = 32 * FM, STAGE = (TN + TM) * 64, WN = TN / 64, WM = TM / 64, NI = WN + WM;
-    constexpr int GROUP = (TN + TM) * 16, NSC = (TN + TM + 255) / 256, RING = NST * STAGE;     // scales of four steps, behind the ring
+// WN x WM waves of FN x FM blocks of 32 x 32
+template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC>
+__global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_params p, int steps, int tiles_n, int tiles_m, int whole) {
+    constexpr int NW = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, ROW = 64 * KS, STAGE = (TN + TM) * ROW;
+    constexpr int RI = 16 / KS;                      // rows of a DMA instruction
+    constexpr int IN = TN / RI / NW, IM = TM / RI / NW, NI = IN + IM;
+    constexpr int GROUP = (TN + TM) * 32, NSC = ((TN + TM) / 32 + NW - 1) / NW, RING = NST * STAGE;     // scales of eight steps, behind the ring
+    constexpr int GS = 8 / KS;                       // stages of a group of scales
+    static_assert(TN % (RI * NW) == 0 && TM % (RI * NW) == 0, "whole DMA instructions a wave");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, kb = lane >> 4;
-    const int wn = wave >> 1, wm = wave & 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, kb = lane >> 5;
+    const int wn = wave / WM, wm = wave - wn * WM;
     // tiles that run at the same time on one XCD share operands: eight rows of tiles deep, then along n
     const int logical = xcd_logical_tile(blockIdx.x, tiles_n * tiles_m);
     const int band = 8 * tiles_n, b0 = logical / band, in = logical - b0 * band, deep = min(8, tiles_m - b0 * 8);
@@ -358,31 +356,37 @@ __global__ __launch_bounds__(256, OCC) void tile_kernel(onedc_mxfp4_params p, in
     const int n0 = tn * TN;
     const int64_t m0 = (int64_t)tm * TM;
 
-    // codes: rows past the last read zeros (their byte offset lies behind the descriptor's end)
+    // codes: rows past the last read zeros (their byte offset lies behind the descriptor's end), and so does the second half of a last
+    // stage that ends with an odd step
     const unsigned row_bytes = (unsigned)steps * 64;
     const i32x4 w_rsrc = raw_rsrc((const char *)p.wc + (int64_t)n0 * row_bytes, (int64_t)(p.N - n0) * row_bytes);
     const i32x4 x_rsrc = raw_rsrc((const char *)p.xc + m0 * row_bytes, (p.M - m0) * (int64_t)row_bytes);
-    const int srow = wave * 16 + (lane >> 2);
-    const unsigned schunk = ((lane & 3) ^ ((lane >> 3) & 3)) << 4;
-    const unsigned voff = (unsigned)srow * row_bytes + schunk;
-    unsigned wv[WN], xv[WM];
+    const int srow = wave * RI + lane / (4 * KS);
+    const int schunk = KS == 2 ? (lane & 7) ^ (srow & 7) : (lane & 3) ^ ((srow >> 1) & 3);
+    const unsigned voff = (unsigned)srow * row_bytes + (unsigned)schunk * 16;
+    unsigned wv[IN], xv[IM];
 #pragma unroll
-    for (int q = 0; q < WN; ++q) wv[q] = voff + (unsigned)(q * 64) * row_bytes;
+    for (int q = 0; q < IN; ++q) wv[q] = voff + (unsigned)(q * RI * NW) * row_bytes;
 #pragma unroll
-    for (int q = 0; q < WM; ++q) xv[q] = voff + (unsigned)(q * 64) * row_bytes;
-    auto stage = [&](int s, int slot) {
+    for (int q = 0; q < IM; ++q) xv[q] = voff + (unsigned)(q * RI * NW) * row_bytes;
+    // Instruction d of a stage's NI.  A stage behind the last, and the second half of a last one that ends with an odd step, write zeros: so
+    // every stage issues the same number, and the products need no branch.
+    auto stage_one = [&](int d, int t, int slot) {
         const unsigned dst = lds0 + slot * STAGE + wave * 1024;
+        const unsigned behind = t * KS + (KS == 2 && schunk >= 4 ? 1 : 0) >= steps ? 0xffff0000u : 0u;
+        if (d < IN) dma16(w_rsrc, wv[d < IN ? d : 0] | behind, (unsigned)t * ROW, dst + d * NW * 1024);
+        else dma16(x_rsrc, xv[d < IN ? 0 : d - IN] | behind, (unsigned)t * ROW, dst + TN * ROW + (d - IN) * NW * 1024);
+    };
+    auto stage = [&](int t, int slot) {
 #pragma unroll
-        for (int q = 0; q < WN; ++q) dma16(w_rsrc, wv[q], (unsigned)s * 64, dst + q * 4096);
-#pragma unroll
-        for (int q = 0; q < WM; ++q) dma16(x_rsrc, xv[q], (unsigned)s * 64, dst + TN * 64 + q * 4096);
+        for (int d = 0; d < NI; ++d) stage_one(d, t, slot);
     };
 
-    // scales: four bytes a step and row.  A group of a last row may end behind the matrix: such a read moves back by `over`
-    const unsigned srb = (unsigned)steps * 4;
+    // scales: four bytes a step and row.  What would end behind the matrix (a last row's last group) moves back by `over` bytes
+    const int srb = steps * 4;
     const int64_t sw_all = (int64_t)(p.N - n0) * srb - 16, sx_all = (p.M - m0) * (int64_t)srb - 16;
     const int sw_max = (int)(sw_all < 0x7ffffff0ll ? sw_all : 0x7ffffff0ll), sx_max = (int)(sx_all < 0x7ffffff0ll ? sx_all : 0x7ffffff0ll);
-    // (the descriptors begin at the matrix, so that moving back from a tile's first row stays inside)
+    // (the descriptors begin up to 16 bytes in front of the tile's first row, so that moving back stays inside)
     const int64_t sw_base = (int64_t)n0 * srb, sx_base = m0 * (int64_t)srb;
     const int64_t sw_lo = sw_base < 16 ? sw_base : 16, sx_lo = sx_base < 16 ? sx_base : 16;
     const i32x4 sw_rsrc = raw_rsrc((const char *)p.ws + sw_base - sw_lo, sw_all + 16 + sw_lo);
@@ -390,112 +394,158 @@ __global__ __launch_bounds__(256, OCC) void tile_kernel(onedc_mxfp4_params p, in
     auto stage_scales = [&](int g) {
 #pragma unroll
         for (int q = 0; q < NSC; ++q) {
-            const int first = min(q * 256 + wave * 64, TN + TM - 64);           // (a wave without rows of its own repeats the last ones)
+            const int first = min((q * NW + wave) * 32, TN + TM - 32);          // (a wave without rows of its own repeats the last ones)
             const bool w = first < TN;                                          // wave-uniform
-            const int row = (w ? first : first - TN) + lane;
-            const int off = min(row * (int)srb + g * 16, w ? sw_max : sx_max) + (int)(w ? sw_lo : sx_lo);
-            dma16(w ? sw_rsrc : sx_rsrc, (unsigned)off, 0, lds0 + RING + (g & 1) * GROUP + first * 16);
+            const int row = (w ? first : first - TN) + (lane >> 1);
+            const int off = min(row * srb + g * 32 + (lane & 1) * 16, w ? sw_max : sx_max) + (int)(w ? sw_lo : sx_lo);
+            dma16(w ? sw_rsrc : sx_rsrc, (unsigned)off, 0, lds0 + RING + first * 32);
         }
     };
-    uint32_t sc[FN + FM];
-    const uint32_t pick = (uint32_t)kb * 0x0101u + 0x0400u;
+    // sc[i][h][q], byte J: the scale of this lane's values 64 h + 32 kb .. + 31 of step 4 q + J of the group
+    uint32_t sc[FN + FM][2][2];
+    const uint32_t pick0 = (uint32_t)kb * 0x0101u + 0x0400u, pick1 = pick0 + 0x0202u;
     auto take_scales = [&](int g) {
-        const char *at = smem + RING + (g & 1) * GROUP;
+        const int left = steps - 8 * g;                                          // steps behind the last: scale 2^-127, never a NaN
+        const uint32_t real[2] = {left >= 4 ? ~0u : (1u << 8 * left) - 1, left >= 8 ? ~0u : left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1};
 #pragma unroll
-        for (int i = 0; i < FN + FM; ++i) {
-            const int row = i < FN ? wn * 16 * FN + i * 16 + r : wm * 16 * FM + (i - FN) * 16 + r;
-            const uint4 raw = *(const uint4 *)(at + ((i < FN ? 0 : TN) + row) * 16);
-            const uint32_t lo = __builtin_amdgcn_perm(raw.y, raw.x, pick), hi = __builtin_amdgcn_perm(raw.w, raw.z, pick);
-            const int over = max(row * (int)srb + g * 16 - (i < FN ? sw_max : sx_max), 0);
-            sc[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u) >> ((over * 2) & 31);
-        }
+        for (int i = 0; i < FN + FM; ++i)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int row = (i < FN ? wn * FN + i : wm * FM + i - FN) * 32 + r;
+                const uint4 raw = *(const uint4 *)(smem + RING + (row + (i < FN ? 0 : TN)) * 32 + q * 16);
+                const int over = (max(row * srb + g * 32 + q * 16 - (i < FN ? sw_max : sx_max), 0) * 2) & 31;
+                sc[i][0][q] = (__builtin_amdgcn_perm(__builtin_amdgcn_perm(raw.w, raw.z, pick0), __builtin_amdgcn_perm(raw.y, raw.x, pick0), 0x05040100u) >> over) & real[q];
+                sc[i][1][q] = (__builtin_amdgcn_perm(__builtin_amdgcn_perm(raw.w, raw.z, pick1), __builtin_amdgcn_perm(raw.y, raw.x, pick1), 0x05040100u) >> over) & real[q];
+            }
     };
 
-    f32x4 acc[FN][FM];
+    f32x16 acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int frag = r * 64 + ((kb ^ ((r >> 1) & 3)) << 4);
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    const int swap = KS == 2 ? r & 7 : (r >> 1) & 3;
 
-    const int groups = (steps + 3) >> 2;
+    const int stages = (steps + KS - 1) / KS, groups = (steps + 7) >> 3;
     stage_scales(0);
+    constexpr int AHEAD = NST > 1 ? NST - 1 : 1;     // stages in flight
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-        if (i < steps) stage(i, i);
+    for (int i = 0; i < AHEAD; ++i) stage(i, i);
     int slot = 0, fill = NST - 1;
-    auto step = [&](auto jc, int s, bool more) {
-        constexpr int J = decltype(jc)::value;
-        // this step's codes (and a new group's scales) have landed: what was issued behind them are the next NST - 2 steps' and, up to the
-        // step that was issued together with them, the next group's scales
-        if (s + NST - 2 < steps) {
-            if (J > 0 && J < NST && more) MX_VMCNT((NST - 2) * NI + NSC);
-            else MX_VMCNT((NST - 2) * NI);
-        } else {
-            MX_VMCNT(0);
-        }
+    // I: stage of the group
+    auto go = [&](auto ic, int t) {
+        constexpr int I = decltype(ic)::value;
+        // This stage's codes (and a new group's scales) have landed: what was issued behind them are the next stages and, up to the stage that
+        // was issued together with them, the next group's scales (issued at the end of a group's second stage).
+        MX_VMCNT((AHEAD - 1) * NI + (I >= 2 && I <= AHEAD + 1 && NST > 1 ? NSC : 0));
         __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        if (s + NST - 1 < steps) stage(s + NST - 1, fill);       // into the slot that every wave left behind at this barrier
-        if (J == 0) {
-            if (more) stage_scales((s >> 2) + 1);
-            take_scales(s >> 2);
+        if (I == 0) take_scales(t * KS >> 3);
+        const char *a = smem + slot * STAGE + (wn * FN * 32 + r) * ROW, *b = smem + slot * STAGE + (TN + wm * FM * 32 + r) * ROW;
+        // The DMA into the slot that every wave left behind at this barrier is spread over the products: issued in one go it would hold
+        // the wave until the address unit has taken it all.
+        constexpr int MUL = 2 * KS * FN * FM, EVERY = MUL / (NI + 1) > 0 ? MUL / (NI + 1) : 1;
+        int done = 0, sent = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 fa[FN], fb[FM];
+                const int at = ((4 * k + 2 * h + kb) ^ swap) << 4;
+#pragma unroll
+                for (int j = 0; j < FM; ++j) fb[j] = *(const uint4 *)(b + j * 32 * ROW + at);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) fa[i] = *(const uint4 *)(a + i * 32 * ROW + at);
+                constexpr int J0 = I * KS;
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) {
+                        if (k == 0) acc[i][j] = mfma_fp4_32<J0 & 3>(fa[i], fb[j], acc[i][j], sc[i][h][J0 >> 2], sc[FN + j][h][J0 >> 2]);
+                        else acc[i][j] = mfma_fp4_32<(J0 + 1) & 3>(fa[i], fb[j], acc[i][j], sc[i][h][((J0 + 1) & 7) >> 2], sc[FN + j][h][((J0 + 1) & 7) >> 2]);
+                        if (NST > 1 && ++done % EVERY == 0 && sent < NI) stage_one(sent++, t + AHEAD, fill);
+                    }
+            }
+        if (NST == 1) {                              // one slot: everybody has read it, then it is filled again
+            __syncthreads();
+            stage(t + 1, 0);
+        } else {
+#pragma unroll
+            for (int d = 0; d < NI; ++d)
+                if (d >= sent) stage_one(d, t + AHEAD, fill);
+            fill = slot;
+            slot = slot + 1 == NST ? 0 : slot + 1;
         }
-        const char *a = smem + slot * STAGE + wn * FN * 1024 + frag, *b = smem + slot * STAGE + TN * 64 + wm * FM * 1024 + frag;
-        uint4 fa[FN], fb[FM];
-#pragma unroll
-        for (int j = 0; j < FM; ++j) fb[j] = *(const uint4 *)(b + j * 1024);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) fa[i] = *(const uint4 *)(a + i * 1024);
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j) acc[i][j] = mfma_fp4<J>(fa[i], fb[j], acc[i][j], sc[i], sc[FN + j]);
-        fill = slot;
-        slot = slot + 1 == NST ? 0 : slot + 1;
+        if (I == 1) stage_scales((t * KS >> 3) + 1);             // (every wave has taken this group's: a barrier ago)
     };
     for (int g = 0; g < groups; ++g) {
-        const bool more = g + 1 < groups;
-        const int s = g * 4;
-        step(std::integral_constant<int, 0>(), s, more);
-        if (s + 1 < steps) step(std::integral_constant<int, 1>(), s + 1, more);
-        if (s + 2 < steps) step(std::integral_constant<int, 2>(), s + 2, more);
-        if (s + 3 < steps) step(std::integral_constant<int, 3>(), s + 3, more);
+        const int t = g * GS;
+        go(std::integral_constant<int, 0>(), t);
+        if (t + 1 < stages) go(std::integral_constant<int, 1>(), t + 1);
+        if (t + 2 < stages) go(std::integral_constant<int, 2>(), t + 2);
+        if (t + 3 < stages) go(std::integral_constant<int, 3>(), t + 3);
+        if constexpr (GS == 8) {
+            if (t + 4 < stages) go(std::integral_constant<int, 4>(), t + 4);
+            if (t + 5 < stages) go(std::integral_constant<int, 5>(), t + 5);
+            if (t + 6 < stages) go(std::integral_constant<int, 6>(), t + 6);
+            if (t + 7 < stages) go(std::integral_constant<int, 7>(), t + 7);
+        }
     }
+    MX_VMCNT(0);
     __syncthreads();                                 // the ring is free: the waves' own scratch from here
 
-    // epilogue: 16 activation rows at a time through LDS, so that a row's outputs leave as whole lines
-    constexpr int PITCH = FN * 16 + 4;
-    float *my = (float *)smem + wave * 16 * PITCH;
-    const bool glu = p.epi == ONEDC_EPI_GEGLU;
-    const int out = glu ? p.N / 2 : p.N, nw = n0 + wn * FN * 16, no = glu ? nw / 2 : nw;
-    f32x4 bias[FN];
+    // epilogue: 32 activation rows at a time through LDS, so that a row's outputs leave as whole lines.  Of a block a lane holds activation
+    // row r and weight rows 8 q + 4 kb + e (q = 0 .. 3, e = 0 .. 3); a gated layer's block is 16 values and their 16 gates
+    constexpr int PITCH = FN * 32 + 4;
+    float *const my = (float *)smem + wave * 32 * PITCH;
+    const int nw = n0 + wn * FN * 32;
+    float bias[FN][16];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bias[i][e] = bias_of(p, nw + i * 16 + kb * 4 + e);
+        for (int q = 0; q < 4; ++q) {
+            const int n = nw + i * 32 + q * 8 + kb * 4;
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-        const int64_t mt = m0 + (wm * FM + j) * 16;
+            for (int e = 0; e < 4; ++e) bias[i][q * 4 + e] = p.bias ? p.bias[min(n + e, p.N - 1)] : 0.f;
+        }
+    auto finish = [&](auto ec) {
+        constexpr int EPI = decltype(ec)::value;
+        constexpr bool GLU = EPI == ONEDC_EPI_GEGLU;
+        constexpr int WIDE = GLU ? FN * 16 : FN * 32, PIECES = WIDE / 8;         // outputs of a row, in pieces of eight
+        const int out = GLU ? p.N / 2 : p.N, no = GLU ? nw / 2 : nw;
 #pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            if (glu && (i & 1)) continue;
-            f32x4 v;
+        for (int j = 0; j < FM; ++j) {
+            const int64_t mt = m0 + (wm * FM + j) * 32;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float t = p.alpha * acc[i][j][e] + bias[i][e];
-                if (glu) v[e] = t * gelu_f(p.alpha * acc[i | 1][j][e] + bias[i | 1][e]);
-                else v[e] = activation(p, t);
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int q = 0; q < (GLU ? 2 : 4); ++q) {
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float t = __builtin_fmaf(p.alpha, acc[i][j][q * 4 + e], bias[i][q * 4 + e]);
+                        if (GLU) v[e] = t * gelu_f(__builtin_fmaf(p.alpha, acc[i][j][(q * 4 + e + 8) & 15], bias[i][(q * 4 + e + 8) & 15]));
+                        else v[e] = EPI == ONEDC_EPI_SILU ? silu_f(t) : EPI == ONEDC_EPI_LEAKY ? leaky(t, p.slope) : t;
+                    }
+                    *(f32x4 *)(my + r * PITCH + i * (GLU ? 16 : 32) + q * 8 + kb * 4) = v;
+                }
+#pragma unroll
+            for (int t0 = 0; t0 < 32 * PIECES; t0 += 64) {
+                const int t = t0 + lane, row = t / PIECES, c = (t - row * PIECES) * 8, n = no + c;
+                const f32x4 lo = *(const f32x4 *)(my + row * PITCH + c), hi = *(const f32x4 *)(my + row * PITCH + c + 4);
+                const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                if (mt + row < p.M && n < out) store8(p, mt + row, n, out, v, whole && n + 8 <= out);
             }
-            *(f32x4 *)(my + r * PITCH + (glu ? i / 2 : i) * 16 + kb * 4) = v;
         }
-        const int pieces = glu ? FN : 2 * FN;                             // eight outputs each, per row
-        for (int t = lane; t < 16 * pieces; t += 64) {
-            const int row = t / pieces, n = no + (t - row * pieces) * 8;
-            const f32x4 lo = *(const f32x4 *)(my + row * PITCH + n - no), hi = *(const f32x4 *)(my + row * PITCH + n - no + 4);
-            const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (mt + row < p.M && n < out) store8(p, mt + row, n, out, v, whole && n + 8 <= out);
-        }
+    };
+    switch (p.epi) {
+    case ONEDC_EPI_GEGLU: finish(std::integral_constant<int, ONEDC_EPI_GEGLU>()); break;
+    case ONEDC_EPI_SILU: finish(std::integral_constant<int, ONEDC_EPI_SILU>()); break;
+    case ONEDC_EPI_LEAKY: finish(std::integral_constant<int, ONEDC_EPI_LEAKY>()); break;
+    default: finish(std::integral_constant<int, ONEDC_EPI_LINEAR>());
     }
 }
 
@@ -519,21 +569,24 @@ int launch_dequantize(const void *codes, const void *scales, void *y, int y_cs, 
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
-template <int FM, bool RAW, bool VEC>
+template <int RAW, bool VEC>
 int launch_skinny(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
-    const int64_t wgs = (int64_t)((p->N + 31) / 32) * ((p->M + 16 * FM - 1) / (16 * FM));
-    hipLaunchKernelGGL((skinny_kernel<FM, RAW, VEC>), dim3((unsigned)wgs), dim3(64 * SKW), 0, as_stream(stream), *p, steps, whole);
+    const int64_t wgs = (int64_t)((p->N + 31) / 32) * ((p->M + 15) / 16);
+    hipLaunchKernelGGL((skinny_kernel<RAW, VEC>), dim3((unsigned)wgs), dim3(64 * SKW), 0, as_stream(stream), *p, steps, whole);
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
-template <int FN, int FM, int NST, int OCC>
+template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC>
 int launch_tiles(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
-    constexpr int ring = 32 * (FN + FM) * (NST * 64 + 2 * 16), scratch = 4 * 16 * (FN * 16 + 4) * 4, lds = ring > scratch ? ring : scratch;
+    static_assert(FN == 1 || FN == 2 || FN == 4, "");
+    constexpr int TN = 32 * WN * FN, TM = 32 * WM * FM;
+    constexpr int ring = (TN + TM) * (NST * KS * 64 + 32), scratch = WN * WM * 32 * (FN * 32 + 4) * 4, lds = ring > scratch ? ring : scratch;
     static OnedcLdsAttrOnce once;
-    once.ensure({{(const void *)tile_kernel<FN, FM, NST, OCC>, lds}});
-    const int64_t tn = (p->N + 32 * FN - 1) / (32 * FN), tm = (p->M + 32 * FM - 1) / (32 * FM);
+    once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, KS, NST, OCC>, lds}});
+    const int64_t tn = (p->N + TN - 1) / TN, tm = (p->M + TM - 1) / TM;
     if (tn * tm > 0x7fffffff) return -2;
-    hipLaunchKernelGGL((tile_kernel<FN, FM, NST, OCC>), dim3((unsigned)(tn * tm)), dim3(256), lds, as_stream(stream), *p, steps, (int)tn, (int)tm, whole);
+    hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, KS, NST, OCC>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM), lds, as_stream(stream), *p, steps,
+                       (int)tn, (int)tm, whole);
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
@@ -579,15 +632,25 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     const int whole = whole_ok(p->y, p->y_cs, p->y_co, p->y_f32) && (!p->res || whole_ok(p->res, p->r_cs, p->r_co, p->y_f32));
     if (((int64_t)(p->N + 31) / 32) * ((p->M + 15) / 16) > 0x7fffffff) return -2;
     if (!p->xc) {
-        if (p->K % 8 == 0 && whole_ok(p->xr, p->xr_cs, p->xr_co, p->xr_f32)) return launch_skinny<1, true, true>(p, steps, whole, stream);
-        return launch_skinny<1, true, false>(p, steps, whole, stream);
+        const bool vec = p->K % 8 == 0 && whole_ok(p->xr, p->xr_cs, p->xr_co, p->xr_f32);
+        if (p->xr_f32) return vec ? launch_skinny<2, true>(p, steps, whole, stream) : launch_skinny<2, false>(p, steps, whole, stream);
+        return vec ? launch_skinny<1, true>(p, steps, whole, stream) : launch_skinny<1, false>(p, steps, whole, stream);
     }
-    if (p->M <= 16) return launch_skinny<1, false, true>(p, steps, whole, stream);
-    if (p->M <= 32 || (int64_t)p->N * steps < 4) return launch_skinny<2, false, true>(p, steps, whole, stream);
-    const int64_t big = (int64_t)((p->N + 127) / 128) * ((p->M + 127) / 128);
-    if (big <= 64) return launch_skinny<4, false, true>(p, steps, whole, stream);
-    if (big <= 512) return launch_tiles<4, 4, 3, 2>(p, steps, whole, stream);
-    return launch_tiles<4, 8, 3, 2>(p, steps, whole, stream);
+    // (the tiles' scale reads need 16 bytes in all)
+    if (p->M <= ONEDC_MXFP4_ROWS_RAW || (int64_t)p->N * steps < 4) return launch_skinny<0, true>(p, steps, whole, stream);
+    // Tiles, by how many of them there are for 256 CUs (measured on grids of M 64 .. 36864, N 320 .. 10240, K 320 .. 8192):
+    //   256 x 256, eight waves, two stages: the fewest bytes into LDS a product.  From 160 tiles on, where it pads no tenth more than 128 x 128;
+    //     gated layers only from 32 steps on (8192 x 4096 x 5120: 95 us against 110; gated 8655 x 10240 x 1280: 117 against 100, there
+    //     the epilogue counts, and nothing else runs on the CU meanwhile)
+    //   64 x 64, three stages, while they fit the CUs' first four each (2048 x 1280 x 5120: 17 us against 19; 4096 x 1280 x 5120: 28 against 26)
+    //   128 x 128: one stage and three workgroups a CU that load and multiply in turn; two stages where there are less than two a CU
+    //     (4096 x 1280 x 5120: 26 us against 28; 8192 x 4096 x 5120: 112 against 110)
+    const auto tiles = [&](int64_t t) { return ((p->N + t - 1) / t) * ((p->M + t - 1) / t); };
+    const bool gated = p->epi == ONEDC_EPI_GEGLU;
+    if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 2>(p, steps, whole, stream);
+    if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 2, 3, 4>(p, steps, whole, stream);
+    if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 2>(p, steps, whole, stream);
+    return launch_tiles<2, 2, 2, 2, 2, 1, 3>(p, steps, whole, stream);
 }
 
 }  // extern "C"
