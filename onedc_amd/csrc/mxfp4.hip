@@ -234,61 +234,95 @@ __device__ __forceinline__ void store8(const onedc_mxfp4_params &p, int64_t m, i
 }
 
 // ---- few rows: the weights' bytes bound it -------------------------------------------------------------------------------------------
-// A workgroup computes 32 weight rows x 16 activation rows; its sixteen waves take every sixteenth 128-value step of K straight from
-// memory (each weight byte is read once, 64 bytes of 16 rows an instruction; four steps' loads in flight a wave) and their sums are added
-// through LDS in wave order.  Raw rows are quantised by the lane that multiplies them, once a workgroup: 70 instructions a step against
-// 2 KB of weights.
-constexpr int SKW = 16;
-// the 32 values of a lane's block as codes and scale
-template <bool F32, bool VEC>
-struct Block32 {
-    Eight<F32, VEC> v[4];
-    __device__ __forceinline__ void load(const void *x, int64_t at, int left) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j].load(x, at + j * 8, left - j * 8);
+// A workgroup computes 32 weight rows x 16 activation rows over rounds of 64 steps of 128 values: each of its sixteen waves takes four
+// consecutive steps of a round straight from memory, 256 bytes of every weight row and 16 bytes of its scales, all in flight at once (steps dealt
+// out in turn instead would send all waves to the same memory channels where a row is a power of two long: 8192 x 8192 against one row 11.3 us
+// that way).  The waves' sums are added through LDS in wave order.  Raw rows are quantised by the workgroup together, under the weights' loads, into LDS.
+constexpr int SKW = 16, SKU = 4, ROUND = SKW * SKU;                       // steps of a round
+constexpr int XPITCH = ROUND * 64 + 16, SPITCH = ROUND * 4 + 16;          // bytes of a row's codes and scales in LDS, off the banks' period
+
+// the scales of four steps of a row, a byte each for this lane's block (kb): from s on, the row ends at `steps`
+__device__ __forceinline__ uint32_t four_scales(const uint8_t *all, int64_t row, int64_t rows, int s, int steps, int kb) {
+    const uint32_t pick = (uint32_t)kb * 0x0101u + 0x0400u;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    int over = 0;
+    if (steps >= 4) {                                // 16 bytes; moved back where they would end behind the matrix
+        const int64_t at = (row * steps + s) * 4, last = rows * steps * 4 - 16;
+        over = at > last ? (int)(at - last) : 0;
+        __builtin_memcpy(&v, all + at - over, 16);
+    } else {
+        const uint32_t *w = (const uint32_t *)all + row * steps + s;
+        v.x = w[0];
+        if (s + 1 < steps) v.y = w[1];
+        if (s + 2 < steps) v.z = w[2];
     }
-    __device__ __forceinline__ uint4 codes(uint32_t &s) const {
-        s = block_scale(max(max(v[0].amax_bits(), v[1].amax_bits()), max(v[2].amax_bits(), v[3].amax_bits())));
-        return make_uint4(v[0].codes(s), v[1].codes(s), v[2].codes(s), v[3].codes(s));
-    }
-};
+    const uint32_t lo = __builtin_amdgcn_perm(v.y, v.x, pick), hi = __builtin_amdgcn_perm(v.w, v.z, pick);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u) >> ((over * 2) & 31);
+}
+
 // RAW 0: codes, 1: 16-bit rows, 2: f32 rows
 template <int RAW, bool VEC>
 __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, int steps, int whole) {
-    __shared__ __attribute__((aligned(16))) float red[SKW][2][16][20];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kb = lane >> 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];              // raw rows' codes, then their scales; the sums over them
+    typedef float Red[2][16][20];
+    Red *const red = (Red *)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, kb = lane >> 4;
     const int nt = (p.N + 31) / 32;
     const int n0 = (int)(blockIdx.x % nt) * 32;
     const int64_t m0 = (int64_t)(blockIdx.x / nt) * 16, m = m0 + r < p.M ? m0 + r : p.M - 1;
+    const int rows = (int)(p.M - m0 < 16 ? p.M - m0 : 16);
     const int na = min(n0 + r, p.N - 1), nc = min(n0 + 16 + r, p.N - 1);
     const uint4 *wa = (const uint4 *)p.wc + (int64_t)na * steps * 4 + kb, *wb = (const uint4 *)p.wc + (int64_t)nc * steps * 4 + kb;
-    const uint8_t *sa = (const uint8_t *)p.ws + (int64_t)na * steps * 4 + kb, *sb = (const uint8_t *)p.ws + (int64_t)nc * steps * 4 + kb;
+    char *const xscale = smem + 16 * XPITCH;
     f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    constexpr int U = RAW == 2 ? 2 : 4;              // steps whose loads are in flight together (behind the last: the last again, as zeros)
-    for (int s0 = wave; s0 < steps; s0 += SKW * U) {
-        uint4 a[U], c[U], x[U];
-        uint32_t xa[U], xc[U], sx[U];
-        Block32<RAW == 2, VEC> raw[U];
+    for (int first = 0; first < steps; first += ROUND) {
+        const int s = first + wave * SKU;
+        uint4 a[SKU], c[SKU], x[SKU];
+        uint32_t xa = 0, xc = 0, sx = 0;
+        if (s < steps) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int s = min(s0 + u * SKW, steps - 1), k0 = s * 128 + kb * 32;
-            a[u] = wa[s * 4], c[u] = wb[s * 4];
-            xa[u] = sa[s * 4], xc[u] = sb[s * 4];
-            if (RAW) {
-                raw[u].load(p.xr, m * p.xr_cs + p.xr_co + k0, s0 + u * SKW < steps ? p.K - k0 : 0);
-            } else {
-                x[u] = ((const uint4 *)p.xc)[(m * steps + s) * 4 + kb];
-                sx[u] = ((const uint8_t *)p.xs)[(m * steps + s) * 4 + kb];
+            for (int u = 0; u < SKU; ++u) {
+                const int su = min(s + u, steps - 1);
+                a[u] = wa[su * 4], c[u] = wb[su * 4];
+                if (!RAW) x[u] = ((const uint4 *)p.xc)[(m * steps + su) * 4 + kb];
+            }
+            xa = four_scales((const uint8_t *)p.ws, na, p.N, s, steps, kb);
+            xc = four_scales((const uint8_t *)p.ws, nc, p.N, s, steps, kb);
+            if (!RAW) sx = four_scales((const uint8_t *)p.xs, m, p.M, s, steps, kb);
+        }
+        if (RAW) {
+            // a row a pass: 1024 threads, eight values each, four neighbours a block
+            const int k = first * 128 + threadIdx.x * 8;
+            if (first) __syncthreads();              // (the last round's codes have been multiplied)
+            for (int i = 0; i < rows; i += 4) {
+                Eight<RAW == 2, VEC> v[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q].load(p.xr, (m0 + i + q) * p.xr_cs + p.xr_co + k, i + q < rows ? p.K - k : 0);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t sc = block_scale(quad_max<0x4e>(quad_max<0xb1>(v[q].amax_bits())));
+                    if (i + q >= rows) continue;     // (uniform)
+                    *(uint32_t *)(smem + (i + q) * XPITCH + threadIdx.x * 4) = v[q].codes(sc);
+                    if ((threadIdx.x & 3) == 0) xscale[(i + q) * SPITCH + (threadIdx.x >> 2)] = (char)sc;
+                }
+            }
+            __syncthreads();
+            if (s < steps) {
+                const int row = min(r, rows - 1);
+#pragma unroll
+                for (int u = 0; u < SKU; ++u) x[u] = *(const uint4 *)(smem + row * XPITCH + (wave * SKU + u) * 64 + kb * 16);
+                const uint4 v = *(const uint4 *)(xscale + row * SPITCH + wave * SKU * 4);
+                const uint32_t pick = (uint32_t)kb * 0x0101u + 0x0400u;
+                sx = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v.w, v.z, pick), __builtin_amdgcn_perm(v.y, v.x, pick), 0x05040100u);
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s0 + u * SKW >= steps) break;
-            if (RAW) x[u] = raw[u].codes(sx[u]);
-            acc[0] = mfma_fp4<0>(a[u], x[u], acc[0], xa[u], sx[u]);
-            acc[1] = mfma_fp4<0>(c[u], x[u], acc[1], xc[u], sx[u]);
-        }
+        if (s >= steps) continue;                    // (wave-uniform, like the next)
+        acc[0] = mfma_fp4<0>(a[0], x[0], acc[0], xa, sx), acc[1] = mfma_fp4<0>(c[0], x[0], acc[1], xc, sx);
+        if (s + 1 < steps) acc[0] = mfma_fp4<1>(a[1], x[1], acc[0], xa, sx), acc[1] = mfma_fp4<1>(c[1], x[1], acc[1], xc, sx);
+        if (s + 2 < steps) acc[0] = mfma_fp4<2>(a[2], x[2], acc[0], xa, sx), acc[1] = mfma_fp4<2>(c[2], x[2], acc[1], xc, sx);
+        if (s + 3 < steps) acc[0] = mfma_fp4<3>(a[3], x[3], acc[0], xa, sx), acc[1] = mfma_fp4<3>(c[3], x[3], acc[1], xc, sx);
     }
+    if (RAW) __syncthreads();
     // lane: activation row r, weight rows 4 kb + e of each half
     *(f32x4 *)&red[wave][0][r][kb * 4] = acc[0];
     *(f32x4 *)&red[wave][1][r][kb * 4] = acc[1];
@@ -304,7 +338,7 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, 
         total = p.alpha * total + bias_of(p, n0 + tn);
     }
     __syncthreads();
-    float (*const row32)[36] = (float (*)[36])&red[0][0][0][0];
+    float (*const row32)[36] = (float (*)[36])smem;
     if (threadIdx.x < 512) row32[tr][tn] = total;
     __syncthreads();
     const int t = threadIdx.x, row = t / pieces, c = (t - row * pieces) * 8, n = (glu ? n0 / 2 : n0) + c;
@@ -572,7 +606,10 @@ int launch_dequantize(const void *codes, const void *scales, void *y, int y_cs, 
 template <int RAW, bool VEC>
 int launch_skinny(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
     const int64_t wgs = (int64_t)((p->N + 31) / 32) * ((p->M + 15) / 16);
-    hipLaunchKernelGGL((skinny_kernel<RAW, VEC>), dim3((unsigned)wgs), dim3(64 * SKW), 0, as_stream(stream), *p, steps, whole);
+    constexpr int sums = SKW * 2 * 16 * 20 * 4, raw = RAW ? 16 * (XPITCH + SPITCH) : 0, lds = sums > raw ? sums : raw;
+    static OnedcLdsAttrOnce once;
+    once.ensure({{(const void *)skinny_kernel<RAW, VEC>, lds}});
+    hipLaunchKernelGGL((skinny_kernel<RAW, VEC>), dim3((unsigned)wgs), dim3(64 * SKW), lds, as_stream(stream), *p, steps, whole);
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
