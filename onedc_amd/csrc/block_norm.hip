@@ -867,6 +867,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
             return -3;
     }
     const bool sums = wants_sums(g);
+    if (sums && (int64_t)p->B * ((p->C + 63) / 64) > 0x7fffffff) return -2;
     const int64_t need = onedc_block_norm_backward_ws_bytes(p, g);
     if (need && (!g->ws || g->ws_bytes < need)) return -15;
     if (!any) {
