@@ -365,9 +365,10 @@ __device__ __forceinline__ i32x4 raw_rsrc(const void *base, int64_t bytes) {
     return i32x4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)(bytes < 0x7ffffff0ll ? bytes : 0x7ffffff0ll), 0x00020000};
 }
 // 16 bytes a lane from base + voff + soff to lds + 16 lane; a lane whose voff lies behind the descriptor's end writes zeros
-// (m0 is reserved: nothing else in these kernels reads it.  No memory clobber: LDS reads may pass it, the waits and barriers order what has to be)
+// (m0 is reserved: nothing else in these kernels reads it.  Five wait states: one for m0, five for a scalar operand that a vector instruction may
+// have written just before.  No memory clobber: LDS reads may pass it, the waits and barriers order what has to be.)
 __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned voff, unsigned soff, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
 // WN x WM waves of FN x FM blocks of 32 x 32

@@ -675,6 +675,8 @@ LIN = [
     (513, 264, 2080, "leaky", True, False),
     (1031, 1280, 384, "linear", True, False),
     (2500, 96, 5120, "silu", False, True),
+    (50, 3, 100, "linear", True, False),
+    (40, 1, 300, "linear", False, True),
 ]
 EPI = {"linear": K.EPI_LINEAR, "leaky": K.EPI_LEAKY, "silu": K.EPI_SILU, "geglu": K.EPI_GEGLU}
 
@@ -707,6 +709,38 @@ def test_mxfp4_linear(M, N, k, epi, bias, res, fmt):
         yr = rows_view(r, cs, co)
         K.mxfp4_linear(rows_view(x), wq, b.to(DEV) if bias else None, yr, epi=EPI[epi], alpha=0.5, slope=0.1, res=yr)
         assert torch.equal(back(yr), back(y)) and untouched(yr)
+
+
+@pytest.mark.parametrize("M,N,k,epi,res", [
+    (2100, 2100, 520, "linear", True),         # 128 x 128, two stages; an odd number of steps
+    (4200, 2624, 260, "geglu", False),         # 128 x 128, one stage
+    (2600, 4200, 200, "silu", True),           # 256 x 256; two steps, ragged both ways
+    (2600, 4224, 4500, "geglu", True),         # 256 x 256, gated; 36 steps
+    (2601, 4195, 1150, "leaky", False),        # 256 x 256, nothing aligned; nine steps: a group of scales with one step
+])
+def test_mxfp4_linear_large_tiles(M, N, k, epi, res, fmt):
+    """The tiles of large layers, against the product of the values that the operands stand for (read back: their own tests) in 64 bits on the
+    GPU, a row and a column that are no numbers among them."""
+    g = torch.Generator(device=DEV).manual_seed(M + k)
+
+    def rnd(*shape, scale=1.0):
+        return torch.randn(*shape, generator=g, device=DEV) * scale
+    x, w, b = rnd(M, k).to(fmt), rnd(N, k, scale=k ** -0.5), rnd(N)
+    x[M - 1, k - 1], w[N - 33, 0] = float("nan"), float("inf")
+    out = N // 2 if epi == "geglu" else N
+    r = rnd(M, out).to(fmt) if res else None
+    xq, wq = K.mxfp4_quantize(View(x, 1, 1, M, k)), pack.pack_mxfp4(w, DEV)
+    xv, wv = torch.empty(M, k, device=DEV), torch.empty(N, k, device=DEV)
+    K.mxfp4_dequantize(xq, View(xv, 1, 1, M, k))
+    K.mxfp4_dequantize(wq, View(wv, 1, 1, N, k))
+    ref, err = linear64(xv.double(), wv.double(), b, EPI[epi], 1.0, 0.1, r)
+    y = torch.full((M + 1, out), 7.0, dtype=fmt, device=DEV)
+    K.mxfp4_linear(xq, wq, b, View(y, 1, 1, M, out), epi=EPI[epi], slope=0.1, res=None if r is None else View(r, 1, 1, M, out))
+    assert bool((y[M] == 7.0).all())
+    got = y[:M].double()
+    assert torch.equal(got.isnan(), ref.isnan()) and bool(ref[M - 1].isnan().all()) and not bool(ref[:M - 1, :(N - 40) // 2].isnan().any())
+    bad = ~(((got - ref).abs() <= half_step(fmt) * ref.abs() + tiny(fmt) + err) | ref.isnan())
+    assert not bool(bad.any()), (int(bad.sum()), float((got - ref).abs()[bad].max()))
 
 
 def test_mxfp4_linear_from_f32_rows(fmt):
