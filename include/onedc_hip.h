@@ -382,7 +382,7 @@ int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_c
  * from t BEFORE xo's rounding.  Every vector is f32 and may be NULL (factor 1, summand 0); gate / scale / shift hold one row per
  * picture, `*_rs` floats apart (0: one row for all pictures, e.g. a learned per-channel residual scale as the gate).
  * x and xo are 16-bit or (x_f32) f32; f, y are 16-bit or (f_f32, only with x_f32) f32.  Rows are NHWC views: channel stride *_cs,
- * offset *_co, any values; xo may be x itself.  B * N rows may be 0.  Launches only, no workspace.
+ * offset *_co, any values; xo may be x itself.  B * N rows: 0 to 2^30.  Launches only, no workspace.
  * Returns -1 for a missing pointer, -2 for sizes or strides, -3 for a combination of options that has no meaning. */
 enum { ONEDC_NORM_LAYER = 0, ONEDC_NORM_RMS = 1 };
 typedef struct onedc_block_norm_params {

@@ -683,7 +683,8 @@ int check_view(const void *p, int cs, int co, int C) { return !p || (cs >= C && 
 
 int check_common(const onedc_block_norm_params *p) {
     if (!p) return -1;
-    if (p->B < 0 || p->N < 0 || p->C < 1 || p->C > (1 << 20) || (int64_t)p->B * p->N > 0x7fffffff) return -2;
+    // (2^30 rows: a run of them, and the workgroup's turn behind it, are counted in 31 bits)
+    if (p->B < 0 || p->N < 0 || p->C < 1 || p->C > (1 << 20) || (int64_t)p->B * p->N > (1 << 30)) return -2;
     if (!p->B || !p->N) return 0;                    // no rows: nothing is read or written (the pointers of empty tensors are NULL)
     if (!p->x) return -1;
     if (check_view(p->x, p->x_cs, p->x_co, p->C) || check_view(p->f, p->f_cs, p->f_co, p->C)) return -2;

@@ -409,8 +409,9 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_par
     auto stage_one = [&](int d, int t, int slot) {
         const unsigned dst = lds0 + slot * STAGE + wave * 1024;
         const unsigned behind = t * KS + (KS == 2 && schunk >= 4 ? 1 : 0) >= steps ? 0xffff0000u : 0u;
-        if (d < IN) dma16(w_rsrc, wv[d < IN ? d : 0] | behind, (unsigned)t * ROW, dst + d * NW * 1024);
-        else dma16(x_rsrc, xv[d < IN ? 0 : d - IN] | behind, (unsigned)t * ROW, dst + TN * ROW + (d - IN) * NW * 1024);
+        const unsigned soff = t * KS < steps ? (unsigned)t * ROW : 0u;           // (never past the descriptor's end: it is taken off that)
+        if (d < IN) dma16(w_rsrc, wv[d < IN ? d : 0] | behind, soff, dst + d * NW * 1024);
+        else dma16(x_rsrc, xv[d < IN ? 0 : d - IN] | behind, soff, dst + TN * ROW + (d - IN) * NW * 1024);
     };
     auto stage = [&](int t, int slot) {
 #pragma unroll
@@ -635,7 +636,7 @@ extern "C" {
 
 int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream) {
     if (!x || !codes || !scales) return -1;
-    if (rows < 0 || rows > 0x7fffffff || K < 1 || K > ONEDC_MXFP4_MAX_K || x_co < 0 || x_cs - K < x_co || !held_ok(codes, scales) ||
+    if (rows < 0 || rows > 0x7fffffff || K < 1 || K > ONEDC_MXFP4_MAX_K || x_co < 0 || (int64_t)x_cs - K < x_co || !held_ok(codes, scales) ||
         rows * ((K + 127) / 128) > (1ll << 36))
         return -2;
     if (!rows) return 0;
@@ -646,7 +647,7 @@ int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *cod
 
 int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y_f32, int y_cs, int y_co, int64_t rows, int K, void *stream) {
     if (!y || !codes || !scales) return -1;
-    if (rows < 0 || rows > 0x7fffffff || K < 1 || K > ONEDC_MXFP4_MAX_K || y_co < 0 || y_cs - K < y_co || !held_ok(codes, scales) ||
+    if (rows < 0 || rows > 0x7fffffff || K < 1 || K > ONEDC_MXFP4_MAX_K || y_co < 0 || (int64_t)y_cs - K < y_co || !held_ok(codes, scales) ||
         rows * ((K + 127) / 128) > (1ll << 36))
         return -2;
     if (!rows) return 0;
@@ -661,9 +662,9 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     if (p->epi == ONEDC_EPI_GEGLU && p->N % 32) return -3;
     const int out = p->epi == ONEDC_EPI_GEGLU ? p->N / 2 : p->N;
     if (p->M < 0 || p->M > 0x7fffffff || p->N < 1 || p->N > (1 << 24) || p->K < 1 || p->K > ONEDC_MXFP4_MAX_K || p->y_co < 0 ||
-        p->y_cs - out < p->y_co || (p->res && (p->r_co < 0 || p->r_cs - out < p->r_co)) || !held_ok(p->wc, p->ws))
+        (int64_t)p->y_cs - out < p->y_co || (p->res && (p->r_co < 0 || (int64_t)p->r_cs - out < p->r_co)) || !held_ok(p->wc, p->ws))
         return -2;
-    if (p->xc ? !held_ok(p->xc, p->xs) : (p->xr_co < 0 || p->xr_cs - p->K < p->xr_co)) return -2;
+    if (p->xc ? !held_ok(p->xc, p->xs) : (p->xr_co < 0 || (int64_t)p->xr_cs - p->K < p->xr_co)) return -2;
     if (!p->xc && p->M > ONEDC_MXFP4_ROWS_RAW) return -4;
     if (!p->M) return 0;
     const int steps = (p->K + 127) / 128;

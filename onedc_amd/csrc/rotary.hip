@@ -162,7 +162,7 @@ extern "C" int onedc_rotary_axes(const onedc_rotary_params *p, void *stream) {
     if (p->B < 0 || p->N < 0 || p->D < 1 || p->D > 4096 || p->pairs < 0 || 2 * p->pairs > p->D || p->axes < 1 || p->axes > 16 || p->qh < 1 ||
         p->kh < 0 || p->qh > 4096 || p->kh > 4096 || (int64_t)p->B * p->N > 0x7fffffff || p->pos_bs < 0)
         return -2;
-    const int cq = p->qh * p->D, ck = p->kh * p->D;
+    const int64_t cq = p->qh * p->D, ck = p->kh * p->D;
     if (p->q_co < 0 || p->q_cs - cq < p->q_co || p->qo_co < 0 || p->qo_cs - cq < p->qo_co) return -2;
     if (p->kh && (p->k_co < 0 || p->k_cs - ck < p->k_co || p->ko_co < 0 || p->ko_cs - ck < p->ko_co)) return -2;
     if (!p->B || !p->N) return 0;

@@ -839,7 +839,7 @@ def _block_norm_args(what, x, f, has_y, side, kind, post, post_w, post_b, gate, 
         raise KernelError(f"{what}: kind must be NORM_LAYER or NORM_RMS, not {kind!r}")
     n, Cc, f32 = x.B * x.H * x.W, x.C, torch.float32
     sx = _span(what, "x", x, n, None, (a16(), f32))
-    if n > 0x7fffffff or Cc > 1 << 20:
+    if n > 1 << 30 or Cc > 1 << 20:
         raise KernelError(f"{what}: {n} rows of {Cc} channels are more than the kernel indexes")
     types = (a16(), f32) if x.t.dtype == f32 else (a16(),)
     sf = None
@@ -928,6 +928,9 @@ def block_norm_backward(x, dy, dx=None, *, dxo=None, f=None, df=None, kind=NORM_
             if of is None:
                 raise KernelError(f"{what}: {name} of a parameter that the call has not")
             _check_vector(what, name, t, x.C * rows)
+    outs = [t.data_ptr() for t in (d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift) if t is not None]
+    if len(set(outs)) != len(outs) and x.B:
+        raise KernelError(f"{what}: two parameter gradients share memory")
     _check_device(what, [v.t for v in (x, f, dy, dxo, dx, df) if v is not None] +
                   [post_w, post_b, gate, w, b, scale, shift, d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift])
     side = f or dy

@@ -109,6 +109,8 @@ def test_block_norm_backward_refusals():
     refused("dx shares memory", bw, x, dy, dx, f=f, df=dx)
     refused("df shares memory", bw, x, dy, dx, dxo=dxo, f=f, df=f)
     refused("dxo is torch.float32", bw, x, dy, dx, dxo=view(B, N, Cc, F32))
+    once = vec(Cc)
+    refused("gradients share memory", bw, x, dy, dx, w=vec(Cc), b=vec(Cc), d_w=once, d_b=once)
     refused("is on cpu", bw, x, dy, dxo, dxo=dxo, f=f, df=dy)
 
 
@@ -124,7 +126,7 @@ def test_block_norm_c_statuses():
     assert block_norm_c(B=0) == 0 and block_norm_c(N=0, x=None, y=None) == 0
     assert block_norm_c(x=None) == -1 and block_norm_c(y=None) == -1
     for bad in (dict(C=0), dict(x_cs=7), dict(x_co=1), dict(x_co=-1), dict(y_cs=4), dict(B=-1), dict(B=1 << 20, N=1 << 20),
-                dict(scale=64, scale_rs=-8)):
+                dict(N=(1 << 30) + 1), dict(x_cs=-2 ** 31), dict(scale=64, scale_rs=-8)):
         assert block_norm_c(**bad) == -2, bad
     for bad in (dict(kind=2), dict(f_f32=1), dict(post=1), dict(gate=64), dict(post_w=64), dict(f=64), dict(xo=64)):
         assert block_norm_c(**bad) == -3, bad
@@ -187,7 +189,7 @@ def test_rotary_c_statuses():
     for name in ("q", "qo", "k", "ko", "pos", "turns", "axis"):
         assert status(**{name: None}) == -1
     for bad in (dict(pairs=5), dict(pairs=-1), dict(D=0), dict(axes=0), dict(qh=0), dict(kh=-1), dict(q_cs=15), dict(k_co=17), dict(ko_co=-1),
-                dict(B=1 << 20, N=1 << 20), dict(pos_bs=-1)):
+                dict(B=1 << 20, N=1 << 20), dict(pos_bs=-1), dict(q_cs=-2 ** 31), dict(ko_cs=-2 ** 31)):
         assert status(**bad) == -2, bad
 
 
@@ -247,7 +249,8 @@ def test_mxfp4_c_statuses():
     assert status() == 0 and status(epi=K.EPI_GEGLU, y_cs=32) == 0
     for bad in (dict(xc=None), dict(xs=None), dict(wc=None), dict(ws=None), dict(y=None)):
         assert status(**bad) == -1, bad
-    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(y_cs=63), dict(y_co=1), dict(wc=4104), dict(xs=4098), dict(res=64, r_co=1)):
+    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(y_cs=63), dict(y_co=1), dict(wc=4104), dict(xs=4098), dict(res=64, r_co=1),
+                dict(y_cs=-2 ** 31), dict(res=64, r_cs=-2 ** 31), dict(xc=None, xr=64, xr_cs=-2 ** 31)):
         assert status(**bad) == -2, bad
     for bad in (dict(epi=K.EPI_GLU_LEAKY), dict(epi=9), dict(epi=K.EPI_GEGLU, N=48, y_cs=64)):
         assert status(**bad) == -3, bad
@@ -258,5 +261,7 @@ def test_mxfp4_c_statuses():
     assert lib.onedc_mxfp4_quantize(None, 0, 8, 0, 64, 64, 1, 8, None) == -1
     assert lib.onedc_mxfp4_quantize(64, 0, 7, 0, 64, 64, 1, 8, None) == -2
     assert lib.onedc_mxfp4_quantize(64, 0, 8, 0, 72, 64, 1, 8, None) == -2
+    assert lib.onedc_mxfp4_quantize(64, 0, -2 ** 31, 0, 64, 64, 0, 8, None) == -2
+    assert lib.onedc_mxfp4_dequantize(64, 64, 64, 0, -2 ** 31, 0, 0, 8, None) == -2
     assert lib.onedc_mxfp4_dequantize(64, 64, 64, 0, 8, 1, 1, 8, None) == -2
     assert lib.onedc_mxfp4_dequantize(64, 64, None, 0, 8, 0, 1, 8, None) == -1
