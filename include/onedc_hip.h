@@ -402,8 +402,8 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream);
  * be dy.  Parameter gradients, f32, each NULL where not wanted: d_post_w, d_post_b, d_w, d_b [C]; d_gate, d_scale, d_shift [C] per
  * picture, dense -- or one row summed over the pictures where the parameter is one row for all (*_rs == 0).
  * Sums over rows run in a fixed order (no atomics): partial sums per run of rows in ws, f32 inside a run, f64 across runs.
- * ws: onedc_block_norm_backward_ws_bytes(p, g) bytes of device scratch, the call's own until it has run (0: none needed).
- * Statuses as above; -15: ws missing or too small. */
+ * ws: onedc_block_norm_backward_ws_bytes(p, g) bytes of device scratch, 16-byte aligned, the call's own until it has run (0: none
+ * needed).  Statuses as above; -15: ws missing, too small or not aligned. */
 typedef struct onedc_block_norm_grad {
     const void *dy; const void *dxo; void *dx; void *df;
     float *d_post_w; float *d_post_b; float *d_gate; float *d_w; float *d_b; float *d_scale; float *d_shift;

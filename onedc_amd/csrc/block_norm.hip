@@ -42,6 +42,19 @@ __device__ __forceinline__ float lanes_sum(float v, int L) {      // (L is wave-
     const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
     return L > 32 ? __uint_as_float(b[0]) + __uint_as_float(b[1]) : v;
 }
+// sum over a wave's groups of L lanes, lane by lane
+__device__ __forceinline__ float groups_sum(float v, int L) {
+    if (L <= 8) v = dpp_add<0x128>(v);               // rotated by 8 within 16
+    if (L <= 16) {
+        const u32x2_t a = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    if (L <= 32) {
+        const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+        v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+    return v;
+}
 // ... or over the workgroup; red: two floats a wave, alternated so that one barrier a sum is enough
 template <int NTH, bool SHARED>
 struct RowSum {
@@ -75,26 +88,39 @@ struct RowSum {
     }
 };
 
-// eight channels as they lie in memory (any alignment of the type's own)
+// Eight channels as they lie in memory (any alignment of the type's own).  A row's ragged last piece is read from the row's last eight
+// channels and moved down when it is needed: a load of single values would be waited for on the spot, in every one of a row's operands
+// (16 x 2304 x 643: 167 us the backward pass that way).
 template <bool F32>
 struct Eight {
     uint4 w[F32 ? 2 : 1];
-    // TAIL: the row may end inside the piece
-    template <bool TAIL>
-    __device__ __forceinline__ void load(const void *base, int64_t at, int left) {
+    // left: channels of the row from here on; past: how many of the eight lie behind its end
+    __device__ __forceinline__ void load(const void *base, int64_t at, int left, int past) {
         typedef typename Elem<F32>::T T;
-        const T *p = (const T *)base + at;
-        if (left >= 8) {
-            __builtin_memcpy(w, p, sizeof(w));
-        } else if (!TAIL) {
+        if (left > 0) {
+            __builtin_memcpy(w, (const T *)base + at - past, sizeof(w));
+        } else {
 #pragma unroll
             for (int j = 0; j < (F32 ? 2 : 1); ++j) w[j] = make_uint4(0, 0, 0, 0);
-        } else {
-            T v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : (T)0;
-            __builtin_memcpy(w, v, sizeof(w));
         }
+    }
+    // `past` channels down, zeros behind
+    __device__ __forceinline__ void settle(int past) {
+        constexpr int N = F32 ? 8 : 4;               // words
+        uint32_t u[N];
+        __builtin_memcpy(u, w, sizeof(w));
+#pragma unroll
+        for (int by = N / 2; by > 0; by >>= 1) {
+            const bool on = past & (F32 ? by : 2 * by);
+#pragma unroll
+            for (int j = 0; j < N; ++j) u[j] = on ? j + by < N ? u[j + by] : 0u : u[j];
+        }
+        if (!F32) {
+            const uint32_t half = (past & 1) * 16;
+#pragma unroll
+            for (int j = 0; j < N; ++j) u[j] = __builtin_amdgcn_alignbit(j + 1 < N ? u[j + 1] : 0u, u[j], half);
+        }
+        __builtin_memcpy(w, u, sizeof(w));
     }
     __device__ __forceinline__ float get(int j) const {
         const uint32_t *u = (const uint32_t *)w;
@@ -122,6 +148,16 @@ __device__ __forceinline__ void put8(void *base, int64_t at, const float (&v)[8]
         for (int j = 0; j < 8; ++j)
             if (j < left) Elem<F32>::put(p + j, v[j]);
     }
+}
+
+// A thread's first piece of a row: its lane.  The ragged last piece reads channels of the piece in front of it, and a call may be in place: the
+// two belong to one wave, whose loads of a row are issued in front of its stores.
+template <bool SHARED, bool TAIL, int NTH>
+__device__ __forceinline__ int piece_of(int L, int C) {
+    const int lane = threadIdx.x & (L - 1);
+    if (SHARED || !TAIL) return lane;
+    const int last = (C >> 3) & (NTH - 1), a = (last + 1) & (NTH - 1), b = (last - 1) & (NTH - 1);
+    return last & 63 ? lane : lane == a ? b : lane == b ? a : lane;
 }
 
 struct Plan {
@@ -217,7 +253,7 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_nor
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const bool has_f = OPT || p.f, has_y = OPT || p.y, post = OPT ? OPT == JOIN_POST : p.post;
     const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
-    const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
+    const int L = SHARED ? pl.L : NTH, step = 8 * L, c0 = piece_of<SHARED, TAIL, NTH>(L, p.C) * 8, each = NTH / L;
     float *at_lds = lds + 4 * (NTH / 64);
     Vector<IT, SHARED, HAS_A> A;
     Vector<IT, SHARED, HAS_AB> Ab;
@@ -232,11 +268,15 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_nor
     const int64_t row0 = (int64_t)b * p.N;
     Eight<X32> x[IT];
     Eight<F32> f[IT];
+    auto past = [&](int i) { return TAIL ? max(c0 + i * step + 8 - p.C, 0) & 7 : 0; };       // (8 on: a piece behind the row)
+    auto settle = [&](auto &piece, int i) {
+        if (TAIL) piece.settle(past(i));
+    };
     auto load = [&](auto &to, const void *from, int cs, int co, int n) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = c0 + i * step;
-            to[i].template load<TAIL>(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0);
+            to[i].load(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0, past(i));
         }
     };
     int n = run * pl.run_rows + threadIdx.x / L;
@@ -250,16 +290,20 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_nor
         const bool more = left_rows > each;
         float t[IT][8];
 #pragma unroll
-        for (int i = 0; i < IT; ++i)
+        for (int i = 0; i < IT; ++i) {
+            settle(x[i], i);
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[i][j] = x[i].get(j);
+        }
         if (more) load(x, p.x, p.x_cs, p.x_co, n + each);
         if (has_f) {
             float v[IT][8];
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                settle(f[i], i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[i][j] = f[i].get(j);
+            }
             if (more) load(f, p.f, p.f_cs, p.f_co, n + each);
             if (post) normalise<TAIL>(v, c0, step, p.C, p.kind, p.eps, sum);
 #pragma unroll
@@ -300,7 +344,7 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 2 ? 3 : 4) void block_nor
 }
 
 // Backward: dx and df of a row; a thread keeps the four sums of its channels over its run of rows, the lane groups of a workgroup add
-// theirs in order, and part[run of a picture][4][C] goes to the next kernel.
+// theirs in a fixed order, and part[run of a picture][4][C rounded up to 8] goes to the next kernel.
 template <int NTH, bool SHARED, int IT, bool X32, bool F32, bool TAIL, int OPT>
 __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_norm_rows_backward_kernel(onedc_block_norm_params p,
                                                                                                        onedc_block_norm_grad g, Plan pl, float *part) {
@@ -308,7 +352,7 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
     const bool has_f = OPT || p.f, has_dy = OPT || g.dy, has_dxo = OPT || g.dxo, has_dx = OPT || g.dx, has_df = OPT || g.df;
     const bool post = OPT ? OPT == JOIN_POST : p.post;
     const int b = blockIdx.x / pl.runs, run = blockIdx.x - b * pl.runs;
-    const int L = SHARED ? pl.L : NTH, lane = threadIdx.x & (L - 1), step = 8 * L, c0 = lane * 8, each = NTH / L;
+    const int L = SHARED ? pl.L : NTH, step = 8 * L, c0 = piece_of<SHARED, TAIL, NTH>(L, p.C) * 8, each = NTH / L;
     float *at_lds = lds + 4 * (NTH / 64);
     Vector<IT, SHARED, HAS_A> A;
     Vector<IT, SHARED, HAS_W> W;
@@ -320,11 +364,15 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
     // (raw until they are needed, and replaced by the next row's at once: rows of two pieces a lane fit 256 registers so)
     Eight<X32> rt[IT], rd[IT];
     Eight<F32> rf[IT], ry[IT];
+    auto past = [&](int i) { return TAIL ? max(c0 + i * step + 8 - p.C, 0) & 7 : 0; };       // (8 on: a piece behind the row)
+    auto settle = [&](auto &piece, int i) {
+        if (TAIL) piece.settle(past(i));
+    };
     auto load = [&](auto &to, const void *from, int cs, int co, int n) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int c = c0 + i * step;
-            to[i].template load<TAIL>(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0);
+            to[i].load(from, (row0 + n) * cs + co + c, n < n1 ? p.C - c : 0, past(i));
         }
     };
     float s1[IT][8], s2[IT][8], t1[IT][8], t2[IT][8];
@@ -349,9 +397,11 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
         if (has_dy) {
             float h[IT][8], u[IT][8];
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                settle(rt[i], i), settle(ry[i], i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] = rt[i].get(j), u[i][j] = ry[i].get(j);
+            }
             if (more) {
                 load(rt, p.x, p.x_cs, p.x_co, n + each);
                 load(ry, g.dy, g.dy_cs, g.dy_co, n + each);
@@ -384,9 +434,11 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
         }
         if (has_dxo) {
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                settle(rd[i], i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[i][j] = has_dy ? d[i][j] + rd[i].get(j) : rd[i].get(j);
+            }
             if (more) load(rd, g.dxo, g.dxo_cs, g.dxo_co, n + each);
         }
         if (has_dx && n < n1) {
@@ -396,9 +448,11 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
         }
         if (has_f) {
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                settle(rf[i], i);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[i][j] = rf[i].get(j);
+            }
             if (more) load(rf, p.f, p.f_cs, p.f_co, n + each);
         } else {
 #pragma unroll
@@ -439,21 +493,33 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
         }
     }
     if (!part) return;
-    float *out = part + (int64_t)blockIdx.x * 4 * p.C;
+    const int C8 = (p.C + 7) & ~7;
+    f32x4 *out = (f32x4 *)(part + (int64_t)blockIdx.x * 4 * C8);
     if constexpr (!SHARED) {                         // the thread's channels are nobody else's
 #pragma unroll
-        for (int i = 0; i < IT; ++i)
+        for (int i = 0; i < IT; ++i) {
+            const int c = c0 + i * step;
+            if (c >= p.C) continue;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = c0 + i * step + j;
-                if (c < p.C) out[c] = s1[i][j], out[p.C + c] = s2[i][j], out[2 * p.C + c] = t1[i][j], out[3 * p.C + c] = t2[i][j];
+            for (int q = 0; q < 4; ++q) {
+                const float(&v)[8] = q == 0 ? s1[i] : q == 1 ? s2[i] : q == 2 ? t1[i] : t2[i];
+                out[(q * C8 + c) / 4] = f32x4{v[0], v[1], v[2], v[3]};
+                out[(q * C8 + c) / 4 + 1] = f32x4{v[4], v[5], v[6], v[7]};
             }
+        }
     } else {
-        const int C8 = (p.C + 7) & ~7, group = threadIdx.x / L;
+        // the lane groups of a wave by exchanges, then the waves in turn
+        auto add_groups = [&](float (&v)[IT][8]) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = groups_sum(v[i][j], L);
+        };
+        add_groups(s1), add_groups(s2), add_groups(t1), add_groups(t2);
         float *acc = lds + 4 * (NTH / 64);           // over the vectors
-        for (int k = 0; k < each; ++k) {
+        for (int k = 0; k < NTH / 64; ++k) {
             __syncthreads();
-            if (group != k) continue;
+            if ((int)(threadIdx.x >> 6) != k || (int)(threadIdx.x & 63) >= L) continue;
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
                 const int c = c0 + i * step;
@@ -469,9 +535,7 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
             }
         }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            for (int c = threadIdx.x; c < p.C; c += NTH) out[q * p.C + c] = acc[q * C8 + c];
+        for (int c = threadIdx.x; c < C8; c += NTH) out[c] = ((const f32x4 *)acc)[c];
     }
 }
 
@@ -542,7 +606,7 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(onedc_block_norm_params 
     }
 }
 
-// dx and df of a row, and the row's four column terms added to this run's sums: sums[4][C] in LDS-free global scratch, one column
+// dx and df of a row, and the row's four column terms added to this run's sums: sums[4][C rounded up to 8] in memory, one column
 // owned by one thread for the whole run (fixed order)
 template <bool X32, bool F32>
 __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, float *part,
@@ -554,9 +618,10 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
     const int n0 = run * run_rows, n1 = min(p.N, n0 + run_rows);
     const float *gate = p.gate ? p.gate + (int64_t)b * p.gate_rs : nullptr;
     const float *scale = p.scale ? p.scale + (int64_t)b * p.scale_rs : nullptr;
-    float *sums = part ? part + (int64_t)blockIdx.x * 4 * p.C : nullptr;
+    const int C8 = (p.C + 7) & ~7;
+    float *sums = part ? part + (int64_t)blockIdx.x * 4 * C8 : nullptr;
     if (sums)
-        for (int c = threadIdx.x; c < 4 * p.C; c += NT) sums[c] = 0.f;      // (a thread's own columns differ from these: barrier below)
+        for (int c = threadIdx.x; c < 4 * C8; c += NT) sums[c] = 0.f;      // (a thread's own columns differ from these: barrier below)
     __syncthreads();
     for (int n = n0; n < n1; ++n) {
         const int64_t row = (int64_t)b * p.N + n;
@@ -603,9 +668,9 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
             if (sums) {
                 const float e = dy ? F::get(dy + c) : 0.f;
                 sums[c] += e;
-                sums[p.C + c] += dy ? e * hat(c) : 0.f;
-                sums[2 * p.C + c] += d;
-                sums[3 * p.C + c] += d * fh;
+                sums[C8 + c] += dy ? e * hat(c) : 0.f;
+                sums[2 * C8 + c] += d;
+                sums[3 * C8 + c] += d * fh;
             }
             // (dx may be dxo, df may be dy: this thread's own columns, read above)
             const float wc = w(c);
@@ -616,7 +681,7 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
     }
 }
 
-// The parameter gradients, in f64 and in a fixed order.  First a picture: 64 channels x 4 quarters of its runs a workgroup.  What has a row
+// The parameter gradients, in f64 and in a fixed order.  First a picture: 32 channels x 32 shares of its runs a workgroup.  What has a row
 // per picture is finished here; the picture's parts of what is summed over the pictures go on, parts[picture][7][C].
 enum { P_GATE, P_SCALE, P_SHIFT, P_W, P_B, P_POST_W, P_POST_B, PARTS };
 __device__ __forceinline__ void finish(const onedc_block_norm_params &p, const onedc_block_norm_grad &g, int c, const double (&t)[PARTS]) {
@@ -631,22 +696,38 @@ __device__ __forceinline__ void finish(const onedc_block_norm_params &p, const o
 
 __global__ __launch_bounds__(NT) void block_norm_picture_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, const float *part, double *parts,
                                                                 int runs) {
-    __shared__ double red[4][4][64];
-    const int columns = (p.C + 63) / 64, lane = threadIdx.x & 63;
+    __shared__ double red[32][4][32];
+    const int columns = (p.C + 31) / 32, C8 = (p.C + 7) & ~7;
     const int64_t b = blockIdx.x / columns;
-    const int c = (int)(blockIdx.x - b * columns) * 64 + lane, quarter = threadIdx.x >> 6;
-    double s[4] = {0, 0, 0, 0};
-    if (c < p.C)
-#pragma unroll 4
-        for (int r = quarter; r < runs; r += 4)
+    const int first = (int)(blockIdx.x - b * columns) * 32, share = threadIdx.x >> 3, at4 = (threadIdx.x & 7) * 4;
+    double sum[4][4] = {};
+    if (first + at4 < p.C)
+#pragma unroll 2
+        for (int r = share; r < runs; r += 32)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] += part[((b * runs + r) * 4 + k) * p.C + c];
+            for (int k = 0; k < 4; ++k) {
+                const f32x4 v = *(const f32x4 *)(part + ((b * runs + r) * 4 + k) * C8 + first + at4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) red[quarter][k][lane] = s[k];
+                for (int e = 0; e < 4; ++e) sum[k][e] += v[e];
+            }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[share][k][at4 + e] = sum[k][e];
     __syncthreads();
-    if (quarter || c >= p.C) return;
+    // two threads a sum, sixteen shares each
+    const int which = threadIdx.x & 127, half = threadIdx.x >> 7;
+    double total = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] = (red[0][k][lane] + red[1][k][lane]) + (red[2][k][lane] + red[3][k][lane]);      // S1, S2, T1, T2
+    for (int i = 0; i < 16; ++i) total += red[half * 16 + i][which >> 5][which & 31];
+    __syncthreads();
+    red[half][which >> 5][which & 31] = total;
+    __syncthreads();
+    const int c = first + threadIdx.x;
+    if (threadIdx.x >= 32 || c >= p.C) return;
+    double s[4];                                     // S1, S2, T1, T2
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = red[0][k][threadIdx.x] + red[1][k][threadIdx.x];
     const double w = at(p.w, c, 1.f), bb = at(p.b, c, 0.f), pw = at(p.post_w, c, 1.f), pb = at(p.post_b, c, 0.f);
     const double sc = 1.0 + at(p.scale, b * p.scale_rs + c, 0.f), ga = p.alpha * (double)at(p.gate, b * p.gate_rs + c, 1.f);
     const double t[PARTS] = {p.alpha * (pw * s[3] + pb * s[2]), w * s[1] + bb * s[0], s[0], sc * s[1], sc * s[0], ga * s[3], ga * s[2]};
@@ -717,12 +798,13 @@ onedc_block_norm_params joined_pictures(const onedc_block_norm_params *p) {
 // of 64 lanes end (1280 channels: 4.3 against 3.8 for one row a workgroup), but not with a ragged end, whose code takes their registers.
 // Wider rows belong to a workgroup each, one piece a thread (two from 8192 channels on, forward).
 struct Shape {
-    int threads, it, most;                // threads a workgroup; pieces a lane; 0: the row is too wide for registers
+    int threads, it;                      // threads a workgroup; pieces a lane; 0: not a row for registers
     bool shared;                          // several rows a workgroup
 };
 Shape row_shape(int C, int widest, bool back, int *L) {
     const int pieces = (C + 7) / 8;
-    Shape s = {NT, 0, widest, true};
+    Shape s = {NT, 0, true};
+    if (C < 8) return s;                             // (less than a piece: the simple kernel)
     for (*L = 8; *L <= 64; *L *= 2)
         if (pieces <= 2 * *L) {
             s.it = pieces <= *L ? 1 : 2;
@@ -751,30 +833,44 @@ void cut_runs(const onedc_block_norm_params &p, int each, int want, Plan *pl) {
     pl->run_rows = (turns + want - 1) / want * each;
     pl->runs = (p.N + pl->run_rows - 1) / pl->run_rows;
 }
+// of the workspace: the pictures' sums, in front of the runs' (whole 16 bytes)
+int64_t pictures_bytes(const onedc_block_norm_params &q, const onedc_block_norm_grad *g) {
+    return q.B > 1 && wants_all(&q, g) ? (((int64_t)q.B * q.C * PARTS * (int64_t)sizeof(double) + 15) & ~15ll) : 0;
+}
 constexpr int WIDEST = 16384, WIDEST_BACK = 8192;
 constexpr int SIMPLE_RUNS = 512;
 
 // shape and runs of a backward pass; false: the simple kernel (it cuts runs of its own)
-bool backward_plan(const onedc_block_norm_params &p, Shape *s, Plan *pl) {
+bool backward_plan(const onedc_block_norm_params &p, bool sums, Shape *s, Plan *pl) {
     *s = row_shape(p.C, WIDEST_BACK, true, &pl->L);
     if (!s->it) {
         cut_runs(p, 1, SIMPLE_RUNS, pl);
         return false;
     }
-    cut_runs(p, s->threads / pl->L, s->shared ? 1024 : s->threads == 256 ? 1024 : 512, pl);
+    const int each = s->threads / pl->L;
+    int want = s->threads == NT ? 1024 : 512;
+    if (sums) {                                      // fewer of them: a run's sums are 16 bytes a channel to write and to read
+        const int64_t fours = (int64_t)p.B * p.N / (4 * each);
+        want = fours < want / 2 ? (int)fours : want / 2;
+        want = want < 256 ? 256 : want;
+    }
+    cut_runs(p, each, want, pl);
     pl->has = (p.f && (p.gate || p.post_w) ? HAS_A : 0) | (p.w || p.scale ? HAS_W : 0);
     return true;
 }
 
-// one instance of a kernel template for every shape, type and end of a row, and what the call has (rows with a ragged end: GENERIC)
+// one instance of a kernel template for every shape, type and end of a row, and what the call has
 template <class Call>
 void by_shape(const Shape &s, bool x32, bool f32, bool tail, int opt, Call &&call) {
     auto types = [&](auto nth, auto shared, auto it) {
         auto ends = [&](auto x, auto f) {
-            if (tail) call(nth, shared, it, x, f, std::true_type(), std::integral_constant<int, GENERIC>());
-            else if (opt == JOIN) call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, JOIN>());
-            else if (opt == JOIN_POST) call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, JOIN_POST>());
-            else call(nth, shared, it, x, f, std::false_type(), std::integral_constant<int, GENERIC>());
+            auto has = [&](auto end) {
+                if (opt == JOIN) call(nth, shared, it, x, f, end, std::integral_constant<int, JOIN>());
+                else if (opt == JOIN_POST) call(nth, shared, it, x, f, end, std::integral_constant<int, JOIN_POST>());
+                else call(nth, shared, it, x, f, end, std::integral_constant<int, GENERIC>());
+            };
+            if (tail) has(std::true_type());
+            else has(std::false_type());
         };
         if (f32) ends(std::true_type(), std::true_type());
         else if (x32) ends(std::true_type(), std::false_type());
@@ -819,7 +915,7 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
                  (p->y && (p->b || p->shift) ? HAS_S : 0);
         cut_runs(q, shape.threads / pl.L, shape.threads > 256 ? 512 : 1024, &pl);
         const int opt = !p->f || !p->y || p->post_b ? GENERIC : p->post ? JOIN_POST : JOIN;
-        if (opt && !(p->C & 7)) pl.has = HAS_A | HAS_W | HAS_S;
+        if (opt) pl.has = HAS_A | HAS_W | HAS_S;
         const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * ((p->C + 7) & ~7) * 4 : 0);
         const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
         by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
@@ -846,9 +942,8 @@ int64_t onedc_block_norm_backward_ws_bytes(const onedc_block_norm_params *p, con
     const onedc_block_norm_params q = joined_pictures(p);
     Shape s;
     Plan pl;
-    backward_plan(q, &s, &pl);
-    // the pictures' sums in front of the runs' (8-byte aligned)
-    return (q.B > 1 && wants_all(p, g) ? (int64_t)q.B * p->C * PARTS * sizeof(double) : 0) + (int64_t)q.B * pl.runs * 4 * p->C * sizeof(float);
+    backward_plan(q, true, &s, &pl);
+    return pictures_bytes(q, g) + (int64_t)q.B * pl.runs * 4 * ((p->C + 7) & ~7) * sizeof(float);
 }
 
 int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_block_norm_grad *g, void *stream) {
@@ -868,14 +963,14 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
             return -3;
     }
     const bool sums = wants_sums(g);
-    if (sums && (int64_t)p->B * ((p->C + 63) / 64) > 0x7fffffff) return -2;
+    if (sums && (int64_t)p->B * ((p->C + 31) / 32) > 0x7fffffff) return -2;
     const int64_t need = onedc_block_norm_backward_ws_bytes(p, g);
-    if (need && (!g->ws || g->ws_bytes < need)) return -15;
+    if (need && (!g->ws || g->ws_bytes < need || (uintptr_t)g->ws & 15)) return -15;
     if (!any) {
         if (sums) {                                  // no rows: every sum is 0
             onedc_block_norm_params none = *p;
             if (p->B) {
-                hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)p->B * ((p->C + 63) / 64))), dim3(NT), 0, as_stream(stream),
+                hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)p->B * ((p->C + 31) / 32))), dim3(NT), 0, as_stream(stream),
                                    none, *g, (const float *)nullptr, (double *)nullptr, 0);
                 ONEDC_LAUNCH_CHECK();
             }
@@ -888,9 +983,9 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     const onedc_block_norm_params q = joined_pictures(p);
     Shape shape;
     Plan pl;
-    const bool rows = backward_plan(q, &shape, &pl);
-    double *pictures = sums && q.B > 1 && wants_all(p, g) ? (double *)g->ws : nullptr;
-    float *part = sums ? (float *)((char *)g->ws + (pictures ? (int64_t)q.B * p->C * PARTS * sizeof(double) : 0)) : nullptr;
+    const bool rows = backward_plan(q, sums, &shape, &pl);
+    double *pictures = sums && pictures_bytes(q, g) ? (double *)g->ws : nullptr;
+    float *part = sums ? (float *)((char *)g->ws + pictures_bytes(q, g)) : nullptr;
     const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
     if (rows) {
         const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most, then the sums)
@@ -912,7 +1007,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     }
     ONEDC_LAUNCH_CHECK();
     if (sums) {
-        hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)q.B * ((p->C + 63) / 64))), dim3(NT), 0, as_stream(stream), q, *g, part,
+        hipLaunchKernelGGL(block_norm_picture_kernel, dim3((unsigned)((int64_t)q.B * ((p->C + 31) / 32))), dim3(NT), 0, as_stream(stream), q, *g, part,
                            pictures, pl.runs);
         ONEDC_LAUNCH_CHECK();
         if (pictures) {

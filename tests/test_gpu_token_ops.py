@@ -253,6 +253,40 @@ def test_block_norm_with_no_epsilon(Cc, fmt):
         assert float((got.reshape(want.shape) - want).norm() / want.norm()) < (2 * half_step(fmt) if name in ("dx", "df") else 2e-5), name
 
 
+@pytest.mark.parametrize("Cc", [8, 11, 643, 1027, 1542, 1283, 2051, 4103, 8193])
+def test_block_norm_in_place_with_a_ragged_end(Cc, fmt):
+    """A row's last channels are read together with those in front of them, which in place other lanes store over (widths around whole
+    waves of a row): the same bits as out of place, forward and backward, without a norm in between that would hold the lanes together."""
+    B, N = 2, 700
+    g = torch.Generator(device=DEV).manual_seed(Cc)
+
+    def mk(dt):
+        return View(torch.randn(B * N * Cc, generator=g, device=DEV).to(dt), B, 1, N, Cc)
+    gate = torch.randn(B, Cc, generator=g, device=DEV)
+    for xt in (fmt, F32):
+        x, f, xo, dxo, dx, df = mk(xt), mk(fmt), mk(xt), mk(xt), mk(xt), mk(fmt)
+        K.block_norm(x, f=f, xo=xo, gate=gate, alpha=0.5)
+        part = (0.5 * gate[:, None] * f.t.float().view(B, N, Cc)).reshape(-1)
+        want = x.t.float() + part                     # (f32 too: four roundings here and there of what is added)
+        assert bool(((xo.t.float() - want).abs() <= half_step(xt) * want.abs() + tiny(xt) + 4 * EPS32 * (x.t.float().abs() + part.abs())).all())
+        keep = x.t.clone()
+        K.block_norm(x, f=f, xo=x, gate=gate, alpha=0.5)
+        assert torch.equal(x.t, xo.t)
+        x.t.copy_(keep)
+        K.block_norm_backward(xo, None, dx, dxo=dxo, f=f, df=df, gate=gate, alpha=0.5)
+        assert torch.equal(dx.t, dxo.t)
+        df2 = mk(fmt)
+        K.block_norm_backward(xo, None, dxo, dxo=dxo, f=f, df=df2, gate=gate, alpha=0.5)
+        assert torch.equal(dx.t, dxo.t) and torch.equal(df.t, df2.t)
+        y, y2, dy = mk(fmt), mk(fmt), mk(fmt)
+        K.block_norm(x, y, f=f, xo=xo, post=True)
+        K.block_norm(x, y2, f=f, xo=x, post=True)
+        assert torch.equal(x.t, xo.t) and torch.equal(y.t, y2.t)
+        K.block_norm_backward(x, dy, dx, dxo=dxo, f=f, df=df, post=True)
+        K.block_norm_backward(x, dy, dxo, dxo=dxo, f=f, df=dy, post=True)
+        assert torch.equal(dx.t, dxo.t) and torch.equal(df.t, dy.t)
+
+
 def test_block_norm_addresses_past_32_bits():
     """Rows 2^30 channels apart: the third begins 2^31 values into the buffer."""
     pitch, Cc = 1 << 30, 320
