@@ -371,18 +371,21 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned voff, unsigned soff, 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
-// WN x WM waves of FN x FM blocks of 32 x 32
-template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC>
-__global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_params p, int steps, int tiles_n, int tiles_m, int whole) {
+// WN x WM waves of FN x FM blocks of 32 x 32; KG such teams share the tile, each with a ring of its own and a part of K, and the first adds their
+// sums in order
+template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC, int KG>
+__global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp4_params p, int steps, int tiles_n, int tiles_m, int whole) {
     constexpr int NW = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, ROW = 64 * KS, STAGE = (TN + TM) * ROW;
     constexpr int RI = 16 / KS;                      // rows of a DMA instruction
     constexpr int IN = TN / RI / NW, IM = TM / RI / NW, NI = IN + IM;
     constexpr int GROUP = (TN + TM) * 32, NSC = ((TN + TM) / 32 + NW - 1) / NW, RING = NST * STAGE;     // scales of eight steps, behind the ring
     constexpr int GS = 8 / KS;                       // stages of a group of scales
     static_assert(TN % (RI * NW) == 0 && TM % (RI * NW) == 0, "whole DMA instructions a wave");
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(16))) char all_smem[];
+    const int lane = threadIdx.x & 63, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, kb = lane >> 5;
+    const int team = KG > 1 ? any_wave / NW : 0, wave = any_wave - team * NW;
+    char *const smem = all_smem + team * (RING + GROUP);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, kb = lane >> 5;
     const int wn = wave / WM, wm = wave - wn * WM;
     // tiles that run at the same time on one XCD share operands: eight rows of tiles deep, then along n
     const int logical = xcd_logical_tile(blockIdx.x, tiles_n * tiles_m);
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_par
     uint32_t sc[FN + FM][2][2];
     const uint32_t pick0 = (uint32_t)kb * 0x0101u + 0x0400u, pick1 = pick0 + 0x0202u;
     auto take_scales = [&](int g) {
-        const int left = steps - 8 * g;                                          // steps behind the last: scale 2^-127, never a NaN
+        const int left = KG > 1 ? max(steps - 8 * g, 0) : steps - 8 * g;          // steps behind the last: scale 2^-127, never a NaN
         const uint32_t real[2] = {left >= 4 ? ~0u : (1u << 8 * left) - 1, left >= 8 ? ~0u : left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1};
 #pragma unroll
         for (int i = 0; i < FN + FM; ++i)
@@ -464,11 +467,12 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_par
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const int swap = KS == 2 ? r & 7 : (r >> 1) & 3;
 
-    const int stages = (steps + KS - 1) / KS, groups = (steps + 7) >> 3;
-    stage_scales(0);
+    // a team's groups of scales, and where they begin; every team makes the same turns (those behind the last step multiply zeros)
+    const int groups = (((steps + 7) >> 3) + KG - 1) / KG, g0 = team * groups, stages = min(g0 * GS + (steps + KS - 1) / KS, (g0 + groups) * GS);
+    stage_scales(g0);
     constexpr int AHEAD = NST > 1 ? NST - 1 : 1;     // stages in flight
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) stage(i, i);
+    for (int i = 0; i < AHEAD; ++i) stage(g0 * GS + i, i);
     int slot = 0, fill = NST - 1;
     // I: stage of the group
     auto go = [&](auto ic, int t) {
@@ -517,7 +521,7 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_par
         }
         if (I == 1) stage_scales((t * KS >> 3) + 1);             // (every wave has taken this group's: a barrier ago)
     };
-    for (int g = 0; g < groups; ++g) {
+    for (int g = g0; g < g0 + groups; ++g) {
         const int t = g * GS;
         go(std::integral_constant<int, 0>(), t);
         if (t + 1 < stages) go(std::integral_constant<int, 1>(), t + 1);
@@ -531,7 +535,22 @@ __global__ __launch_bounds__(64 * WN * WM, OCC) void tile_kernel(onedc_mxfp4_par
         }
     }
     MX_VMCNT(0);
-    __syncthreads();                                 // the ring is free: the waves' own scratch from here
+    __syncthreads();                                 // the rings are free: the waves' own scratch from here
+    if constexpr (KG > 1) {
+        f32x4 *const sums = (f32x4 *)(all_smem + NW * 32 * (FN * 32 + 4) * 4);          // behind that scratch
+        constexpr int PER = FN * FM * 4;
+        if (team) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                sums[(((team - 1) * NW + wave) * PER + i) * 64 + lane] = *((const f32x4 *)&acc[0][0] + i);
+        }
+        __syncthreads();
+        if (team) return;
+#pragma unroll
+        for (int t = 0; t < KG - 1; ++t)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) *((f32x4 *)&acc[0][0] + i) += sums[((t * NW + wave) * PER + i) * 64 + lane];
+    }
 
     // epilogue: 32 activation rows at a time through LDS, so that a row's outputs leave as whole lines.  Of a block a lane holds activation
     // row r and weight rows 8 q + 4 kb + e (q = 0 .. 3, e = 0 .. 3); a gated layer's block is 16 values and their 16 gates
@@ -615,16 +634,18 @@ int launch_skinny(const onedc_mxfp4_params *p, int steps, int whole, void *strea
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
-template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC>
+template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC, int KG>
 int launch_tiles(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
     static_assert(FN == 1 || FN == 2 || FN == 4, "");
     constexpr int TN = 32 * WN * FN, TM = 32 * WM * FM;
-    constexpr int ring = (TN + TM) * (NST * KS * 64 + 32), scratch = WN * WM * 32 * (FN * 32 + 4) * 4, lds = ring > scratch ? ring : scratch;
+    constexpr int ring = KG * (TN + TM) * (NST * KS * 64 + 32), scratch = WN * WM * (32 * (FN * 32 + 4) * 4 + (KG - 1) * FN * FM * 4096);
+    constexpr int lds = ring > scratch ? ring : scratch;
+    static_assert(lds <= 160 * 1024, "");
     static OnedcLdsAttrOnce once;
-    once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, KS, NST, OCC>, lds}});
+    once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, KS, NST, OCC, KG>, lds}});
     const int64_t tn = (p->N + TN - 1) / TN, tm = (p->M + TM - 1) / TM;
     if (tn * tm > 0x7fffffff) return -2;
-    hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, KS, NST, OCC>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM), lds, as_stream(stream), *p, steps,
+    hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, KS, NST, OCC, KG>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM * KG), lds, as_stream(stream), *p, steps,
                        (int)tn, (int)tm, whole);
     ONEDC_LAUNCH_CHECK();
     return 0;
@@ -681,15 +702,19 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     //   256 x 256, eight waves, two stages: the fewest bytes into LDS a product.  From 160 tiles on, where it pads no tenth more than 128 x 128;
     //     gated layers only from 32 steps on (8192 x 4096 x 5120: 95 us against 110; gated 8655 x 10240 x 1280: 117 against 100, there
     //     the epilogue counts, and nothing else runs on the CU meanwhile)
+    //   64 x 64, two teams of four waves that halve a long K, while there is no second workgroup for a CU: one team waits where the other
+    //     multiplies (300 x 520 x 8192: 9.8 us against 12.4, 1024 x 1024 x 8192: 12.0 against 14.1; with 10 steps 9.8 against 5.9, three or four
+    //     teams 10.2 and 10.5 in the first case)
     //   64 x 64, three stages, while they fit the CUs' first four each (2048 x 1280 x 5120: 17 us against 19; 4096 x 1280 x 5120: 28 against 26)
     //   128 x 128: one stage and three workgroups a CU that load and multiply in turn; two stages where there are less than two a CU
     //     (4096 x 1280 x 5120: 26 us against 28; 8192 x 4096 x 5120: 112 against 110)
     const auto tiles = [&](int64_t t) { return ((p->N + t - 1) / t) * ((p->M + t - 1) / t); };
     const bool gated = p->epi == ONEDC_EPI_GEGLU;
-    if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 2>(p, steps, whole, stream);
-    if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 2, 3, 4>(p, steps, whole, stream);
-    if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 2>(p, steps, whole, stream);
-    return launch_tiles<2, 2, 2, 2, 2, 1, 3>(p, steps, whole, stream);
+    if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 2, 1>(p, steps, whole, stream);
+    if (tiles(64) <= 256 && steps >= 32) return launch_tiles<2, 2, 1, 1, 2, 3, 2, 2>(p, steps, whole, stream);
+    if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 2, 3, 4, 1>(p, steps, whole, stream);
+    if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 2, 1>(p, steps, whole, stream);
+    return launch_tiles<2, 2, 2, 2, 2, 1, 3, 1>(p, steps, whole, stream);
 }
 
 }  // extern "C"

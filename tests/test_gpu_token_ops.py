@@ -710,6 +710,8 @@ LIN = [
     (1031, 1280, 384, "linear", True, False),
     (2500, 96, 5120, "silu", False, True),
     (50, 3, 100, "linear", True, False),
+    (33, 65, 4097, "silu", True, False),
+    (70, 160, 8191, "geglu", True, True),
     (40, 1, 300, "linear", False, True),
 ]
 EPI = {"linear": K.EPI_LINEAR, "leaky": K.EPI_LEAKY, "silu": K.EPI_SILU, "geglu": K.EPI_GEGLU}
