@@ -1,9 +1,9 @@
 // mxfp4.hip — 4-bit microscaled floating point (OCP MX v1.0, MXFP4): quantise, read back, and the product of two such matrices.
 //
 // A block of 32 consecutive values of a row is 2^e * q, q in e2m1: e = max(floor(log2 amax) - 2, -127), so amax * 2^-e lies in [4, 8)
-// and is the only place where the largest code, 6, saturates.  v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 rows over
-// 128 values: lane l holds row l % 16, values 32 (l / 16) .. + 31 (16 bytes of codes) and that block's scale byte -- the memory
-// layout itself, no shuffle.  Its products are exact, the sums f32.
+// and is the only place where the largest code, 6, saturates.  The scaled matrix instructions take 32 values of a row in a lane -- 16 bytes of codes
+// and that block's scale byte -- which is the memory layout itself, no shuffle: 16x16x128 (lane l: row l % 16, values 32 (l / 16) on)
+// for few rows, 32x32x64 (row l % 32, values 32 (l / 32) on) for tiles.  Products are exact, sums f32.
 #include <type_traits>
 
 #include "conv_common.h"
@@ -100,7 +100,8 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true));
 }
 
-// Four neighbouring lanes hold a block, eight values each: a wave reads 1 KB (16-bit) in a row and writes 256 bytes of codes.  HBM bound.
+// Four neighbouring lanes hold a block, eight values each: a wave reads 1 KB (16-bit) in a row and writes 256 bytes of codes.  HBM bound: 16384 x 8192
+// bf16 to codes 59 us, 5.7 TB/s, and back 60 us, 5.6 TB/s (f32 109 us, 5.6 TB/s; back 155 us, 3.9 TB/s: 32 bytes a lane to store).
 // A workgroup takes QN consecutive groups of 256 pieces of eight values, the pieces of all rows counted through.
 constexpr int QN = 4;
 template <bool F32, bool VEC>
@@ -238,6 +239,7 @@ __device__ __forceinline__ void store8(const onedc_mxfp4_params &p, int64_t m, i
 // consecutive steps of a round straight from memory, 256 bytes of every weight row and 16 bytes of its scales, all in flight at once (steps dealt
 // out in turn instead would send all waves to the same memory channels where a row is a power of two long: 8192 x 8192 against one row 11.3 us
 // that way).  The waves' sums are added through LDS in wave order.  Raw rows are quantised by the workgroup together, under the weights' loads, into LDS.
+// 8192 x 8192 against one row of codes 8.2 us (4.3 TB/s of weights), a raw row 8.7 us, sixteen 9.8 and 13.1 us.
 constexpr int SKW = 16, SKU = 4, ROUND = SKW * SKU;                       // steps of a round
 constexpr int XPITCH = ROUND * 64 + 16, SPITCH = ROUND * 4 + 16;          // bytes of a row's codes and scales in LDS, off the banks' period
 
@@ -356,6 +358,11 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, 
 // words that the matrix instruction picks from.
 // The DMA is written as instructions (it has no destination register): behind the builtin the compiler drains every DMA in flight
 // before each LDS read.
+// 32x32x64 in place of 16x16x128: 6.4 against 5.2 - 5.9 PFLOP/s from registers on random codes, where power bounds it (9.7 on zeros).
+// 16384 x 8192 x 8192, 256 x 256: 550 - 572 us, 3.8 - 4.0 PFLOP/s.  Without the DMA it takes 465, without the LDS reads 524, without both
+// 373, without the stores 507, the products alone 337: the feeding and the power limit bound it together.  Stages of one step in rings of
+// three and four, 2 x 4 waves, other spacings of the DMA and outputs stored from registers (605 us) gained nothing.  4096^3 40 us, 3.4 PFLOP/s;
+// 8655 x 10240 x 1280 gated 98 - 102 us, 2.2 PFLOP/s: ten steps a tile, its GELU costs as much as its products.
 #define MX_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;

@@ -7,7 +7,12 @@
 //
 // Bound by HBM: q and k are read and written once, 3 operations an element.  What has to stay off that path are the angles: a
 // workgroup computes the sines and cosines of its T tokens once, into LDS, and all heads of those tokens read them from there (neighbouring
-// lanes hold neighbouring heads, so most of a wave's LDS reads are one address).
+// lanes hold neighbouring heads, so most of a wave's LDS reads are one address).  Pieces of 16 bytes where the sizes allow it, two or four of a
+// thread in flight.  16-bit heads: 49152 tokens x 32 x 80 in 101 us, 5.0 TB/s (a copy of 1 GB reaches 5.15; with the angles computed at every element
+// 328 us), 36864 x 16 x 80, which the last-level cache holds, 31 - 33 us, 5.8 - 6.1 TB/s; pairs of which only four share a piece (16384 x 32 x 72) 25 us,
+// 6.0 TB/s, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; one token 3.0 us in a graph, a launch's own time.
+#include <type_traits>
+
 #include "conv_common.h"
 #include "elem.h"
 
@@ -56,7 +61,8 @@ struct Units {
     OnedcFastDiv by_unit, by_head, by_pair;
 };
 
-template <bool F32, int VEC, bool NEIGHBOURS>
+// units of a thread in flight
+template <bool F32, int VEC, bool NEIGHBOURS, int FLY>
 __global__ __launch_bounds__(NT) void rotary_kernel(onedc_rotary_params p, Units u) {
     typedef typename Elem<F32>::T T;
     extern __shared__ __attribute__((aligned(16))) float table[];         // [T][pairs] cosines, then sines
@@ -79,57 +85,62 @@ __global__ __launch_bounds__(NT) void rotary_kernel(onedc_rotary_params p, Units
     __syncthreads();
 
     const int heads = p.qh + p.kh, total = tokens * heads * u.per;
-    for (int i = threadIdx.x; i < total; i += NT) {
-        const int th = u.by_unit.div(i), unit = i - th * u.per;
-        const int t = u.by_head.div(th), h = th - t * heads;
-        const int64_t row = row0 + t;
-        const bool isq = h < p.qh;
-        const T *src = isq ? (const T *)p.q + row * p.q_cs + p.q_co + h * p.D : (const T *)p.k + row * p.k_cs + p.k_co + (h - p.qh) * p.D;
-        T *dst = isq ? (T *)p.qo + row * p.qo_cs + p.qo_co + h * p.D : (T *)p.ko + row * p.ko_cs + p.ko_co + (h - p.qh) * p.D;
-        if (unit >= u.turn) {
-            const int at = 2 * p.pairs + (unit - u.turn) * VEC;
-            Piece<F32, VEC> v;
-            v.load(src + at);
-            v.store(dst + at);
-            continue;
+    constexpr bool TWO = VEC == 1 || !NEIGHBOURS;    // pieces of a turning unit
+    for (int i0 = threadIdx.x; i0 < total; i0 += NT * FLY) {
+        T *dst[FLY];
+        int first[FLY], second[FLY], entry[FLY];     // where its pieces begin in the head, and its pairs in the table (-1: passes through)
+        Piece<F32, VEC> a[FLY], b[FLY];
+#pragma unroll
+        for (int q = 0; q < FLY; ++q) {
+            const int i = min(i0 + q * NT, total - 1);       // (behind the last: loaded, not stored)
+            const int th = u.by_unit.div(i), unit = i - th * u.per;
+            const int t = u.by_head.div(th), h = th - t * heads;
+            const int64_t row = row0 + t;
+            const bool isq = h < p.qh;
+            const T *src = isq ? (const T *)p.q + row * p.q_cs + p.q_co + h * p.D : (const T *)p.k + row * p.k_cs + p.k_co + (h - p.qh) * p.D;
+            dst[q] = isq ? (T *)p.qo + row * p.qo_cs + p.qo_co + h * p.D : (T *)p.ko + row * p.ko_cs + p.ko_co + (h - p.qh) * p.D;
+            const bool turns = unit < u.turn;
+            const int wide = VEC == 1 && NEIGHBOURS ? 2 : VEC, passed = 2 * p.pairs + (unit - u.turn) * VEC;
+            first[q] = turns ? unit * wide : passed;
+            second[q] = !turns ? passed : NEIGHBOURS ? unit * wide + 1 : unit * VEC + p.pairs;
+            entry[q] = turns ? t * p.pairs + unit * (VEC == 1 ? 1 : NEIGHBOURS ? VEC / 2 : VEC) : -1;
+            a[q].load(src + first[q]);
+            if (TWO) b[q].load(src + second[q]);
         }
-        if constexpr (VEC == 1) {                                        // one pair
-            const float c = cosines[t * p.pairs + unit], s = sines[t * p.pairs + unit];
-            const int ia = NEIGHBOURS ? 2 * unit : unit, ib = NEIGHBOURS ? 2 * unit + 1 : unit + p.pairs;
-            Piece<F32, 1> a, b;
-            a.load(src + ia), b.load(src + ib);
-            const float x = a.get(0), y = b.get(0);
-            a.set1(x * c - y * s), b.set1(y * c + x * s);
-            a.store(dst + ia), b.store(dst + ib);
-        } else if constexpr (NEIGHBOURS) {                                // VEC / 2 pairs
-            typedef __attribute__((ext_vector_type(VEC / 2))) float C;
-            const C c = *(const C *)(cosines + t * p.pairs + unit * (VEC / 2)), s = *(const C *)(sines + t * p.pairs + unit * (VEC / 2));
-            Piece<F32, VEC> v;
-            v.load(src + unit * VEC);
 #pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) {
-                const float x = v.get(2 * j), y = v.get(2 * j + 1);
-                v.set(2 * j, x * c[j] - y * s[j], y * c[j] + x * s[j]);
-            }
-            v.store(dst + unit * VEC);
-        } else {                                                          // VEC pairs
-            typedef __attribute__((ext_vector_type(4))) float C;           // (four at a time: the table is 16-byte aligned)
-            C c[VEC / 4], s[VEC / 4];
+        for (int q = 0; q < FLY; ++q) {
+            if (i0 + q * NT >= total) continue;
+            if (entry[q] >= 0) {
+                if constexpr (VEC == 1) {                                 // one pair
+                    const float c = cosines[entry[q]], s = sines[entry[q]], x = a[q].get(0), y = b[q].get(0);
+                    a[q].set1(x * c - y * s), b[q].set1(y * c + x * s);
+                } else if constexpr (NEIGHBOURS) {                         // VEC / 2 pairs
+                    typedef __attribute__((ext_vector_type(VEC / 2))) float C;
+                    const C c = *(const C *)(cosines + entry[q]), s = *(const C *)(sines + entry[q]);
 #pragma unroll
-            for (int j = 0; j < VEC / 4; ++j) {
-                c[j] = *(const C *)(cosines + t * p.pairs + unit * VEC + 4 * j);
-                s[j] = *(const C *)(sines + t * p.pairs + unit * VEC + 4 * j);
-            }
-            Piece<F32, VEC> a, b;
-            a.load(src + unit * VEC), b.load(src + unit * VEC + p.pairs);
+                    for (int j = 0; j < VEC / 2; ++j) {
+                        const float x = a[q].get(2 * j), y = a[q].get(2 * j + 1);
+                        a[q].set(2 * j, x * c[j] - y * s[j], y * c[j] + x * s[j]);
+                    }
+                } else {                                                  // VEC pairs
+                    typedef __attribute__((ext_vector_type(4))) float C;   // (four at a time: the table is 16-byte aligned)
+                    C c[VEC / 4], s[VEC / 4];
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-                const float x0 = a.get(j), x1 = a.get(j + 1), y0 = b.get(j), y1 = b.get(j + 1);
-                const float c0 = c[j / 4][j % 4], c1 = c[j / 4][j % 4 + 1], s0 = s[j / 4][j % 4], s1 = s[j / 4][j % 4 + 1];
-                a.set(j, x0 * c0 - y0 * s0, x1 * c1 - y1 * s1);
-                b.set(j, y0 * c0 + x0 * s0, y1 * c1 + x1 * s1);
+                    for (int j = 0; j < VEC / 4; ++j) {
+                        c[j] = *(const C *)(cosines + entry[q] + 4 * j);
+                        s[j] = *(const C *)(sines + entry[q] + 4 * j);
+                    }
+#pragma unroll
+                    for (int j = 0; j < VEC; j += 2) {
+                        const float x0 = a[q].get(j), x1 = a[q].get(j + 1), y0 = b[q].get(j), y1 = b[q].get(j + 1);
+                        const float c0 = c[j / 4][j % 4], c1 = c[j / 4][j % 4 + 1], s0 = s[j / 4][j % 4], s1 = s[j / 4][j % 4 + 1];
+                        a[q].set(j, x0 * c0 - y0 * s0, x1 * c1 - y1 * s1);
+                        b[q].set(j, y0 * c0 + x0 * s0, y1 * c1 + x1 * s1);
+                    }
+                }
+                if (TWO) b[q].store(dst[q] + second[q]);
             }
-            a.store(dst + unit * VEC), b.store(dst + unit * VEC + p.pairs);
+            a[q].store(dst[q] + first[q]);
         }
     }
 }
@@ -142,15 +153,23 @@ int launch(const onedc_rotary_params *p, void *stream) {
     // tokens a workgroup: up to 2048 units (8 a thread), fewer where that leaves under two workgroups a CU
     const int64_t rows = (int64_t)p->B * p->N;
     const int heads = p->qh + p->kh;
-    int64_t T = 2048 / ((int64_t)heads * u.per) + 1, most = (rows + 511) / 512;
+    int64_t T = 2048 / ((int64_t)heads * u.per), most = (rows + 511) / 512;
     if (T > most) T = most;
     if (p->pairs && T > MAX_TABLE / p->pairs) T = MAX_TABLE / p->pairs;
     u.T = (int)(T < 1 ? 1 : T);
     u.by_unit = OnedcFastDiv(u.per), u.by_head = OnedcFastDiv(heads), u.by_pair = OnedcFastDiv(p->pairs ? p->pairs : 1);
     const dim3 grid((unsigned)((rows + u.T - 1) / u.T));
     const size_t lds = (size_t)u.T * p->pairs * 8 + 16;
-    if (p->neighbours) hipLaunchKernelGGL((rotary_kernel<F32, VEC, true>), grid, dim3(NT), lds, as_stream(stream), *p, u);
-    else hipLaunchKernelGGL((rotary_kernel<F32, VEC, false>), grid, dim3(NT), lds, as_stream(stream), *p, u);
+    // four units of a thread in flight where the tensors come from memory, two where the last-level cache holds them (49152 x 32 x 80: 104 us against
+    // 110; 36864 x 16 x 80: 35.5 against 33.4)
+    const bool far = rows * heads * p->D * (F32 ? 8 : 4) > (256ll << 20);
+    const auto go = [&](auto nb, auto fly) {
+        hipLaunchKernelGGL((rotary_kernel<F32, VEC, decltype(nb)::value, decltype(fly)::value>), grid, dim3(NT), lds, as_stream(stream), *p, u);
+    };
+    typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
+    if (p->neighbours) far ? go(std::true_type(), Four()) : go(std::true_type(), Two());
+    else far ? go(std::false_type(), Four()) : go(std::false_type(), Two());
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
