@@ -7,6 +7,7 @@ There is no CPU or eager fallback: without the built library `_native.hip()` rai
 import contextlib
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -19,11 +20,15 @@ from . import _native
 # CALLING CONTEXT (thread-local): layers pack their weights and allocate their outputs in the format that is current when
 # they are built / called, and `lib()` hands out the matching library.
 DEFAULT_ACT = os.environ.get("ONEDC_ACT", "f16")
-_tls = threading.local()
+class _ThreadFormat(threading.local):
+    act = None
+
+
+_tls = _ThreadFormat()
 
 
 def act():
-    return getattr(_tls, "act", None) or DEFAULT_ACT
+    return _tls.act or DEFAULT_ACT
 
 
 def a16():
@@ -48,14 +53,23 @@ def in_own_format(method):
     return wrapper
 
 
-@contextlib.contextmanager
-def act_format(name):
-    prev = getattr(_tls, "act", None)
-    set_act(name)
-    try:
-        yield
-    finally:
-        _tls.act = prev
+class act_format(contextlib.ContextDecorator):
+    """The 16-bit format `name` for a block of code (or, as a decorator, for the calls of a function), in this thread."""
+    __slots__ = ("name", "prev")
+
+    def __init__(self, name):
+        self.name = name
+
+    def __enter__(self):
+        self.prev = _tls.act
+        set_act(self.name)
+
+    def __exit__(self, *exc):
+        _tls.act = self.prev
+
+    def _recreate_cm(self):
+        return act_format(self.name)
+
 
 EPI_LINEAR, EPI_LEAKY, EPI_SILU, EPI_GLU_LEAKY, EPI_GEGLU = range(5)
 
@@ -205,7 +219,7 @@ ABI_VERSION = 5        # ONEDC_HIP_ABI_VERSION of include/onedc_hip.h this bindi
 
 
 def lib(fmt=None):
-    fmt = fmt or act()
+    fmt = fmt or _tls.act or DEFAULT_ACT
     l = _libs.get(fmt)
     if l is None:
         l = attach_signatures(_native.hip(fmt))
@@ -769,20 +783,35 @@ def add(a, b, y):
 NORM_LAYER, NORM_RMS = 0, 1
 
 
+def _filler(cls):
+    """cls(*values) for all its fields at once, addresses as numbers: a third of the constructor's time."""
+    pack = struct.Struct("".join({_P: "P", _L: "q", C.c_int32: "i", _F: "f"}[t] for _, t in cls._fields_) + "0P").pack
+    make = cls.from_buffer_copy
+    return lambda *values: make(pack(*values))
+
+
+_block_norm_params, _block_norm_grad, _rotary_params, _mxfp4_params = map(_filler, (BlockNormParams, BlockNormGrad, RotaryParams, MxFp4Params))
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _span(what, name, v, n, channels, dtypes):
     """Checks a View of n rows against its buffer and what the call needs of it (`channels` wide or None, one of `dtypes`) and returns where it
     lies: (first byte, end, bytes between rows, bytes of a row, buffer)."""
     t, cs, co, c = v.t, v.cs, v.co, v.C
+    dtype = t.dtype
     if v.B * v.H * v.W != n:
         raise KernelError(f"{what}: {name} has {v.B * v.H * v.W} rows, not {n}")
-    if c < 1 or co < 0 or co + c > cs or not t.is_contiguous() or (n and (n - 1) * cs + co + c > t.numel()):
+    if c < 1 or co < 0 or co + c > cs or cs > 0x7fffffff or not t.is_contiguous() or (n and (n - 1) * cs + co + c > t.numel()):
         raise KernelError(f"{what}: {name} is a view outside its buffer ({n} rows, channels {co}..{co + c} of {cs}, {t.numel()} values"
                           f"{'' if t.is_contiguous() else ', not contiguous'})")
     if channels is not None and c != channels:
         raise KernelError(f"{what}: {name} has {c} channels, not {channels}")
-    if t.dtype not in dtypes:
-        raise KernelError(f"{what}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)} (current format: {act()})")
-    es = 4 if t.dtype == torch.float32 else 2
+    if dtype not in dtypes:
+        raise KernelError(f"{what}: {name} is {dtype}, not {' or '.join(str(d) for d in dtypes)} (current format: {act()})")
+    es = 4 if dtype is torch.float32 else 2
     base = t.data_ptr()
     lo = base + co * es
     return lo, (lo + ((n - 1) * cs + c) * es if n else lo), cs * es, c * es, base
@@ -795,14 +824,11 @@ def _check_pictures(what, name, v, like):
 
 def _check_device(what, tensors):
     """Every tensor on the device whose current stream the launch goes to."""
-    here = None
+    here = torch.cuda.current_device() if tensors[0].is_cuda else None
     for t in tensors:
-        if t is not None:
-            if here is None and t.is_cuda:
-                here = torch.cuda.current_device()
-            if t.get_device() != here:
-                raise KernelError(f"{what}: a tensor is on {t.device}, the launch goes to {'no GPU' if here is None else f'cuda:{here}'} "
-                                  "(torch.cuda.device selects it)")
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the launch goes to {'no GPU' if here is None else f'cuda:{here}'} "
+                              "(torch.cuda.device selects it)")
 
 
 def _check_apart(what, name, out, others):
@@ -888,10 +914,11 @@ def block_norm(x, y=None, *, f=None, xo=None, kind=NORM_LAYER, eps=1e-5, post=Fa
         _check_apart(what, "y", sy, (sx, sf, so))
     _check_device(what, (x.t, None if f is None else f.t, None if xo is None else xo.t, None if y is None else y.t, post_w, post_b, gate, w, b,
                          scale, shift))
-    p = BlockNormParams(sx[4], sf and sf[4], so and so[4], sy and sy[4], _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale),
-                        _ptr(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, xo.cs if so else 0, xo.co if so else 0,
-                        y.cs if sy else 0, y.co if sy else 0, gate_rs, scale_rs, shift_rs, kind, int(bool(post)), int(x.t.dtype == torch.float32),
-                        int((f or y).t.dtype == torch.float32), alpha, eps)
+    p = _block_norm_params(sx[4], sf[4] if sf else 0, so[4] if so else 0, sy[4] if sy else 0, _address(post_w), _address(post_b), _address(gate),
+                           _address(w), _address(b), _address(scale), _address(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0,
+                           f.co if sf else 0, xo.cs if so else 0, xo.co if so else 0, y.cs if sy else 0, y.co if sy else 0, gate_rs, scale_rs,
+                           shift_rs, kind, 1 if post else 0, 1 if x.t.dtype is torch.float32 else 0, 1 if (f or y).t.dtype is torch.float32 else 0,
+                           alpha, eps)
     _ok(lib().onedc_block_norm(C.byref(p), stream()), "onedc_block_norm")
     return xo, y
 
@@ -934,17 +961,20 @@ def block_norm_backward(x, dy, dx=None, *, dxo=None, f=None, df=None, kind=NORM_
     _check_device(what, [v.t for v in (x, f, dy, dxo, dx, df) if v is not None] +
                   [post_w, post_b, gate, w, b, scale, shift, d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift])
     side = f or dy
-    p = BlockNormParams(sx[4], sf and sf[4], None, None, _ptr(post_w), _ptr(post_b), _ptr(gate), _ptr(w), _ptr(b), _ptr(scale), _ptr(shift), x.B,
-                        x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, 0, 0, 0, 0, gate_rs, scale_rs, shift_rs, kind,
-                        int(bool(post)), int(x.t.dtype == torch.float32), int(side is not None and side.t.dtype == torch.float32), alpha, eps)
-    g = BlockNormGrad(sy and sy[4], so and so[4], sdx and sdx[4], sdf and sdf[4], _ptr(d_post_w), _ptr(d_post_b), _ptr(d_gate), _ptr(d_w),
-                      _ptr(d_b), _ptr(d_scale), _ptr(d_shift), None, 0, dy.cs if sy else 0, dy.co if sy else 0, dxo.cs if so else 0,
-                      dxo.co if so else 0, dx.cs if sdx else 0, dx.co if sdx else 0, df.cs if sdf else 0, df.co if sdf else 0)
-    need = lib().onedc_block_norm_backward_ws_bytes(C.byref(p), C.byref(g))
+    p = _block_norm_params(sx[4], sf[4] if sf else 0, 0, 0, _address(post_w), _address(post_b), _address(gate), _address(w), _address(b),
+                           _address(scale), _address(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, 0, 0, 0, 0,
+                           gate_rs, scale_rs, shift_rs, kind, 1 if post else 0, 1 if x.t.dtype is torch.float32 else 0,
+                           1 if side is not None and side.t.dtype is torch.float32 else 0, alpha, eps)
+    g = _block_norm_grad(sy[4] if sy else 0, so[4] if so else 0, sdx[4] if sdx else 0, sdf[4] if sdf else 0, _address(d_post_w),
+                         _address(d_post_b), _address(d_gate), _address(d_w), _address(d_b), _address(d_scale), _address(d_shift), 0, 0,
+                         dy.cs if sy else 0, dy.co if sy else 0, dxo.cs if so else 0, dxo.co if so else 0, dx.cs if sdx else 0,
+                         dx.co if sdx else 0, df.cs if sdf else 0, df.co if sdf else 0)
+    native, at_p, at_g = lib(), C.byref(p), C.byref(g)
+    need = native.onedc_block_norm_backward_ws_bytes(at_p, at_g)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=x.t.device)          # the call's own: two captured graphs never share it
         g.ws, g.ws_bytes = ws.data_ptr(), need
-    _ok(lib().onedc_block_norm_backward(C.byref(p), C.byref(g), stream()), "onedc_block_norm_backward")
+    _ok(native.onedc_block_norm_backward(at_p, at_g, stream()), "onedc_block_norm_backward")
     return dx, df
 
 
@@ -1014,10 +1044,10 @@ def rotary_axes(plan, pos, q, qo=None, k=None, ko=None, inverse=False):
     _check_device(what, (q.t, qo.t, None if k is None else k.t, None if k is None else ko.t, pos, plan.turns, plan.axis))
     if not n:
         return qo, ko
-    p = RotaryParams(sq[4], sqo[4], sk and sk[4], sko and sko[4], pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), q.B, N, D, plan.pairs,
-                     plan.axes, qh, kh, q.cs, q.co, qo.cs, qo.co, k.cs if kh else 0, k.co if kh else 0, ko.cs if kh else 0, ko.co if kh else 0,
-                     int(q.t.dtype == torch.float32), int(pos.dtype == torch.float32), int(plan.neighbours), int(bool(inverse)),
-                     N * plan.axes if len(shape) == 3 and shape[0] > 1 else 0)
+    p = _rotary_params(sq[4], sqo[4], sk[4] if sk else 0, sko[4] if sko else 0, pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), q.B, N,
+                       D, plan.pairs, plan.axes, qh, kh, q.cs, q.co, qo.cs, qo.co, k.cs if kh else 0, k.co if kh else 0, ko.cs if kh else 0,
+                       ko.co if kh else 0, 1 if dtype[0] is torch.float32 else 0, 1 if pos.dtype is torch.float32 else 0,
+                       1 if plan.neighbours else 0, 1 if inverse else 0, N * plan.axes if len(shape) == 3 and shape[0] > 1 else 0)
     _ok(lib().onedc_rotary_axes(C.byref(p), stream()), "onedc_rotary_axes")
     return qo, ko
 
@@ -1107,11 +1137,20 @@ def mxfp4_linear(x, w, bias, y, *, epi=EPI_LINEAR, slope=0.01, alpha=1.0, res=No
     _check_device(what, (x.codes if held else x.t, x.scales if held else None, w.codes, w.scales, y.t, bias, None if res is None else res.t))
     if not rows:
         return y
-    if not held and rows > MXFP4_ROWS_RAW:
-        x, held = mxfp4_quantize(x), True
-    p = MxFp4Params(x.codes.data_ptr() if held else None, x.scales.data_ptr() if held else None, None if held else sx[4], w.codes.data_ptr(),
-                    w.scales.data_ptr(), _ptr(bias), sr and sr[4], sy[4], rows, w.rows, w.K, 0 if held else x.cs, 0 if held else x.co,
-                    int(not held and x.t.dtype == f32), y.cs, y.co, res.cs if sr else 0, res.co if sr else 0, int(y.t.dtype == f32), epi, alpha,
-                    slope)
-    _ok(lib().onedc_mxfp4_linear(C.byref(p), stream()), "onedc_mxfp4_linear")
+    native, codes, scales, raw, x32 = lib(), 0, 0, 0, 0
+    if held:
+        codes, scales = x.codes.data_ptr(), x.scales.data_ptr()
+    else:
+        raw, x32 = sx[4], 1 if x.t.dtype is f32 else 0
+        if rows > MXFP4_ROWS_RAW:                     # codes and scales in a buffer of the call's own
+            part = rows * ((kx + 127) // 128) * 64
+            ws = torch.empty(part + part // 16, dtype=torch.uint8, device=x.t.device)
+            codes = ws.data_ptr()
+            scales = codes + part
+            _ok(native.onedc_mxfp4_quantize(raw, x32, x.cs, x.co, codes, scales, rows, kx, stream()), "onedc_mxfp4_quantize")
+            raw = 0
+    p = _mxfp4_params(codes, scales, raw, w.codes.data_ptr(), w.scales.data_ptr(), _address(bias), sr[4] if sr else 0, sy[4], rows, w.rows, kx,
+                      x.cs if raw else 0, x.co if raw else 0, x32, y.cs, y.co, res.cs if sr else 0, res.co if sr else 0,
+                      1 if y.t.dtype is f32 else 0, epi, alpha, slope)
+    _ok(native.onedc_mxfp4_linear(C.byref(p), stream()), "onedc_mxfp4_linear")
     return y
