@@ -446,8 +446,9 @@ int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y
                            void *stream);
 /* Product of two such matrices along K with the epilogues of onedc_conv_gemm:
  *   y[m][n] = act(alpha * sum_k x[m][k] w[n][k] + bias[n]) + res[m][n]
- * products exact, sums in f32, one rounding to y's type (16-bit or y_f32).  epi: ONEDC_EPI_LINEAR, _LEAKY (slope), _SILU, or _GEGLU,
- * where rows of w come in blocks of 16, values in front of their gates, N % 32 == 0, y and res have N / 2 channels.  res has y's type.
+ * products exact, sums in f32 (in an order that follows M, N and K), one rounding to y's type (16-bit or y_f32).  epi: ONEDC_EPI_LINEAR,
+ * _LEAKY (slope), _SILU, or _GEGLU, where rows of w come in blocks of 16, values in front of their gates, N % 32 == 0, y and res have
+ * N / 2 channels.  res has y's type and may be y.
  * x: either (xc, xs) as above, or, xc NULL, raw rows xr (16-bit or xr_f32, stride xr_cs, offset xr_co) that are quantised on the way:
  * only for M <= ONEDC_MXFP4_ROWS_RAW, without scratch.  M may be 0.
  * Returns -1 for a missing pointer, -2 for sizes, strides or alignment, -3 for an epilogue it does not know or a GEGLU layer with

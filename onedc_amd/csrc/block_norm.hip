@@ -24,6 +24,10 @@ constexpr int NT = 256;
 //   A = alpha gate post_w, Ab = alpha gate post_b (join);  W = w (1 + scale), S = b (1 + scale) + shift (norm behind it)
 // into LDS where several rows of a wave share them, into registers where a thread owns its channels.  The next row's loads are in
 // flight while a row is computed.
+// 16-bit, gated, modulated, norms on both sides: 16 x 9216 x 320 in 83 us (4.6 TB/s of 5.15 that a large copy reaches), 16 x 2304 x 640 34 us (5.5),
+// 16 x 576 x 1280 22 us (4.4), 16 x 2304 x 643 36 us (5.3), 16 x 576 x 4096 69 us (4.4); with every gradient backward 130 us (4.4), 64 us (4.4),
+// 48 us (2.9), 78 us (3.6), 113 us (4.0), of which the sums over the rows are 7 to 11.
+// Outputs stored past the cache take the first to 62 us and give it all back in whoever reads them.
 
 // sum over the L neighbouring lanes of v's row, the same bits in each of them
 template <int O>
@@ -539,7 +543,11 @@ __global__ __launch_bounds__(NTH, NTH > 256 ? 1 : IT > 1 ? 2 : 3) void block_nor
     }
 }
 
-// ---- wider rows: a workgroup passes over its row again for every sum -------------------------------------------------------------------
+// ---- wider rows, and rows of less than a piece: a workgroup passes over its row again for every sum ----------------------------------------
+// Bound by the latency of those passes, which come from the caches: 512 x 20000 in 85 us (1.0 TB/s), backward 286 us (256 threads a row instead
+// of 1024: 212 and 494); a million rows of four channels 676 us, backward 1.3 ms.
+constexpr int NTW = 1024;
+int simple_threads(int C) { return C < 8 ? 64 : NTW; }
 
 // sum of v over the workgroup, the same value in every thread
 __device__ __forceinline__ float block_sum(float v, float *red) {
@@ -549,8 +557,7 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) s += red[i];
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += red[i];
     return s;
 }
 
@@ -560,11 +567,11 @@ __device__ __forceinline__ float2 row_norm(V v, int C, int kind, float eps, floa
     float m = 0.f;
     if (kind == ONEDC_NORM_LAYER) {
         float s = 0.f;
-        for (int c = threadIdx.x; c < C; c += NT) s += v(c);
+        for (int c = threadIdx.x; c < C; c += blockDim.x) s += v(c);
         m = block_sum(s, red) / C;
     }
     float q = 0.f;
-    for (int c = threadIdx.x; c < C; c += NT) {
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
         const float d = v(c) - m;
         q += d * d;
     }
@@ -572,48 +579,49 @@ __device__ __forceinline__ float2 row_norm(V v, int C, int kind, float eps, floa
 }
 
 template <bool X32, bool F32>
-__global__ __launch_bounds__(NT) void block_norm_kernel(onedc_block_norm_params p) {
+__global__ __launch_bounds__(NTW) void block_norm_kernel(onedc_block_norm_params p) {
     typedef Elem<X32> X;
     typedef Elem<F32> F;
-    __shared__ float red[NT / 64];
-    const int64_t row = blockIdx.x;
-    const int64_t b = row / p.N;
-    const typename X::T *x = (const typename X::T *)p.x + row * p.x_cs + p.x_co;
-    const typename F::T *f = p.f ? (const typename F::T *)p.f + row * p.f_cs + p.f_co : nullptr;
-    const float *gate = p.gate ? p.gate + b * p.gate_rs : nullptr;
-    float2 fn = make_float2(0.f, 1.f);
-    if (p.post) fn = row_norm([&](int c) { return F::get(f + c); }, p.C, p.kind, p.eps, red);
-    auto joined = [&](int c) {
-        float t = X::get(x + c);
-        if (f) {
-            const float v = (F::get(f + c) - fn.x) * fn.y * at(p.post_w, c, 1.f) + at(p.post_b, c, 0.f);
-            t = __builtin_fmaf(p.alpha * at(gate, c, 1.f), v, t);
+    __shared__ float red[NTW / 64];
+    for (int64_t row = blockIdx.x; row < (int64_t)p.B * p.N; row += gridDim.x) {
+        const int64_t b = row / p.N;
+        const typename X::T *x = (const typename X::T *)p.x + row * p.x_cs + p.x_co;
+        const typename F::T *f = p.f ? (const typename F::T *)p.f + row * p.f_cs + p.f_co : nullptr;
+        const float *gate = p.gate ? p.gate + b * p.gate_rs : nullptr;
+        float2 fn = make_float2(0.f, 1.f);
+        if (p.post) fn = row_norm([&](int c) { return F::get(f + c); }, p.C, p.kind, p.eps, red);
+        auto joined = [&](int c) {
+            float t = X::get(x + c);
+            if (f) {
+                const float v = (F::get(f + c) - fn.x) * fn.y * at(p.post_w, c, 1.f) + at(p.post_b, c, 0.f);
+                t = __builtin_fmaf(p.alpha * at(gate, c, 1.f), v, t);
+            }
+            return t;
+        };
+        if (p.y) {
+            const float2 tn = row_norm(joined, p.C, p.kind, p.eps, red);
+            const float *scale = p.scale ? p.scale + b * p.scale_rs : nullptr, *shift = p.shift ? p.shift + b * p.shift_rs : nullptr;
+            typename F::T *y = (typename F::T *)p.y + row * p.y_cs + p.y_co;
+            for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
+                const float v = (joined(c) - tn.x) * tn.y * at(p.w, c, 1.f) + at(p.b, c, 0.f);
+                F::put(y + c, __builtin_fmaf(v, 1.f + at(scale, c, 0.f), at(shift, c, 0.f)));
+            }
         }
-        return t;
-    };
-    if (p.y) {
-        const float2 tn = row_norm(joined, p.C, p.kind, p.eps, red);
-        const float *scale = p.scale ? p.scale + b * p.scale_rs : nullptr, *shift = p.shift ? p.shift + b * p.shift_rs : nullptr;
-        typename F::T *y = (typename F::T *)p.y + row * p.y_cs + p.y_co;
-        for (int c = threadIdx.x; c < p.C; c += NT) {
-            const float v = (joined(c) - tn.x) * tn.y * at(p.w, c, 1.f) + at(p.b, c, 0.f);
-            F::put(y + c, __builtin_fmaf(v, 1.f + at(scale, c, 0.f), at(shift, c, 0.f)));
+        if (p.xo) {                                      // (behind the norm's passes: xo may be x)
+            typename X::T *xo = (typename X::T *)p.xo + row * p.xo_cs + p.xo_co;
+            for (int c = threadIdx.x; c < p.C; c += blockDim.x) X::put(xo + c, joined(c));
         }
-    }
-    if (p.xo) {                                      // (behind the norm's passes: xo may be x)
-        typename X::T *xo = (typename X::T *)p.xo + row * p.xo_cs + p.xo_co;
-        for (int c = threadIdx.x; c < p.C; c += NT) X::put(xo + c, joined(c));
     }
 }
 
 // dx and df of a row, and the row's four column terms added to this run's sums: sums[4][C rounded up to 8] in memory, one column
 // owned by one thread for the whole run (fixed order)
 template <bool X32, bool F32>
-__global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, float *part,
+__global__ __launch_bounds__(NTW) void block_norm_backward_kernel(onedc_block_norm_params p, onedc_block_norm_grad g, float *part,
                                                                  int runs, int run_rows) {
     typedef Elem<X32> X;
     typedef Elem<F32> F;
-    __shared__ float red[NT / 64];
+    __shared__ float red[NTW / 64];
     const int b = blockIdx.x / runs, run = blockIdx.x - b * runs;
     const int n0 = run * run_rows, n1 = min(p.N, n0 + run_rows);
     const float *gate = p.gate ? p.gate + (int64_t)b * p.gate_rs : nullptr;
@@ -621,7 +629,7 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
     const int C8 = (p.C + 7) & ~7;
     float *sums = part ? part + (int64_t)blockIdx.x * 4 * C8 : nullptr;
     if (sums)
-        for (int c = threadIdx.x; c < 4 * C8; c += NT) sums[c] = 0.f;      // (a thread's own columns differ from these: barrier below)
+        for (int c = threadIdx.x; c < 4 * C8; c += blockDim.x) sums[c] = 0.f;      // (a thread's own columns differ from these: barrier below)
     __syncthreads();
     for (int n = n0; n < n1; ++n) {
         const int64_t row = (int64_t)b * p.N + n;
@@ -636,7 +644,7 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
         if (dy) {
             tn = row_norm([&](int c) { return X::get(t + c); }, p.C, p.kind, p.eps, red);
             float su = 0.f, sh = 0.f;
-            for (int c = threadIdx.x; c < p.C; c += NT) {
+            for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
                 const float v = u(c);
                 su += v;
                 sh += v * hat(c);
@@ -655,7 +663,7 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
         if (p.post) {
             fn = row_norm([&](int c) { return F::get(f + c); }, p.C, p.kind, p.eps, red);
             float sw = 0.f, sf = 0.f;
-            for (int c = threadIdx.x; c < p.C; c += NT) {
+            for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
                 const float v = w(c);
                 sw += v;
                 sf += v * fhat(c);
@@ -663,7 +671,7 @@ __global__ __launch_bounds__(NT) void block_norm_backward_kernel(onedc_block_nor
             mw = p.kind == ONEDC_NORM_LAYER ? block_sum(sw, red) / p.C : 0.f;
             mf = block_sum(sf, red) / p.C;
         }
-        for (int c = threadIdx.x; c < p.C; c += NT) {
+        for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
             const float d = dt(c), fh = f ? fhat(c) : 0.f;
             if (sums) {
                 const float e = dy ? F::get(dy + c) : 0.f;
@@ -844,7 +852,7 @@ constexpr int SIMPLE_RUNS = 512;
 bool backward_plan(const onedc_block_norm_params &p, bool sums, Shape *s, Plan *pl) {
     *s = row_shape(p.C, WIDEST_BACK, true, &pl->L);
     if (!s->it) {
-        cut_runs(p, 1, SIMPLE_RUNS, pl);
+        cut_runs(p, 1, p.C < 8 ? 32 * SIMPLE_RUNS : SIMPLE_RUNS, pl);
         return false;
     }
     const int each = s->threads / pl->L;
@@ -928,11 +936,11 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
         return 0;
     }
     if (p->f_f32)
-        hipLaunchKernelGGL((block_norm_kernel<true, true>), dim3((unsigned)rows), dim3(NT), 0, as_stream(stream), *p);
+        hipLaunchKernelGGL((block_norm_kernel<true, true>), dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(simple_threads(p->C)), 0, as_stream(stream), *p);
     else if (p->x_f32)
-        hipLaunchKernelGGL((block_norm_kernel<true, false>), dim3((unsigned)rows), dim3(NT), 0, as_stream(stream), *p);
+        hipLaunchKernelGGL((block_norm_kernel<true, false>), dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(simple_threads(p->C)), 0, as_stream(stream), *p);
     else
-        hipLaunchKernelGGL((block_norm_kernel<false, false>), dim3((unsigned)rows), dim3(NT), 0, as_stream(stream), *p);
+        hipLaunchKernelGGL((block_norm_kernel<false, false>), dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(simple_threads(p->C)), 0, as_stream(stream), *p);
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
@@ -999,11 +1007,11 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
                 hipLaunchKernelGGL((block_norm_rows_backward_kernel<NTH, SH, IT, X, F, TL, OPT>), grid, dim3(NTH), lds, as_stream(stream), q, *g, pl, part);
         });
     } else if (p->f_f32) {
-        hipLaunchKernelGGL((block_norm_backward_kernel<true, true>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+        hipLaunchKernelGGL((block_norm_backward_kernel<true, true>), grid, dim3(simple_threads(p->C)), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
     } else if (p->x_f32) {
-        hipLaunchKernelGGL((block_norm_backward_kernel<true, false>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+        hipLaunchKernelGGL((block_norm_backward_kernel<true, false>), grid, dim3(simple_threads(p->C)), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
     } else {
-        hipLaunchKernelGGL((block_norm_backward_kernel<false, false>), grid, dim3(NT), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
+        hipLaunchKernelGGL((block_norm_backward_kernel<false, false>), grid, dim3(simple_threads(p->C)), 0, as_stream(stream), q, *g, part, pl.runs, pl.run_rows);
     }
     ONEDC_LAUNCH_CHECK();
     if (sums) {

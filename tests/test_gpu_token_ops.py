@@ -170,6 +170,8 @@ CASES = [
     (1, 5, 2500, "layer", False, "one", None, True, 1.0),
     (1, 2, 5001, "rms", True, "each", "each", True, 1.0),
     (70000, 1, 8, "layer", False, "each", "each", False, 1.0),
+    (1, 70000, 3, "layer", False, "one", None, True, 1.0),
+    (2, 40, 7, "rms", True, "each", "each", True, 1.0),
 ]
 
 
