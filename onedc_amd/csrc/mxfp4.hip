@@ -362,7 +362,7 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, 
 // 16384 x 8192 x 8192, 256 x 256: 550 - 572 us, 3.8 - 4.0 PFLOP/s.  Without the DMA it takes 465, without the LDS reads 524, without both
 // 373, without the stores 507, the products alone 337: the feeding and the power limit bound it together.  Stages of one step in rings of
 // three and four, 2 x 4 waves, other spacings of the DMA and outputs stored from registers (605 us) gained nothing.  4096^3 40 us, 3.4 PFLOP/s;
-// 8655 x 10240 x 1280 gated 98 - 102 us, 2.2 PFLOP/s: ten steps a tile, its GELU costs as much as its products.
+// 8655 x 10240 x 1280 gated 96 - 115 us, 2.0 - 2.3 PFLOP/s: ten steps a tile, its GELU costs as much as its products.
 #define MX_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -715,12 +715,15 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     //   64 x 64, three stages, while they fit the CUs' first four each (2048 x 1280 x 5120: 17 us against 19; 4096 x 1280 x 5120: 28 against 26)
     //   128 x 128: one stage and three workgroups a CU that load and multiply in turn; two stages where there are less than two a CU
     //     (4096 x 1280 x 5120: 26 us against 28; 8192 x 4096 x 5120: 112 against 110)
+    //   128 x 256, four waves, one stage, two workgroups a CU: gated layers of very many tiles, whose epilogue weighs most (8655 x 10240 x 1280: 115.5 us
+    //     against 120, 36864 x 5120 x 640: 171.5 against 175; linear 36864 x 640 x 640 28 against 25)
     const auto tiles = [&](int64_t t) { return ((p->N + t - 1) / t) * ((p->M + t - 1) / t); };
     const bool gated = p->epi == ONEDC_EPI_GEGLU;
     if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 2, 1>(p, steps, whole, stream);
     if (tiles(64) <= 256 && steps >= 32) return launch_tiles<2, 2, 1, 1, 2, 3, 2, 2>(p, steps, whole, stream);
     if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 2, 3, 4, 1>(p, steps, whole, stream);
     if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 2, 1>(p, steps, whole, stream);
+    if (gated && tiles(128) > 2048) return launch_tiles<2, 2, 2, 4, 2, 1, 2, 1>(p, steps, whole, stream);
     return launch_tiles<2, 2, 2, 2, 2, 1, 3, 1>(p, steps, whole, stream);
 }
 

@@ -752,6 +752,7 @@ def test_mxfp4_linear(M, N, k, epi, bias, res, fmt):
 @pytest.mark.parametrize("M,N,k,epi,res", [
     (2100, 2100, 520, "linear", True),         # 128 x 128, two stages; an odd number of steps
     (4200, 2624, 260, "geglu", False),         # 128 x 128, one stage
+    (6001, 5664, 300, "geglu", True),          # 128 x 256
     (2600, 4200, 200, "silu", True),           # 256 x 256; two steps, ragged both ways
     (2600, 4224, 4500, "geglu", True),         # 256 x 256, gated; 36 steps
     (2601, 4195, 1150, "leaky", False),        # 256 x 256, nothing aligned; nine steps: a group of scales with one step
