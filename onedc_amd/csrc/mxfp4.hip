@@ -352,8 +352,8 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, 
 }
 
 // ---- tiles: the matrix cores and what feeds them bound it ---------------------------------------------------------------------------------
-// A workgroup of WN x WM waves computes 32 WN FN weight rows x 32 WM FM activation rows.  A stage is KS steps of 128 values of both operands,
-// LDS-DMA'd into a ring of NST: rows of 64 KS bytes whose 16-byte chunks are permuted so that the rows that a fragment read touches
+// A workgroup of WN x WM waves computes 32 WN FN weight rows x 32 WM FM activation rows.  A stage is two steps of 128 values of both operands,
+// LDS-DMA'd into a ring of NST: rows of 128 bytes whose 16-byte chunks are permuted so that the rows that a fragment read touches
 // together lie on different banks.  Scales come eight steps (32 bytes a row) at a time; byte permutes collect a lane's scales into the
 // words that the matrix instruction picks from.
 // The DMA is written as instructions (it has no destination register): behind the builtin the compiler drains every DMA in flight
@@ -378,12 +378,14 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned voff, unsigned soff, 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff));
 }
 
+constexpr int KS = 2, ROW = 64 * KS;               // steps of a stage, bytes of its rows
+
 // WN x WM waves of FN x FM blocks of 32 x 32; KG such teams share the tile, each with a ring of its own and a part of K, and the first adds their
 // sums in order
-template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC, int KG>
+template <int WN, int WM, int FN, int FM, int NST, int OCC, int KG>
 __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp4_params p, int steps, int tiles_n, int tiles_m, int whole) {
-    constexpr int NW = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, ROW = 64 * KS, STAGE = (TN + TM) * ROW;
-    constexpr int RI = 16 / KS;                      // rows of a DMA instruction
+    constexpr int NW = WN * WM, TN = 32 * WN * FN, TM = 32 * WM * FM, STAGE = (TN + TM) * ROW;
+    constexpr int RI = 1024 / ROW;                   // rows of a DMA instruction
     constexpr int IN = TN / RI / NW, IM = TM / RI / NW, NI = IN + IM;
     constexpr int GROUP = (TN + TM) * 32, NSC = ((TN + TM) / 32 + NW - 1) / NW, RING = NST * STAGE;     // scales of eight steps, behind the ring
     constexpr int GS = 8 / KS;                       // stages of a group of scales
@@ -406,8 +408,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp
     const unsigned row_bytes = (unsigned)steps * 64;
     const i32x4 w_rsrc = raw_rsrc((const char *)p.wc + (int64_t)n0 * row_bytes, (int64_t)(p.N - n0) * row_bytes);
     const i32x4 x_rsrc = raw_rsrc((const char *)p.xc + m0 * row_bytes, (p.M - m0) * (int64_t)row_bytes);
-    const int srow = wave * RI + lane / (4 * KS);
-    const int schunk = KS == 2 ? (lane & 7) ^ (srow & 7) : (lane & 3) ^ ((srow >> 1) & 3);
+    const int srow = wave * RI + (lane >> 3), schunk = (lane & 7) ^ (srow & 7);
     const unsigned voff = (unsigned)srow * row_bytes + (unsigned)schunk * 16;
     unsigned wv[IN], xv[IM];
 #pragma unroll
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp
     // every stage issues the same number, and the products need no branch.
     auto stage_one = [&](int d, int t, int slot) {
         const unsigned dst = lds0 + slot * STAGE + wave * 1024;
-        const unsigned behind = t * KS + (KS == 2 && schunk >= 4 ? 1 : 0) >= steps ? 0xffff0000u : 0u;
+        const unsigned behind = t * KS + (schunk >> 2) >= steps ? 0xffff0000u : 0u;
         const unsigned soff = t * KS < steps ? (unsigned)t * ROW : 0u;           // (never past the descriptor's end: it is taken off that)
         if (d < IN) dma16(w_rsrc, wv[d < IN ? d : 0] | behind, soff, dst + d * NW * 1024);
         else dma16(x_rsrc, xv[d < IN ? 0 : d - IN] | behind, soff, dst + TN * ROW + (d - IN) * NW * 1024);
@@ -472,7 +473,7 @@ __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp
         for (int j = 0; j < FM; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    const int swap = KS == 2 ? r & 7 : (r >> 1) & 3;
+    const int swap = r & 7;
 
     // a team's groups of scales, and where they begin; every team makes the same turns (those behind the last step multiply zeros)
     const int groups = (((steps + 7) >> 3) + KG - 1) / KG, g0 = team * groups, stages = min(g0 * GS + (steps + KS - 1) / KS, (g0 + groups) * GS);
@@ -534,12 +535,6 @@ __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp
         if (t + 1 < stages) go(std::integral_constant<int, 1>(), t + 1);
         if (t + 2 < stages) go(std::integral_constant<int, 2>(), t + 2);
         if (t + 3 < stages) go(std::integral_constant<int, 3>(), t + 3);
-        if constexpr (GS == 8) {
-            if (t + 4 < stages) go(std::integral_constant<int, 4>(), t + 4);
-            if (t + 5 < stages) go(std::integral_constant<int, 5>(), t + 5);
-            if (t + 6 < stages) go(std::integral_constant<int, 6>(), t + 6);
-            if (t + 7 < stages) go(std::integral_constant<int, 7>(), t + 7);
-        }
     }
     MX_VMCNT(0);
     __syncthreads();                                 // the rings are free: the waves' own scratch from here
@@ -641,18 +636,18 @@ int launch_skinny(const onedc_mxfp4_params *p, int steps, int whole, void *strea
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
-template <int WN, int WM, int FN, int FM, int KS, int NST, int OCC, int KG>
+template <int WN, int WM, int FN, int FM, int NST, int OCC, int KG>
 int launch_tiles(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
     static_assert(FN == 1 || FN == 2 || FN == 4, "");
     constexpr int TN = 32 * WN * FN, TM = 32 * WM * FM;
-    constexpr int ring = KG * (TN + TM) * (NST * KS * 64 + 32), scratch = WN * WM * (32 * (FN * 32 + 4) * 4 + (KG - 1) * FN * FM * 4096);
+    constexpr int ring = KG * (TN + TM) * (NST * ROW + 32), scratch = WN * WM * (32 * (FN * 32 + 4) * 4 + (KG - 1) * FN * FM * 4096);
     constexpr int lds = ring > scratch ? ring : scratch;
     static_assert(lds <= 160 * 1024, "");
     static OnedcLdsAttrOnce once;
-    once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, KS, NST, OCC, KG>, lds}});
+    once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, NST, OCC, KG>, lds}});
     const int64_t tn = (p->N + TN - 1) / TN, tm = (p->M + TM - 1) / TM;
     if (tn * tm > 0x7fffffff) return -2;
-    hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, KS, NST, OCC, KG>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM * KG), lds, as_stream(stream), *p, steps,
+    hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, NST, OCC, KG>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM * KG), lds, as_stream(stream), *p, steps,
                        (int)tn, (int)tm, whole);
     ONEDC_LAUNCH_CHECK();
     return 0;
@@ -719,12 +714,12 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     //     against 120, 36864 x 5120 x 640: 171.5 against 175; linear 36864 x 640 x 640 28 against 25)
     const auto tiles = [&](int64_t t) { return ((p->N + t - 1) / t) * ((p->M + t - 1) / t); };
     const bool gated = p->epi == ONEDC_EPI_GEGLU;
-    if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 2, 1>(p, steps, whole, stream);
-    if (tiles(64) <= 256 && steps >= 32) return launch_tiles<2, 2, 1, 1, 2, 3, 2, 2>(p, steps, whole, stream);
-    if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 2, 3, 4, 1>(p, steps, whole, stream);
-    if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 2, 1>(p, steps, whole, stream);
-    if (gated && tiles(128) > 2048) return launch_tiles<2, 2, 2, 4, 2, 1, 2, 1>(p, steps, whole, stream);
-    return launch_tiles<2, 2, 2, 2, 2, 1, 3, 1>(p, steps, whole, stream);
+    if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 1>(p, steps, whole, stream);
+    if (tiles(64) <= 256 && steps >= 32) return launch_tiles<2, 2, 1, 1, 3, 2, 2>(p, steps, whole, stream);
+    if (tiles(64) <= 1024) return launch_tiles<2, 2, 1, 1, 3, 4, 1>(p, steps, whole, stream);
+    if (tiles(128) <= 512) return launch_tiles<2, 2, 2, 2, 2, 2, 1>(p, steps, whole, stream);
+    if (gated && tiles(128) > 2048) return launch_tiles<2, 2, 2, 4, 1, 2, 1>(p, steps, whole, stream);
+    return launch_tiles<2, 2, 2, 2, 1, 3, 1>(p, steps, whole, stream);
 }
 
 }  // extern "C"
