@@ -9,8 +9,8 @@
 // workgroup computes the sines and cosines of its T tokens once, into LDS, and all heads of those tokens read them from there (neighbouring
 // lanes hold neighbouring heads, so most of a wave's LDS reads are one address).  Pieces of 16 bytes where the sizes allow it, two or four of a
 // thread in flight.  16-bit heads: 49152 tokens x 32 x 80 in 101 us, 5.0 TB/s (a copy of 1 GB reaches 5.15; with the angles computed at every element
-// 328 us), 36864 x 16 x 80, which the last-level cache holds, 31 - 33 us, 5.8 - 6.1 TB/s; pairs of which only four share a piece (16384 x 32 x 72) 25 us,
-// 6.0 TB/s, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; one token 3.0 us in a graph, a launch's own time.
+// 328 us), 36864 x 16 x 80 40 - 44 us, or, held by the last-level cache, 31 - 33; pairs of which only four share a piece (16384 x 32 x 72, held too)
+// 25 us, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; one token 3.0 us in a graph, a launch's own time.
 #include <type_traits>
 
 #include "conv_common.h"
@@ -160,16 +160,16 @@ int launch(const onedc_rotary_params *p, void *stream) {
     u.by_unit = OnedcFastDiv(u.per), u.by_head = OnedcFastDiv(heads), u.by_pair = OnedcFastDiv(p->pairs ? p->pairs : 1);
     const dim3 grid((unsigned)((rows + u.T - 1) / u.T));
     const size_t lds = (size_t)u.T * p->pairs * 8 + 16;
-    // four units of a thread in flight where the tensors come from memory, two where the last-level cache holds them (49152 x 32 x 80: 104 us against
-    // 110; 36864 x 16 x 80: 35.5 against 33.4)
-    const bool far = rows * heads * p->D * (F32 ? 8 : 4) > (256ll << 20);
+    // four units of a thread in flight, two for small calls, whose threads have no more (tensors that no cache holds: 36864 x 16 x 80 39.6 us against
+    // 41.8, 49152 x 32 x 80 102 against 109; 8000 x 16 x 64 8.3 against 7.9)
+    const bool many = rows * heads * p->D * (F32 ? 8 : 4) > (32ll << 20);
     const auto go = [&](auto nb, auto fly) {
         hipLaunchKernelGGL((rotary_kernel<F32, VEC, decltype(nb)::value, decltype(fly)::value>), grid, dim3(NT), lds, as_stream(stream), *p, u);
     };
     typedef std::integral_constant<int, 2> Two;
     typedef std::integral_constant<int, 4> Four;
-    if (p->neighbours) far ? go(std::true_type(), Four()) : go(std::true_type(), Two());
-    else far ? go(std::false_type(), Four()) : go(std::false_type(), Two());
+    if (p->neighbours) many ? go(std::true_type(), Four()) : go(std::true_type(), Two());
+    else many ? go(std::false_type(), Four()) : go(std::false_type(), Two());
     ONEDC_LAUNCH_CHECK();
     return 0;
 }
