@@ -1,0 +1,197 @@
+"""Transformer-block operators on the GPU, at the sizes and values where a bound per element says little: norms of the error of every output
+of block_norm and its backward pass, rotary_axes as large calls run it, subnormal blocks.
+
+half_step(t) = finfo(t).eps / 2 relative to a value is one rounding to t; EPS32 = 2^-24 is half a step of f32.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from onedc_amd import kernels as K
+from onedc_amd.kernels import RotaryAxes, View
+from test_gpu_token_ops import (CASES, DEV, EPS32, F32, FORMATS, back, empty, gen, grads64, half_step, held64, in64, join64, norm64, on_gpu,
+                                options, rand, rows_view, tiny, tokens)
+
+
+@pytest.fixture(params=["f16", "bf16"])
+def fmt(request):
+    with K.act_format(request.param):
+        yield FORMATS[request.param]
+
+
+# ---- block_norm: the error of a whole output -----------------------------------------------------------------------------------------
+# A sum over a row is at most 24 additions in a lane (three pieces of eight, or 20001 / 1024 channels a thread), 6 exchanges and 16 waves: relative to
+# the sum of magnitudes 46 EPS32.  So a mean is off by 46 EPS32 mean|v|, a normalised value by 75 EPS32 (1 + top r) times its row's size (top: the
+# row's largest magnitude, r: its reciprocal deviation), and the gradient through a norm, r (u - mean u - h mean(u h)), by that twice, two such means
+# and its own roundings: SUM = 300 EPS32 (1 + top r) r |u| in the row's norm.  A parameter's gradient adds its terms' errors and those of a run of
+# rows, of which there are at least 256 where there are rows enough (N / 256 + 64 additions).
+SUM = 300 * EPS32
+
+
+def rows_norm(v):
+    return v.norm(dim=-1, keepdim=True)
+
+
+@pytest.mark.parametrize("types", ["16", "32/16", "32"])
+@pytest.mark.parametrize("case", [c for c in CASES if c[2] > 1], ids=lambda c: "-".join(str(v) for v in c))
+def test_block_norm_norms_of_the_error(case, types, fmt):
+    B, N, Cc, kind, post, gate, mod, affine, alpha = case
+    xt, ft = (F32 if types != "16" else fmt), (F32 if types == "32" else fmt)
+    g = gen(3 * Cc + N)
+    kind, eps = K.NORM_LAYER if kind == "layer" else K.NORM_RMS, 1e-3
+    a = options(g, B, Cc, kind, post, gate, mod, affine, alpha)
+    x, f = rand(g, B, N, Cc, scale=2.0, shift=0.5).to(xt), rand(g, B, N, Cc, shift=0.2).to(ft)
+    dy, dxo = rand(g, B, N, Cc).to(ft), rand(g, B, N, Cc, scale=0.5).to(xt)
+    p, wide, xo, y = on_gpu(a), in64(a), empty(B, N, Cc, xt), empty(B, N, Cc, ft)
+    K.block_norm(tokens(x), y, f=tokens(f), xo=xo, eps=eps, **p)
+    dx, df = empty(B, N, Cc, xt), empty(B, N, Cc, ft)
+    grads = {"d_" + n: torch.full(p[n].shape, 9.0, device=DEV) for n in ("post_w", "post_b", "gate", "w", "b", "scale", "shift") if n in p}
+    K.block_norm_backward(tokens(x), tokens(dy), dx, dxo=tokens(dxo), f=tokens(f), df=df, eps=eps, **p, **grads)
+
+    x, f, dy, dxo = (v.double() for v in (x, f, dy, dxo))
+    ref = grads64(x, f, dy, dxo, wide, eps)
+    ref["xo"], ref["y"] = join64(x, f, wide, eps)
+
+    def spread(v):                                       # (reciprocal deviation, 1 + largest magnitude times it) of every row
+        c = v - v.mean(-1, keepdim=True) if kind == K.NORM_LAYER else v
+        r = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+        return r, 1 + v.abs().amax(-1, keepdim=True) * r
+
+    def each(v):                                         # a parameter per picture against [B, N, C]
+        return v[:, None] if v.dim() == 2 else v
+
+    def of(name, none):
+        return each(wide[name]) if name in wide else torch.tensor(none, dtype=torch.float64)
+    (rx, lx), (rf, lf), (_, lt) = spread(x), spread(f), spread(ref["xo"])
+    pw, ga, w, sc, b = of("post_w", 1.0), alpha * of("gate", 1.0), of("w", 1.0), 1 + of("scale", 0.0), of("b", 0.0)
+    branch = f * 1.0 if not post else norm64(f, kind, eps)
+    # rows: the norm of what a row may be off by, in front of the rounding to the output's type
+    e_xo = SUM * (rows_norm(ga * pw * branch) * (lf if post else 1) + rows_norm(x) + rows_norm(ref["xo"]))
+    hat_t = norm64(ref["xo"], kind, eps)
+    e_y = (SUM * lt * rows_norm(hat_t) + 2 * spread(ref["xo"])[0] * e_xo) * (w * sc).abs().amax() + SUM * rows_norm(ref["y"])
+    u = dy * sc * w
+    e_dx = SUM * lx * rx * rows_norm(u) + 4 * EPS32 * rows_norm(dxo)
+    v = ref["dx"] * ga * pw
+    top = (ga * pw).abs().amax()
+    e_df = (SUM * lf * rf * rows_norm(v) + 3 * rf * top * e_dx) if post else top * e_dx + 4 * EPS32 * rows_norm(v)
+    off = {"xo": e_xo, "y": e_y, "dx": e_dx, "df": e_df}
+    got = {"xo": back(xo), "y": back(y), "dx": back(dx), "df": back(df), **{k: t.cpu() for k, t in grads.items()}}
+    for name, t in (("xo", xt), ("y", ft), ("dx", xt), ("df", ft)):
+        full, size = ref[name], float(ref[name].norm())
+        allowed = half_step(t) * size + float(off[name].norm()) + tiny(t) * full.numel() ** 0.5
+        assert allowed < 0.05 * size, (name, allowed / size)               # (the bound says something: no gradient at all would be off by 1)
+        assert float((got[name].double() - full).norm()) <= allowed, (name, float((got[name].double() - full).norm()) / size, allowed / size)
+    # sums over rows: magnitudes of the terms, with their errors spread evenly over a row's channels
+    hat, run = norm64(x, kind, eps), (N / 256 + 64) * EPS32
+    n1, n2 = dy.abs() * run, dy.abs() * (SUM * lx * (hat.abs() + 1) + run * hat.abs())
+    flat = e_dx / Cc ** 0.5
+    m1, m2 = ref["dx"].abs() * run + flat, ref["dx"].abs() * (run * branch.abs() + (SUM * lf * (branch.abs() + 1) if post else 0)) + flat * branch.abs()
+    pb = of("post_b", 0.0)
+    terms = {"d_shift": n1, "d_scale": w.abs() * n2 + b.abs() * n1, "d_w": sc.abs() * n2, "d_b": sc.abs() * n1,
+             "d_gate": abs(alpha) * (pw.abs() * m2 + pb.abs() * m1), "d_post_w": ga.abs() * m2, "d_post_b": ga.abs() * m1}
+    for name in grads:
+        e, full = terms[name].expand(B, N, Cc).sum(1), ref[name]
+        allowed, size = float((e if got[name].dim() == 2 else e.sum(0)).norm()) + EPS32 * float(full.norm()), float(full.norm())
+        assert allowed < 0.15 * size, (name, allowed / size)
+        assert float((got[name].double() - full).norm()) <= allowed, (name, float((got[name].double() - full).norm()) / size, allowed / size)
+
+
+# ---- rotary: as large calls run it ------------------------------------------------------------------------------------------------
+def turned64(x, heads, plan, pos, theta, inverse):
+    """[B, N, heads D] on the GPU in 64 bits, from the definition: a pair is a complex number, turned."""
+    sections, rot = plan.sections, sum(plan.sections)
+    freq = [theta ** (-2.0 * j / n) for n in sections for j in range(n // 2)]
+    if plan.shared_spectrum:
+        freq = [theta ** (-2.0 * i / rot) for i in range(rot // 2)]
+    freq = torch.tensor(freq, dtype=torch.float64, device=x.device)
+    axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n // 2)], device=x.device)
+    angle = pos.double()[..., axis] * freq * (-1.0 if inverse else 1.0)
+    turn = torch.polar(torch.ones_like(angle), angle)
+    turn = turn[:, :, None] if turn.dim() == 3 else turn[None, :, None]
+    v = x.double().reshape(*x.shape[:2], heads, plan.D).clone()
+    a, b = (slice(0, rot, 2), slice(1, rot, 2)) if plan.neighbours else (slice(0, rot // 2), slice(rot // 2, rot))
+    z = torch.complex(v[..., a], v[..., b]) * turn
+    v[..., a], v[..., b] = z.real, z.imag
+    return v.reshape(x.shape)
+
+
+def close_turns(got, x, ref, heads, D, t):
+    """One rounding to t, and of the pair's largest magnitude 2^-20 (sine and cosine to 2^-21, two products and a sum)."""
+    top = x.double().view(-1, heads, D).abs().amax(-1, keepdim=True).expand(-1, heads, D).reshape(x.shape)
+    off = (got.double() - ref).abs() - half_step(t) * ref.abs() - tiny(t) - 2.0 ** -20 * top
+    assert float(off.max()) <= 0, float(off.max())
+
+
+LARGE = [
+    # B, N, q heads, k heads, D, sections: rows enough for several tokens a workgroup; N no multiple of any number of them
+    (3, 2741, 2, 2, 64, (24, 20, 20)),                     # 16-byte pieces of 16-bit halves
+    (2, 4099, 4, 1, 80, (28, 26, 26)),
+    (3, 1501, 3, 3, 72, (24, 24, 24)),                     # halves: 8-byte pieces, neighbours: 16
+    (2, 2999, 2, 2, 72, (24, 22, 22)),                     # four dims pass through; neighbours: 8-byte pieces, halves single values
+    (1, 5003, 2, 1, 128, (32, 32, 32)),                    # 32 dims pass through
+    (2, 2503, 2, 0, 40, (20, 20)),
+    (5, 1013, 1, 1, 160, (64, 48, 48)),
+    (2, 3001, 2, 2, 96, (16, 16, 16)),
+]
+
+
+@pytest.mark.parametrize("dtype", ["16", "32"])
+@pytest.mark.parametrize("neighbours,shared,inverse,real,own", [(False, False, False, False, True), (True, True, True, True, True),
+                                                               (True, False, False, False, False), (False, True, True, True, False)])
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "-".join(str(v) for v in c))
+def test_rotary_of_many_tokens(case, neighbours, shared, inverse, real, own, dtype, fmt):
+    """Aligned heads; own: positions per picture, so that a workgroup's tokens lie in two of them."""
+    check_rotary(*case, neighbours, shared, inverse, real, own, F32 if dtype == "32" else fmt)
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("dtype", ["16", "32"])
+def test_rotary_of_more_than_a_cache(dtype, neighbours, fmt):
+    """Over 32 MB read and written: four pieces of a thread in flight, a last turn that has fewer."""
+    check_rotary(2, 9007, 7, 2, 64, (24, 20, 20), neighbours, False, False, False, True, F32 if dtype == "32" else fmt)
+    check_rotary(1, 17011, 3, 3, 88, (20, 20, 20), neighbours, False, True, True, False, F32 if dtype == "32" else fmt)
+
+
+def check_rotary(B, N, hq, hk, D, sections, neighbours, shared, inverse, real, own, t):
+    g = torch.Generator(device=DEV).manual_seed(N + D)
+    heads = hq + hk
+    buf = torch.randn(B, N, heads * D + 8, generator=g, device=DEV).to(t)        # 16 bytes of another operand in front of the queries
+    buf[..., :8] = 7.0
+    out = torch.full_like(buf, 5.0)
+    pos = torch.randint(0, 4000, (B, N, len(sections)), generator=g, device=DEV, dtype=torch.int32)
+    pos = pos.float() * 0.37 - 100 if real else pos
+    pos = pos if own else pos[0].contiguous()
+    plan = RotaryAxes(D, sections, 10000.0, neighbours, shared, DEV)
+    v, o = (View(b.view(-1), B, 1, N, heads * D + 8) for b in (buf, out))
+    keep = buf.clone()
+
+    def parts(w):
+        return w.slice(8, hq * D), w.slice(8 + hq * D, hk * D) if hk else None
+    (q, k), (qo, ko) = parts(v), parts(o)
+    K.rotary_axes(plan, pos, q, qo, k, ko, inverse=inverse)
+    assert torch.equal(buf, keep) and bool((out[..., :8] == 5.0).all())
+    x = buf[..., 8:].contiguous()
+    ref = turned64(x, heads, plan, pos, 10000.0, inverse)
+    close_turns(out[..., 8:], x, ref, heads, D, t)
+    K.rotary_axes(plan, pos, q, None, k, None, inverse=inverse)                  # in place: the same bits
+    assert torch.equal(buf[..., 8:], out[..., 8:]) and bool((buf[..., :8] == 7.0).all())
+
+
+# ---- mxfp4 ------------------------------------------------------------------------------------------------------------------------
+def test_mxfp4_of_subnormal_blocks(fmt):
+    """Blocks whose largest magnitude is a subnormal of the 16-bit type, down to its smallest, and blocks that reach from there to normal values."""
+    small = torch.finfo(fmt).smallest_normal * torch.finfo(fmt).eps
+    g = gen(40)
+    rows = [torch.randint(-n, n + 1, (96,), generator=g).double() * small for n in (1, 2, 3, 7, 100, 127)]
+    if fmt == torch.float16:
+        rows += [torch.randint(-1023, 1024, (96,), generator=g).double() * small]
+    rows += [rows[-1].clone(), torch.zeros(96, dtype=torch.float64)]
+    rows[-2][::32] = torch.finfo(fmt).smallest_normal * 1.5
+    x = torch.stack(rows).to(fmt)
+    q = K.mxfp4_quantize(rows_view(x))
+    codes, scales, val = held64(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    y = empty(1, x.shape[0], 96, F32)
+    K.mxfp4_dequantize(q, y)
+    assert torch.equal(back(y)[0], val.float())
