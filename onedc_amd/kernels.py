@@ -23,6 +23,9 @@ DEFAULT_ACT = os.environ.get("ONEDC_ACT", "f16")
 class _ThreadFormat(threading.local):
     act = None
 
+    def __init__(self):
+        self.outer = []              # the formats in front of the blocks that this thread is in
+
 
 _tls = _ThreadFormat()
 
@@ -54,18 +57,20 @@ def in_own_format(method):
 
 
 class act_format(contextlib.ContextDecorator):
-    """The 16-bit format `name` for a block of code (or, as a decorator, for the calls of a function), in this thread."""
-    __slots__ = ("name", "prev")
+    """The 16-bit format `name` for a block of code (or, as a decorator, for the calls of a function), in this thread.  The format to go
+    back to is the thread's, not the object's: one object may be entered again inside its own block, and by several threads."""
+    __slots__ = ("name",)
 
     def __init__(self, name):
         self.name = name
 
     def __enter__(self):
-        self.prev = _tls.act
+        prev = _tls.act
         set_act(self.name)
+        _tls.outer.append(prev)
 
     def __exit__(self, *exc):
-        _tls.act = self.prev
+        _tls.act = _tls.outer.pop()
 
     def _recreate_cm(self):
         return act_format(self.name)
