@@ -77,10 +77,10 @@ struct RowSum {
         for (int i = 1; i < NTH / 64; ++i) s.x += r[i].x, s.y += r[i].y;
         return s;
     }
-    // v / C, rounded once but for a rare last bit
+    // v / C, rounded once but for a rare last bit; an infinite sum (of squares: r is 0 then) stays infinite
     __device__ __forceinline__ float over_C(float v) const {
         const float q = v * inv_C;
-        return __builtin_fmaf(__builtin_fmaf(-q, C, v), inv_C, q);
+        return fabsf(q) < __builtin_inff() ? __builtin_fmaf(__builtin_fmaf(-q, C, v), inv_C, q) : q;
     }
     __device__ __forceinline__ float mean(float v) {
         if constexpr (SHARED) return over_C(lanes_sum(v, L));
@@ -192,7 +192,7 @@ struct Vector {
         on = on_;
         if (!on) return;
         if constexpr (SHARED) {
-            last = ((p.C + 7) & ~7) - 8;
+            last = (p.C + 7) & ~7;
             for (int c = threadIdx.x; c < last + 8; c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
             lds = at_lds;
             at_lds += last + 8;
@@ -200,10 +200,14 @@ struct Vector {
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = combined(p, WHICH, b, min(c0 + i * step + j, p.C - 1));
+                for (int j = 0; j < 8; ++j) {
+                    const int c = c0 + i * step + j;
+                    const float q = combined(p, WHICH, b, min(c, p.C - 1));
+                    v[i][j] = c < p.C ? q : 0.f;
+                }
         }
     }
-    // eight of them from channel c on; a piece behind the row gets the last ones (finite: it multiplies zeros)
+    // eight of them from channel c on; zeros behind the row (an infinite one there would make a sum over the row no number)
     __device__ __forceinline__ void get(int i, int c, float (&o)[8]) const {
         if constexpr (SHARED) {
             c = min(c, last);
@@ -924,7 +928,7 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
         cut_runs(q, shape.threads / pl.L, shape.threads > 256 ? 512 : 1024, &pl);
         const int opt = !p->f || !p->y || p->post_b ? GENERIC : p->post ? JOIN_POST : JOIN;
         if (opt) pl.has = HAS_A | HAS_W | HAS_S;
-        const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * ((p->C + 7) & ~7) * 4 : 0);
+        const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * (((p->C + 7) & ~7) + 8) * 4 : 0);
         const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
         by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
             constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
@@ -996,7 +1000,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     float *part = sums ? (float *)((char *)g->ws + pictures_bytes(q, g)) : nullptr;
     const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
     if (rows) {
-        const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most, then the sums)
+        const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most with their zeros, then the sums)
         const size_t lds = shape.threads / 64 * 16 + scratch;
         const int opt = !p->f || !g->dy || !g->dxo || !g->dx || !g->df ? GENERIC : p->post ? JOIN_POST : JOIN;
         by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {

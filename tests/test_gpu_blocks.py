@@ -1,5 +1,5 @@
 """Transformer-block operators on the GPU, at the sizes and values where a bound per element says little: norms of the error of every output
-of block_norm and its backward pass, rotary_axes as large calls run it, subnormal blocks.
+of block_norm and its backward pass, rotary_axes as large calls run it, infinities and subnormals.
 
 half_step(t) = finfo(t).eps / 2 relative to a value is one rounding to t; EPS32 = 2^-24 is half a step of f32.
 """
@@ -95,6 +95,38 @@ def test_block_norm_norms_of_the_error(case, types, fmt):
         allowed, size = float((e if got[name].dim() == 2 else e.sum(0)).norm()) + EPS32 * float(full.norm()), float(full.norm())
         assert allowed < 0.15 * size, (name, allowed / size)
         assert float((got[name].double() - full).norm()) <= allowed, (name, float((got[name].double() - full).norm()) / size, allowed / size)
+
+
+WIDTHS = [5, 64, 100, 320, 643, 1280, 1283, 2048, 4096, 8200, 20001]          # every shape that a row has in registers, with and without a ragged end
+
+
+@pytest.mark.parametrize("types", ["16", "32"])
+@pytest.mark.parametrize("Cc", WIDTHS)
+def test_block_norm_of_an_infinite_value(Cc, types, fmt):
+    """RMSNorm of a row with an infinity: v / sqrt(inf) is 0 for every finite value and no number at the infinity itself.  The same where the
+    squares leave f32's range, in which they are summed.  LayerNorm: nothing is a number (inf - inf)."""
+    t = F32 if types == "32" else fmt
+    x = rand(gen(Cc), 1, 4, Cc).to(t)
+    x[0, 1, Cc // 2], x[0, 2, Cc - 1] = float("inf"), -float("inf")
+    if t != torch.float16:
+        x[0, 3] = 2.0 ** 70
+    w, b = rand(gen(1), Cc, shift=1.0), rand(gen(2), Cc)
+    y, xo = empty(1, 4, Cc, t), empty(1, 4, Cc, t)
+    K.block_norm(tokens(x), y, kind=K.NORM_RMS, eps=1e-6, w=w.to(DEV), b=b.to(DEV))
+    got, want = back(y)[0], b.to(t)
+    lost = torch.isinf(x[0])
+    assert torch.equal(got.isnan(), lost)
+    assert all(torch.equal(got[i][~lost[i]], want[~lost[i]]) for i in ((1, 2) if t == torch.float16 else (1, 2, 3)))
+    K.block_norm(tokens(x), y, kind=K.NORM_LAYER, eps=1e-6, w=w.to(DEV), b=b.to(DEV))
+    assert back(y)[0][1:3].isnan().all()
+    # the infinity comes from a gate: of the last channel, whose combined vector is read on behind the row
+    gate, f = torch.ones(Cc), rand(gen(3), 1, 4, Cc).to(t)
+    gate[Cc - 1] = float("inf")
+    x = rand(gen(4), 1, 4, Cc).to(t)
+    K.block_norm(tokens(x), y, f=tokens(f), xo=xo, kind=K.NORM_RMS, eps=1e-6, gate=gate.to(DEV), w=w.to(DEV), b=b.to(DEV))
+    got, last = back(y)[0], torch.arange(Cc) == Cc - 1
+    assert got[:, last].isnan().all() and torch.equal(got[:, ~last], want[~last].expand(4, -1))
+    assert torch.equal(back(xo)[0][:, last].double(), f[0][:, last].double().sign() * float("inf"))
 
 
 # ---- rotary: as large calls run it ------------------------------------------------------------------------------------------------
