@@ -77,14 +77,16 @@ struct RowSum {
         for (int i = 1; i < NTH / 64; ++i) s.x += r[i].x, s.y += r[i].y;
         return s;
     }
-    // v / C, rounded once but for a rare last bit; an infinite sum (of squares: r is 0 then) stays infinite
+    // v / C, rounded once but for a rare last bit.  INF: an infinite v stays infinite (its remainder, inf - inf, is taken as a finite number)
+    template <bool INF = false>
     __device__ __forceinline__ float over_C(float v) const {
-        const float q = v * inv_C;
-        return fabsf(q) < __builtin_inff() ? __builtin_fmaf(__builtin_fmaf(-q, C, v), inv_C, q) : q;
+        const float q = v * inv_C, e = __builtin_fmaf(-q, C, v);
+        return __builtin_fmaf(INF ? __builtin_fmaxf(e, -3.4e38f) : e, inv_C, q);
     }
+    template <bool INF = false>
     __device__ __forceinline__ float mean(float v) {
-        if constexpr (SHARED) return over_C(lanes_sum(v, L));
-        return over_C((*this)(v, 0.f).x);
+        if constexpr (SHARED) return over_C<INF>(lanes_sum(v, L));
+        return over_C<INF>((*this)(v, 0.f).x);
     }
     __device__ __forceinline__ float2 means(float v, float w) {
         const float2 s = (*this)(v, w);
@@ -243,7 +245,7 @@ __device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, 
     for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) q = __builtin_fmaf(v[i][j], v[i][j], q);
-    const float r = rsqrtf(sum.mean(q) + eps);
+    const float r = rsqrtf(sum.template mean<true>(q) + eps);         // (0 where the squares leave f32's range)
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
