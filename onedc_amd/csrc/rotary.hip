@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int NT = 256;
-constexpr int MAX_TABLE = 8192;           // pairs of sine and cosine in LDS: 64 KB
+constexpr int MAX_TABLE = 8192;           // pairs of sine and cosine in LDS: 64 KB, all that a launch has without asking for more
 
 // VEC values at p as f32
 template <bool F32, int VEC>
@@ -159,7 +159,7 @@ int launch(const onedc_rotary_params *p, void *stream) {
     u.T = (int)(T < 1 ? 1 : T);
     u.by_unit = OnedcFastDiv(u.per), u.by_head = OnedcFastDiv(heads), u.by_pair = OnedcFastDiv(p->pairs ? p->pairs : 1);
     const dim3 grid((unsigned)((rows + u.T - 1) / u.T));
-    const size_t lds = (size_t)u.T * p->pairs * 8 + 16;
+    const size_t lds = (size_t)u.T * p->pairs * 8;
     // four units of a thread in flight, two for small calls, whose threads have no more (tensors that no cache holds: 36864 x 16 x 80 39.6 us against
     // 41.8, 49152 x 32 x 80 102 against 109; 8000 x 16 x 64 8.3 against 7.9)
     const bool many = rows * heads * p->D * (F32 ? 8 : 4) > (32ll << 20);

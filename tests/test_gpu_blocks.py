@@ -185,6 +185,12 @@ def test_rotary_of_more_than_a_cache(dtype, neighbours, fmt):
     check_rotary(1, 17011, 3, 3, 88, (20, 20, 20), neighbours, False, True, True, False, F32 if dtype == "32" else fmt)
 
 
+@pytest.mark.parametrize("qh,kh,D,N", [(1, 1, 128, 70001), (1, 0, 128, 66000), (1, 1, 64, 131077)])
+def test_rotary_with_the_largest_table(qh, kh, D, N, fmt):
+    """Few heads of many tokens: sines and cosines fill the 64 KB of LDS that a launch may have."""
+    check_rotary(1, N, qh, kh, D, (D // 2, D // 4, D // 4), False, False, False, False, False, fmt)
+
+
 def check_rotary(B, N, hq, hk, D, sections, neighbours, shared, inverse, real, own, t):
     g = torch.Generator(device=DEV).manual_seed(N + D)
     heads = hq + hk
