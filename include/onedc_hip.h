@@ -382,7 +382,8 @@ int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_c
  * from t BEFORE xo's rounding.  Every vector is f32 and may be NULL (factor 1, summand 0); gate / scale / shift hold one row per
  * picture, `*_rs` floats apart (0: one row for all pictures, e.g. a learned per-channel residual scale as the gate).
  * x and xo are 16-bit or (x_f32) f32; f, y are 16-bit or (f_f32, only with x_f32) f32.  Rows are NHWC views: channel stride *_cs,
- * offset *_co, any values; xo may be x itself.  B * N rows: 0 to 2^30.  Launches only, no workspace.
+ * offset *_co, any values; xo may be x itself.  B * N rows: 0 to 2^30; with a parameter per picture a picture is a workgroup at least, and
+ * a launch holds fewer than 2^32 threads: B up to 2^24 - 1, 2^23 - 1 from 2049 and 2^22 - 1 from 4097 channels on.  Launches only, no workspace.
  * Returns -1 for a missing pointer, -2 for sizes or strides, -3 for a combination of options that has no meaning. */
 enum { ONEDC_NORM_LAYER = 0, ONEDC_NORM_RMS = 1 };
 typedef struct onedc_block_norm_params {
@@ -402,6 +403,7 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream);
  * be dy.  Parameter gradients, f32, each NULL where not wanted: d_post_w, d_post_b, d_w, d_b [C]; d_gate, d_scale, d_shift [C] per
  * picture, dense -- or one row summed over the pictures where the parameter is one row for all (*_rs == 0).
  * Sums over rows run in a fixed order (no atomics): partial sums per run of rows in ws, f32 inside a run, f64 across runs.
+ * With a parameter per picture and any parameter gradient, B * ceil(C / 32) is under 2^24 too.
  * ws: onedc_block_norm_backward_ws_bytes(p, g) bytes of device scratch, 16-byte aligned, the call's own until it has run (0: none
  * needed).  Statuses as above; -15: ws missing, too small or not aligned. */
 typedef struct onedc_block_norm_grad {
@@ -439,7 +441,7 @@ int onedc_rotary_axes(const onedc_rotary_params *p, void *stream);
  *              code, magnitudes over 6 to 6; a block with a NaN or an infinity becomes NaN.  x: 16-bit or (x_f32) f32 rows of K
  *              channels, stride x_cs, offset x_co
  *   dequantize the values, rounded once to y's type
- * Returns -1 for a missing pointer, -2 for sizes (K up to ONEDC_MXFP4_MAX_K), strides or a code
+ * Returns -1 for a missing pointer, -2 for sizes (K up to ONEDC_MXFP4_MAX_K, rows * ceil(K / 128) under 2^30 - 64), strides or a code
  * pointer that is not 16-byte aligned (scales: 4-byte). */
 int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream);
 int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y_f32, int y_cs, int y_co, int64_t rows, int K,
@@ -450,7 +452,8 @@ int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y
  * _LEAKY (slope), _SILU, or _GEGLU, where rows of w come in blocks of 16, values in front of their gates, N % 32 == 0, y and res have
  * N / 2 channels.  res has y's type and may be y.
  * x: either (xc, xs) as above, or, xc NULL, raw rows xr (16-bit or xr_f32, stride xr_cs, offset xr_co) that are quantised on the way:
- * only for M <= ONEDC_MXFP4_ROWS_RAW, without scratch.  M may be 0.
+ * only for M <= ONEDC_MXFP4_ROWS_RAW, without scratch.  M may be 0; from 17 rows on
+ * ceil(M / 128) * ceil(N / 128) is under 2^24, or M up to 2^26 - 16 where N * ceil(K / 128) < 4.
  * Returns -1 for a missing pointer, -2 for sizes, strides or alignment, -3 for an epilogue it does not know or a GEGLU layer with
  * N % 32, -4 for raw rows with M > ONEDC_MXFP4_ROWS_RAW. */
 #define ONEDC_MXFP4_ROWS_RAW 16

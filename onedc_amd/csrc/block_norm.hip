@@ -928,6 +928,7 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
         pl.has = (p->f && (p->gate || p->post_w) ? HAS_A : 0) | (p->f && p->post_b ? HAS_AB : 0) | (p->y && (p->w || p->scale) ? HAS_W : 0) |
                  (p->y && (p->b || p->shift) ? HAS_S : 0);
         cut_runs(q, shape.threads / pl.L, shape.threads > 256 ? 512 : 1024, &pl);
+        if (!onedc_grid_fits((int64_t)q.B * pl.runs, shape.threads)) return -2;
         const int opt = !p->f || !p->y || p->post_b ? GENERIC : p->post ? JOIN_POST : JOIN;
         if (opt) pl.has = HAS_A | HAS_W | HAS_S;
         const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * (((p->C + 7) & ~7) + 8) * 4 : 0);
@@ -977,7 +978,12 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
             return -3;
     }
     const bool sums = wants_sums(g);
-    if (sums && (int64_t)p->B * ((p->C + 31) / 32) > 0x7fffffff) return -2;
+    const onedc_block_norm_params q = joined_pictures(p);
+    Shape shape;
+    Plan pl;
+    const bool rows = any && backward_plan(q, sums, &shape, &pl);
+    if (any && !onedc_grid_fits((int64_t)q.B * pl.runs, rows ? shape.threads : simple_threads(p->C))) return -2;
+    if (sums && !onedc_grid_fits((int64_t)(any ? q.B : p->B) * ((p->C + 31) / 32), NT)) return -2;
     const int64_t need = onedc_block_norm_backward_ws_bytes(p, g);
     if (need && (!g->ws || g->ws_bytes < need || (uintptr_t)g->ws & 15)) return -15;
     if (!any) {
@@ -994,10 +1000,6 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
         }
         return 0;
     }
-    const onedc_block_norm_params q = joined_pictures(p);
-    Shape shape;
-    Plan pl;
-    const bool rows = backward_plan(q, sums, &shape, &pl);
     double *pictures = sums && pictures_bytes(q, g) ? (double *)g->ws : nullptr;
     float *part = sums ? (float *)((char *)g->ws + pictures_bytes(q, g)) : nullptr;
     const dim3 grid((unsigned)((int64_t)q.B * pl.runs));

@@ -23,6 +23,9 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
         if (e__ != hipSuccess) return (int)e__;      \
     } while (0)
 
+// The runtime takes fewer than 2^32 work items along an axis.
+inline bool onedc_grid_fits(int64_t workgroups, int threads) { return workgroups <= 0xffffffffll / threads; }
+
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 #ifdef ONEDC_ACT_F16
 typedef __attribute__((ext_vector_type(2))) _Float16 a16x2_t;

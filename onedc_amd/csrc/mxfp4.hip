@@ -613,7 +613,9 @@ bool whole_ok(const void *t, int cs, int co, bool f32) { return ((uintptr_t)t & 
 template <bool F32, bool VEC>
 int launch_quantize(const void *x, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream) {
     const int per = (K + 127) / 128 * 16;
-    hipLaunchKernelGGL((quantize_kernel<F32, VEC>), dim3((unsigned)((rows * per + 256 * QN - 1) / (256 * QN))), dim3(256), 0, as_stream(stream), x,
+    const int64_t wgs = (rows * per + 256 * QN - 1) / (256 * QN);
+    if (!onedc_grid_fits(wgs, 256)) return -2;
+    hipLaunchKernelGGL((quantize_kernel<F32, VEC>), dim3((unsigned)wgs), dim3(256), 0, as_stream(stream), x,
                        x_cs, x_co, (uint32_t *)codes, (uint8_t *)scales, rows, K, per, OnedcFastDiv(per));
     ONEDC_LAUNCH_CHECK();
     return 0;
@@ -621,7 +623,9 @@ int launch_quantize(const void *x, int x_cs, int x_co, void *codes, void *scales
 template <bool F32, bool VEC>
 int launch_dequantize(const void *codes, const void *scales, void *y, int y_cs, int y_co, int64_t rows, int K, void *stream) {
     const int per = (K + 127) / 128 * 16;
-    hipLaunchKernelGGL((dequantize_kernel<F32, VEC>), dim3((unsigned)((rows * per + 256 * QN - 1) / (256 * QN))), dim3(256), 0, as_stream(stream),
+    const int64_t wgs = (rows * per + 256 * QN - 1) / (256 * QN);
+    if (!onedc_grid_fits(wgs, 256)) return -2;
+    hipLaunchKernelGGL((dequantize_kernel<F32, VEC>), dim3((unsigned)wgs), dim3(256), 0, as_stream(stream),
                        (const uint32_t *)codes, (const uint8_t *)scales, y, y_cs, y_co, rows, K, per, OnedcFastDiv(per));
     ONEDC_LAUNCH_CHECK();
     return 0;
@@ -629,6 +633,7 @@ int launch_dequantize(const void *codes, const void *scales, void *y, int y_cs, 
 template <int RAW, bool VEC>
 int launch_skinny(const onedc_mxfp4_params *p, int steps, int whole, void *stream) {
     const int64_t wgs = (int64_t)((p->N + 31) / 32) * ((p->M + 15) / 16);
+    if (!onedc_grid_fits(wgs, 64 * SKW)) return -2;
     constexpr int sums = SKW * 2 * 16 * 20 * 4, raw = RAW ? 16 * (XPITCH + SPITCH) : 0, lds = sums > raw ? sums : raw;
     static OnedcLdsAttrOnce once;
     once.ensure({{(const void *)skinny_kernel<RAW, VEC>, lds}});
@@ -646,7 +651,7 @@ int launch_tiles(const onedc_mxfp4_params *p, int steps, int whole, void *stream
     static OnedcLdsAttrOnce once;
     once.ensure({{(const void *)tile_kernel<WN, WM, FN, FM, NST, OCC, KG>, lds}});
     const int64_t tn = (p->N + TN - 1) / TN, tm = (p->M + TM - 1) / TM;
-    if (tn * tm > 0x7fffffff) return -2;
+    if (!onedc_grid_fits(tn * tm, 64 * WN * WM * KG)) return -2;
     hipLaunchKernelGGL((tile_kernel<WN, WM, FN, FM, NST, OCC, KG>), dim3((unsigned)(tn * tm)), dim3(64 * WN * WM * KG), lds, as_stream(stream), *p, steps,
                        (int)tn, (int)tm, whole);
     ONEDC_LAUNCH_CHECK();
@@ -692,7 +697,6 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     if (!p->M) return 0;
     const int steps = (p->K + 127) / 128;
     const int whole = whole_ok(p->y, p->y_cs, p->y_co, p->y_f32) && (!p->res || whole_ok(p->res, p->r_cs, p->r_co, p->y_f32));
-    if (((int64_t)(p->N + 31) / 32) * ((p->M + 15) / 16) > 0x7fffffff) return -2;
     if (!p->xc) {
         const bool vec = p->K % 8 == 0 && whole_ok(p->xr, p->xr_cs, p->xr_co, p->xr_f32);
         if (p->xr_f32) return vec ? launch_skinny<2, true>(p, steps, whole, stream) : launch_skinny<2, false>(p, steps, whole, stream);

@@ -158,6 +158,7 @@ int launch(const onedc_rotary_params *p, void *stream) {
     if (p->pairs && T > MAX_TABLE / p->pairs) T = MAX_TABLE / p->pairs;
     u.T = (int)(T < 1 ? 1 : T);
     u.by_unit = OnedcFastDiv(u.per), u.by_head = OnedcFastDiv(heads), u.by_pair = OnedcFastDiv(p->pairs ? p->pairs : 1);
+    if (!onedc_grid_fits((rows + u.T - 1) / u.T, NT)) return -2;
     const dim3 grid((unsigned)((rows + u.T - 1) / u.T));
     const size_t lds = (size_t)u.T * p->pairs * 8;
     // four units of a thread in flight, two for small calls, whose threads have no more (tensors that no cache holds: 36864 x 16 x 80 39.6 us against

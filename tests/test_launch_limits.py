@@ -109,3 +109,71 @@ def test_rotary_asks_for_no_more_than_64_kb(launches):
     got = launches(calls)
     assert [(c, rc, ls) for c, (rc, ls) in zip(calls, got) if rc or len(ls) != 1] == []
     inside_limits(calls, got)
+
+
+def norm(B, C, *, picture, N=1, **over):
+    p = dict(x=FAR, f=2 * FAR, xo=3 * FAR, y=4 * FAR, gate=5 * FAR, B=B, N=N, C=C, x_cs=C, f_cs=C, xo_cs=C, y_cs=C, gate_rs=C if picture else 0,
+             alpha=1.0, eps=1e-5)
+    return ["onedc_block_norm", {**p, **over}]
+
+
+def norm_back(B, C, *, picture, sums, N=1):
+    p = dict(x=FAR, f=2 * FAR, gate=5 * FAR, w=9 * FAR, B=B, N=N, C=C, x_cs=C, f_cs=C, gate_rs=C if picture else 0, alpha=1.0, eps=1e-5)
+    g = dict(dy=6 * FAR, dy_cs=C, dx=7 * FAR, dx_cs=C, df=8 * FAR, df_cs=C)
+    if sums:
+        g.update(d_gate=10 * FAR, d_w=11 * FAR)
+    return ["onedc_block_norm_backward", [p, g]]
+
+
+def linear(M, N, K_, epi=0):
+    out = N // 2 if epi == 4 else N
+    return ["onedc_mxfp4_linear", dict(xc=FAR, xs=2 * FAR, wc=3 * FAR, ws=4 * FAR, y=5 * FAR, M=M, N=N, K=K_, y_cs=out, alpha=1.0, epi=epi)]
+
+
+M31 = 0x7fffffff
+FITS = [
+    # the last call that a launch holds, and the first that it does not
+    (norm((1 << 24) - 1, 64, picture=True), norm(1 << 24, 64, picture=True)),
+    (norm((1 << 23) - 1, 4000, picture=True), norm(1 << 23, 4000, picture=True)),
+    (norm((1 << 22) - 1, 8200, picture=True), norm(1 << 22, 8200, picture=True)),
+    (norm_back((1 << 24) - 1, 64, picture=True, sums=False), norm_back(1 << 24, 64, picture=True, sums=False)),
+    (norm_back((1 << 23) - 1, 64, picture=True, sums=True), norm_back(1 << 23, 64, picture=True, sums=True)),
+    (norm_back(((1 << 24) - 1) // 10, 320, picture=True, sums=True), norm_back(((1 << 24) - 1) // 10 + 1, 320, picture=True, sums=True)),
+    (norm_back((1 << 22) - 1, 20000, picture=True, sums=False), norm_back(1 << 22, 20000, picture=True, sums=False)),
+    (["onedc_mxfp4_quantize", [FAR, 0, 1, 0, 2 * FAR, 3 * FAR, (1 << 30) - 64, 1]], ["onedc_mxfp4_quantize", [FAR, 0, 1, 0, 2 * FAR, 3 * FAR, 1 << 30, 1]]),
+    (["onedc_mxfp4_dequantize", [FAR, 2 * FAR, 3 * FAR, 1, 1, 0, (1 << 30) - 64, 1]], ["onedc_mxfp4_dequantize", [FAR, 2 * FAR, 3 * FAR, 1, 1, 0, 1 << 30, 1]]),
+    (linear((1 << 26) - 16, 1, 1), linear(1 << 26, 1, 1)),
+    (linear(M31 - 128, 128, 128), linear(M31, 128, 128)),
+    (linear((1 << 28) - 128, 1024, 128, epi=4), linear(1 << 29, 1024, 128, epi=4)),
+    (rotary((1 << 24) - 1, 16, 1, 128, 0, x_f32=1), rotary(1 << 24, 128, 1, 128, 0, x_f32=1)),
+]
+
+
+def test_what_a_launch_does_not_hold_is_refused(launches):
+    calls = [c for pair in FITS for c in pair]
+    got = launches(calls)
+    inside_limits(calls, got)
+    for i, (fits, not_) in enumerate(FITS):
+        assert got[2 * i][0] == 0 and got[2 * i][1], fits
+        assert got[2 * i + 1] == (-2, []), not_
+
+
+def test_rows_without_a_parameter_per_picture_are_one_picture(launches):
+    """2^30 rows, however they are cut into pictures."""
+    calls = [norm(1 << 30, 64, picture=False), norm(1, 320, picture=False, N=1 << 30), norm(1 << 20, 5, picture=False, N=1 << 10),
+             norm_back(1 << 30, 64, picture=False, sums=True), norm_back(1 << 15, 1283, picture=False, sums=True, N=1 << 15)]
+    got = launches(calls)
+    assert [rc for rc, _ in got] == [0] * len(calls)
+    inside_limits(calls, got)
+
+
+def test_launches_over_the_range_of_sizes(launches):
+    sizes = [1, 2, 15, 17, 100, 513, 4097, 36864]
+    calls = [linear(M, N, K_, epi) for M in sizes for N in (32, 96, 320, 2048, 10240) for K_ in (1, 129, 640, 8192) for epi in (0, 4)]
+    calls += [norm(B, C, picture=pic, N=N) for B in (1, 3, 16) for N in (1, 7, 9216) for pic in (False, True)
+              for C in (1, 7, 8, 64, 65, 512, 1024, 1025, 1280, 1536, 1537, 2048, 4096, 8192, 8193, 16384, 16385, 100000)]
+    calls += [norm_back(B, C, picture=pic, sums=s, N=N) for B in (1, 16) for N in (1, 9216) for pic in (False, True) for s in (False, True)
+              for C in (1, 8, 64, 512, 1024, 1025, 2048, 4096, 8192, 8193, 100000)]
+    got = launches(calls)
+    assert [(c, rc) for c, (rc, ls) in zip(calls, got) if rc or not ls] == []
+    inside_limits(calls, got)
