@@ -372,6 +372,10 @@ int onedc_ref_prior_indexes(const float *params, const float *thresholds, int n_
 int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_cs, int x_co, int y_cs, int y_co,
                           void *stream);
 
+/* Status of the transformer-block operators: an output lies in the memory of something else that the call reads or writes, and the form is not
+ * one that the operator's comment allows.  (Other channels of rows of one pitch are other memory.) */
+#define ONEDC_SHARED_MEMORY (-17)
+
 /* ---- transformer-block operators for image / video tokens ---------------------------------------------------------------
  * Norms before and after a block fused with the block's gate and the residual scale: the join between two sub-blocks of a
  * transformer block in one pass over the residual stream.  Per token row (b, n) of C channels:
@@ -442,7 +446,7 @@ int onedc_rotary_axes(const onedc_rotary_params *p, void *stream);
  *              channels, stride x_cs, offset x_co
  *   dequantize the values, rounded once to y's type
  * Returns -1 for a missing pointer, -2 for sizes (K up to ONEDC_MXFP4_MAX_K, rows * ceil(K / 128) under 2^30 - 64), strides or a code
- * pointer that is not 16-byte aligned (scales: 4-byte). */
+ * pointer that is not 16-byte aligned (scales: 4-byte), ONEDC_SHARED_MEMORY where what is written shares memory with another operand. */
 int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *codes, void *scales, int64_t rows, int K, void *stream);
 int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y_f32, int y_cs, int y_co, int64_t rows, int K,
                            void *stream);
@@ -455,7 +459,7 @@ int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y
  * only for M <= ONEDC_MXFP4_ROWS_RAW, without scratch.  M may be 0; from 17 rows on
  * ceil(M / 128) * ceil(N / 128) is under 2^24, or M up to 2^26 - 16 where N * ceil(K / 128) < 4.
  * Returns -1 for a missing pointer, -2 for sizes, strides or alignment, -3 for an epilogue it does not know or a GEGLU layer with
- * N % 32, -4 for raw rows with M > ONEDC_MXFP4_ROWS_RAW. */
+ * N % 32, -4 for raw rows with M > ONEDC_MXFP4_ROWS_RAW, ONEDC_SHARED_MEMORY where y shares memory with x, w or the bias. */
 #define ONEDC_MXFP4_ROWS_RAW 16
 #define ONEDC_MXFP4_MAX_K (1 << 22)
 typedef struct onedc_mxfp4_params {

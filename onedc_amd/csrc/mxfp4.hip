@@ -6,6 +6,7 @@
 // for few rows, 32x32x64 (row l % 32, values 32 (l / 32) on) for tiles.  Products are exact, sums f32.
 #include <type_traits>
 
+#include "apart.h"
 #include "conv_common.h"
 #include "elem.h"
 
@@ -606,6 +607,10 @@ __global__ __launch_bounds__(64 * WN * WM * KG, OCC) void tile_kernel(onedc_mxfp
     }
 }
 
+// the codes and the scales of a matrix
+OnedcMem codes_of(const void *p, int64_t rows, int K) { return onedc_mem(p, rows * ((K + 127) / 128) * 64); }
+OnedcMem scales_of(const void *p, int64_t rows, int K) { return onedc_mem(p, rows * ((K + 127) / 128) * 4); }
+
 bool held_ok(const void *codes, const void *scales) { return ((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 3) == 0; }
 // whole 16-byte pieces of eight (16-bit) or four (f32) values at every row
 bool whole_ok(const void *t, int cs, int co, bool f32) { return ((uintptr_t)t & 15) == 0 && ((cs | co) & (f32 ? 3 : 7)) == 0; }
@@ -668,6 +673,8 @@ int onedc_mxfp4_quantize(const void *x, int x_f32, int x_cs, int x_co, void *cod
         rows * ((K + 127) / 128) > (1ll << 36))
         return -2;
     if (!rows) return 0;
+    const OnedcMem c = codes_of(codes, rows, K), e = scales_of(scales, rows, K), from = onedc_mem_rows(x, rows, x_cs, x_co, K, x_f32 ? 4 : 2);
+    if (onedc_mem_shared(c, from) || onedc_mem_shared(e, from) || onedc_mem_shared(c, e)) return ONEDC_SHARED_MEMORY;
     const bool vec = K % 8 == 0 && whole_ok(x, x_cs, x_co, x_f32);
     if (x_f32) return vec ? launch_quantize<true, true>(x, x_cs, x_co, codes, scales, rows, K, stream) : launch_quantize<true, false>(x, x_cs, x_co, codes, scales, rows, K, stream);
     return vec ? launch_quantize<false, true>(x, x_cs, x_co, codes, scales, rows, K, stream) : launch_quantize<false, false>(x, x_cs, x_co, codes, scales, rows, K, stream);
@@ -679,6 +686,8 @@ int onedc_mxfp4_dequantize(const void *codes, const void *scales, void *y, int y
         rows * ((K + 127) / 128) > (1ll << 36))
         return -2;
     if (!rows) return 0;
+    const OnedcMem to = onedc_mem_rows(y, rows, y_cs, y_co, K, y_f32 ? 4 : 2);
+    if (onedc_mem_shared(to, codes_of(codes, rows, K)) || onedc_mem_shared(to, scales_of(scales, rows, K))) return ONEDC_SHARED_MEMORY;
     const bool vec = K % 8 == 0 && whole_ok(y, y_cs, y_co, y_f32);
     if (y_f32) return vec ? launch_dequantize<true, true>(codes, scales, y, y_cs, y_co, rows, K, stream) : launch_dequantize<true, false>(codes, scales, y, y_cs, y_co, rows, K, stream);
     return vec ? launch_dequantize<false, true>(codes, scales, y, y_cs, y_co, rows, K, stream) : launch_dequantize<false, false>(codes, scales, y, y_cs, y_co, rows, K, stream);
@@ -695,6 +704,11 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     if (p->xc ? !held_ok(p->xc, p->xs) : (p->xr_co < 0 || (int64_t)p->xr_cs - p->K < p->xr_co)) return -2;
     if (!p->xc && p->M > ONEDC_MXFP4_ROWS_RAW) return -4;
     if (!p->M) return 0;
+    const OnedcMem y[1] = {onedc_mem_rows(p->y, p->M, p->y_cs, p->y_co, out, p->y_f32 ? 4 : 2)};
+    const OnedcMem read[] = {codes_of(p->wc, p->N, p->K), scales_of(p->ws, p->N, p->K), p->xc ? codes_of(p->xc, p->M, p->K) : OnedcMem(),
+                             p->xc ? scales_of(p->xs, p->M, p->K) : onedc_mem_rows(p->xr, p->M, p->xr_cs, p->xr_co, p->K, p->xr_f32 ? 4 : 2),
+                             onedc_mem(p->bias, (int64_t)p->N * 4)};
+    if (onedc_mem_any_shared(y, read)) return ONEDC_SHARED_MEMORY;
     const int steps = (p->K + 127) / 128;
     const int whole = whole_ok(p->y, p->y_cs, p->y_co, p->y_f32) && (!p->res || whole_ok(p->res, p->r_cs, p->r_co, p->y_f32));
     if (!p->xc) {

@@ -262,9 +262,12 @@ class HalfRangeError(FloatingPointError):
                          f"({act} activations: half-precision range exceeded); set act_dtype: bf16 in the config")
 
 
+SHARED_MEMORY = -17        # ONEDC_SHARED_MEMORY of include/onedc_hip.h
+
+
 def _ok(rc, name):
     if rc != 0:
-        raise KernelError(f"{name} failed with status {rc}")
+        raise KernelError(f"{name}: an output shares memory with another operand" if rc == SHARED_MEMORY else f"{name} failed with status {rc}")
 
 
 # the raw handle without a Stream object around it where torch has that call (2.7 us less a launch)

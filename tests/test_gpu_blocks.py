@@ -9,7 +9,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from onedc_amd import kernels as K
-from onedc_amd.kernels import RotaryAxes, View
+from onedc_amd.kernels import KernelError, RotaryAxes, View
 from test_gpu_token_ops import (CASES, DEV, EPS32, F32, FORMATS, back, empty, gen, grads64, half_step, held64, in64, join64, norm64, on_gpu,
                                 options, rand, rows_view, tiny, tokens)
 
@@ -233,3 +233,36 @@ def test_mxfp4_of_subnormal_blocks(fmt):
     y = empty(1, x.shape[0], 96, F32)
     K.mxfp4_dequantize(q, y)
     assert torch.equal(back(y)[0], val.float())
+
+
+# ---- operands in each other's memory: refused before a launch ------------------------------------------------------------------------
+def shared(fn, *a, **k):
+    with pytest.raises(KernelError, match="shares memory"):
+        fn(*a, **k)
+
+
+def test_mxfp4_outputs_in_operands(fmt):
+    M, N, k = 40, 64, 256
+    x, w = rows_view(rand(gen(50), M, k).to(fmt)), K.mxfp4_quantize(rows_view(rand(gen(51), N, k)))
+    q = K.mxfp4_quantize(x)
+    bias = torch.ones(M * N, device=DEV)
+    keep = [t.clone() for t in (q.codes, q.scales, w.codes, w.scales)]
+
+    def over(t, rows, Cc, dtype=fmt):                     # a View of rows in t's memory
+        return View(t.view(-1).view(dtype), 1, 1, rows, Cc)
+    for t in (q.codes, w.codes):
+        shared(K.mxfp4_linear, q, w, None, over(t, 40, 64))
+    big = torch.zeros(M * N * 8, dtype=torch.uint8, device=DEV)                  # scales of a matrix inside the output's memory
+    for held in (q, w):
+        scales = big[64:64 + held.scales.numel()].view(held.scales.shape).copy_(held.scales)
+        inside = K.MxFp4(held.codes, scales, held.rows, k)
+        shared(K.mxfp4_linear, inside if held is q else q, inside if held is w else w, None, over(big, M, N, F32))
+    shared(K.mxfp4_linear, q, w, bias[:N], View(bias, 1, 1, M, N))
+    assert all(torch.equal(a, b) for a, b in zip((q.codes, q.scales, w.codes, w.scales), keep))
+    room = torch.zeros(M * k * 4, dtype=torch.uint8, device=DEV)                 # x, and in its memory the codes or the scales
+    y = View(room.view(F32), 1, 1, M, k)
+    shared(K.mxfp4_quantize, y, K.MxFp4(room[:M * k // 2].view(M, k // 2), q.scales, M, k))
+    shared(K.mxfp4_quantize, y, K.MxFp4(q.codes, room[-M * k // 32:].view(M, k // 32), M, k))
+    shared(K.mxfp4_quantize, x, K.MxFp4(room[:M * k // 2].view(M, k // 2), room[64:64 + M * k // 32].view(M, k // 32), M, k))
+    shared(K.mxfp4_dequantize, K.MxFp4(room[:M * k // 2].view(M, k // 2), q.scales, M, k), y)
+    shared(K.mxfp4_dequantize, K.MxFp4(q.codes, room[-M * k // 32:].view(M, k // 32), M, k), y)

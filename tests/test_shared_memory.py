@@ -1,0 +1,110 @@
+"""Operands of the transformer-block operators that lie in each other's memory: what the C entries refuse (on the host, nothing is launched).
+
+Addresses are made up.  The comparison itself (csrc/apart.h) is compiled for the host."""
+import ctypes as C
+import itertools
+import os
+import subprocess
+
+import pytest
+
+from onedc_amd import build, kernels as K
+from test_launch_limits import launches  # noqa: F401  (a fixture)
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SHARED = -17
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _hip():
+    build.build_hip()
+
+
+def test_the_status_is_the_headers(tmp_path):
+    src = tmp_path / "status.cpp"
+    src.write_text('#include "onedc_hip.h"\n#include <cstdio>\nint main() { printf("%d", ONEDC_SHARED_MEMORY); }\n')
+    subprocess.run(["g++", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "status"), str(src)], check=True)
+    got = int(subprocess.run([str(tmp_path / "status")], check=True, capture_output=True, text=True).stdout)
+    assert got == SHARED == K.SHARED_MEMORY
+    with pytest.raises(K.KernelError, match="shares memory"):
+        K._ok(SHARED, "onedc_mxfp4_linear")
+
+
+def test_rows_that_meet_or_do_not(tmp_path):
+    """Against the bytes themselves, over small operands: nothing shared is missed; what is apart is called shared only for rows of different pitches."""
+    src = tmp_path / "apart.cpp"
+    src.write_text('#include "apart.h"\nextern "C" int shared(long a, long n, long cs, long w, long b, long m, long ds, long v) {\n'
+                   "    return onedc_mem_shared(onedc_mem_rows((void *)a, n, cs, 0, w, 1), onedc_mem_rows((void *)b, m, ds, 0, v, 1)); }\n")
+    so = str(tmp_path / "apart.so")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "onedc_amd", "csrc"), "-o", so, str(src)], check=True)
+    shared = C.CDLL(so).shared
+    shared.argtypes = [C.c_long] * 8
+
+    def bytes_of(at, rows, pitch, width):
+        return {at + r * pitch + i for r in range(rows) for i in range(width)}
+    over = 0
+    for n, cs, w, m, ds, v in itertools.product((1, 2, 3), (3, 4, 8), (1, 2, 3), (1, 2, 4), (2, 4, 12), (1, 2)):
+        for b in range(970, 1040):
+            meet = bool(bytes_of(1000, n, cs, w) & bytes_of(b, m, ds, v))
+            got = bool(shared(1000, n, cs, w, b, m, ds, v))
+            assert got or not meet, (n, cs, w, b, m, ds, v)
+            if got and not meet:
+                over += 1
+                assert n > 1 and m > 1 and cs != ds or w > cs or v > ds or n == 1 or m == 1, (n, cs, w, b, m, ds, v)
+    assert over
+    assert not shared(0, 3, 8, 2, 1, 1, 8, 1)             # NULL: no operand
+
+
+# ---- mxfp4 ------------------------------------------------------------------------------------------------------------------------
+M, N, KV = 40, 64, 200                                    # two steps of 128: 128 bytes of codes and 8 of scales a row
+AT = dict(xc=0x100000, xs=0x200000, wc=0x300000, ws=0x400000, bias=0x500000, y=0x600000)
+SIZE = dict(xc=M * 128, xs=M * 8, wc=N * 128, ws=N * 8, bias=N * 4)
+
+
+def linear(**over):
+    p = K.MxFp4Params(**{**AT, **dict(M=M, N=N, K=KV, y_cs=N, alpha=1.0), **over})
+    return K.lib().onedc_mxfp4_linear(C.byref(p), None)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("name", sorted(SIZE))
+def test_mxfp4_linear_over_what_it_reads(name, f32):
+    rows = ((M - 1) * N + N) * (4 if f32 else 2)
+    for y in (AT[name], AT[name] + SIZE[name] - (4 if f32 else 2), AT[name] - rows + 4, AT[name] - rows // 2 // 4 * 4):
+        assert linear(y=y, y_f32=f32) == SHARED, (name, hex(y))
+    if name == "bias":                                   # (the end of a row lies on it, and it does not fit between the rows)
+        assert linear(y=AT[name] - 128 * 4, y_cs=256, y_f32=1, y_co=96) == SHARED
+
+
+def test_what_stays_allowed(launches):
+    """Other columns of one buffer's rows, and memory that begins where another operand ends."""
+    p = dict(M=16, N=N, K=KV, alpha=1.0, wc=AT["wc"], ws=AT["ws"])
+    calls = [["onedc_mxfp4_linear", dict(**p, xr=0x100000, xr_cs=300, y=0x100000, y_cs=300, y_co=KV)],
+             ["onedc_mxfp4_linear", dict(**p, xr=0x100000, xr_cs=300, xr_co=100, y=0x100000, y_cs=300, y_co=36, res=0x100000, r_cs=300, r_co=36)],
+             ["onedc_mxfp4_linear", dict(**p, xr=0x100000, xr_cs=KV, y=AT["wc"] + N * 128, y_cs=N, bias=AT["wc"] - 4 * N)],
+             ["onedc_mxfp4_quantize", [0x100000, 0, KV, 0, 0x100000 + 8 * KV * 2, 0x100000 - 64, 8, KV]],
+             ["onedc_mxfp4_dequantize", [0x100000, 0x100000 + 8 * 128, 0x100000 + 8 * 136, 0, KV, 0, 8, KV]]]
+    assert [rc for rc, _ in launches(calls)] == [0] * len(calls)
+
+
+def test_mxfp4_linear_over_raw_rows():
+    raw = dict(xc=None, xs=None, xr=0x100000, xr_cs=KV, M=16)
+    assert linear(**raw, y=0x100000) == SHARED
+    assert linear(**{**raw, "xr_cs": 300}, y=0x100000, y_cs=300, y_co=KV - 1) == SHARED
+    assert linear(**{**raw, "xr_f32": 1}, y=0x100000 + 4 * (16 * KV - 1)) == SHARED
+
+
+def test_mxfp4_quantize_and_back_over_their_operands():
+    lib, x, c, s = K.lib(), 0x100000, 0x200000, 0x300000
+
+    def quantize(x, c, s, rows=8, f32=0):
+        return lib.onedc_mxfp4_quantize(x, f32, KV, 0, c, s, rows, KV, None)
+
+    def back(c, s, y, rows=8, f32=0, cs=KV, co=0):
+        return lib.onedc_mxfp4_dequantize(c, s, y, f32, cs, co, rows, KV, None)
+    assert quantize(x, x, s) == quantize(x, x + 8 * KV * 2 - 16, s) == quantize(x + 8 * 128 - 2, x, s) == SHARED
+    assert quantize(x, c, x) == quantize(x, c, x + 8 * KV * 2 - 4) == SHARED
+    assert quantize(x, c, x + 8 * KV * 4 - 4, f32=1) == SHARED
+    assert quantize(x, c, c) == quantize(x, c, c + 8 * 128 - 4) == quantize(x, c + 32, c) == SHARED
+    assert back(c, s, c) == back(c, s, c + 8 * 128 - 2) == back(c, s, s) == back(c, s, s + 8 * 8 - 2) == SHARED
+    assert back(c, s, c - 4 * KV, f32=1) == back(c, s, c, cs=KV + 8, co=8) == SHARED
