@@ -20,6 +20,9 @@ from . import _native
 # CALLING CONTEXT (thread-local): layers pack their weights and allocate their outputs in the format that is current when
 # they are built / called, and `lib()` hands out the matching library.
 DEFAULT_ACT = os.environ.get("ONEDC_ACT", "f16")
+ACT_FORMATS = ("bf16", "f16")
+
+
 class _ThreadFormat(threading.local):
     act = None
 
@@ -40,7 +43,7 @@ def a16():
 
 
 def set_act(name):
-    if name not in ("bf16", "f16"):
+    if name not in ACT_FORMATS:
         raise ValueError(f"activation format must be 'bf16' or 'f16', not {name!r}")
     _tls.act = name
 
@@ -65,9 +68,10 @@ class act_format(contextlib.ContextDecorator):
         self.name = name
 
     def __enter__(self):
-        prev = _tls.act
-        set_act(self.name)
-        _tls.outer.append(prev)
+        if self.name not in ACT_FORMATS:
+            set_act(self.name)                           # (says what is wrong)
+        _tls.outer.append(_tls.act)
+        _tls.act = self.name
 
     def __exit__(self, *exc):
         _tls.act = _tls.outer.pop()
