@@ -388,7 +388,8 @@ int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_c
  * x and xo are 16-bit or (x_f32) f32; f, y are 16-bit or (f_f32, only with x_f32) f32.  Rows are NHWC views: channel stride *_cs,
  * offset *_co, any values; xo may be x itself.  B * N rows: 0 to 2^30; with a parameter per picture a picture is a workgroup at least, and
  * a launch holds fewer than 2^32 threads: B up to 2^24 - 1, 2^23 - 1 from 2049 and 2^22 - 1 from 4097 channels on.  Launches only, no workspace.
- * Returns -1 for a missing pointer, -2 for sizes or strides, -3 for a combination of options that has no meaning. */
+ * Returns -1 for a missing pointer, -2 for sizes or strides, -3 for a combination of options that has no meaning, ONEDC_SHARED_MEMORY where
+ * xo or y lies in a vector's memory. */
 enum { ONEDC_NORM_LAYER = 0, ONEDC_NORM_RMS = 1 };
 typedef struct onedc_block_norm_params {
     const void *x; const void *f; void *xo; void *y;
@@ -409,7 +410,8 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream);
  * Sums over rows run in a fixed order (no atomics): partial sums per run of rows in ws, f32 inside a run, f64 across runs.
  * With a parameter per picture and any parameter gradient, B * ceil(C / 32) is under 2^24 too.
  * ws: onedc_block_norm_backward_ws_bytes(p, g) bytes of device scratch, 16-byte aligned, the call's own until it has run (0: none
- * needed).  Statuses as above; -15: ws missing, too small or not aligned. */
+ * needed).  Statuses as above; -15: ws missing, too small or not aligned; ONEDC_SHARED_MEMORY also where a
+ * parameter gradient or ws lies in the memory of anything else, part of it or all. */
 typedef struct onedc_block_norm_grad {
     const void *dy; const void *dxo; void *dx; void *df;
     float *d_post_w; float *d_post_b; float *d_gate; float *d_w; float *d_b; float *d_scale; float *d_shift;

@@ -8,8 +8,10 @@
 //   df = the same step through norm(f) on alpha * gate * post_w * dt, or alpha * gate * dt without the post norm
 // and every parameter gradient follows from four sums over the rows of a picture: S1 = sum dy, S2 = sum dy * norm(t),
 // T1 = sum dt, T2 = sum dt * norm(f) (f itself without the post norm).
+#include <iterator>
 #include <type_traits>
 
+#include "apart.h"
 #include "elem.h"
 
 namespace {
@@ -195,7 +197,8 @@ struct Vector {
         if (!on) return;
         if constexpr (SHARED) {
             last = (p.C + 7) & ~7;
-            for (int c = threadIdx.x; c < last + 8; c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
+            for (int c = threadIdx.x; c < last; c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
+            if (threadIdx.x < 8) at_lds[last + threadIdx.x] = 0.f;
             lds = at_lds;
             at_lds += last + 8;
         } else {
@@ -807,6 +810,36 @@ onedc_block_norm_params joined_pictures(const onedc_block_norm_params *p) {
     return q;
 }
 
+// The vectors that a call reads: per channel, and per picture
+constexpr int VECTORS = 7;
+void vectors_of(const onedc_block_norm_params *p, OnedcMem (&m)[VECTORS]) {
+    const auto each = [&](const float *v, int rs) { return onedc_mem_rows(v, rs ? p->B : 1, rs, 0, p->C, 4); };
+    const float *all[] = {p->post_w, p->post_b, p->w, p->b};
+    for (int i = 0; i < 4; ++i) m[i] = onedc_mem(all[i], (int64_t)p->C * 4);
+    m[4] = each(p->gate, p->gate_rs), m[5] = each(p->scale, p->scale_rs), m[6] = each(p->shift, p->shift_rs);
+}
+OnedcMem rows_of(const onedc_block_norm_params *p, const void *t, int cs, int co, int f32) {
+    return onedc_mem_rows(t, (int64_t)p->B * p->N, cs, co, p->C, f32 ? 4 : 2);
+}
+// A parameter's gradient lies apart from everything else; dx and df apart from the vectors (from rows of x, f, dy and dxo: the caller's affair, who
+// may name some of them again); the workspace apart from all
+bool gradients_apart(const onedc_block_norm_params *p, const onedc_block_norm_grad *g, int64_t need) {
+    OnedcMem v[VECTORS];
+    vectors_of(p, v);
+    const int64_t one = (int64_t)p->C * 4, each = one * p->B;
+    const OnedcMem d[] = {onedc_mem(g->d_post_w, one), onedc_mem(g->d_post_b, one), onedc_mem(g->d_w, one), onedc_mem(g->d_b, one),
+                          onedc_mem(g->d_gate, p->gate_rs ? each : one), onedc_mem(g->d_scale, p->scale_rs ? each : one),
+                          onedc_mem(g->d_shift, p->shift_rs ? each : one), onedc_mem(need ? g->ws : nullptr, need)};
+    const OnedcMem out[] = {rows_of(p, g->dx, g->dx_cs, g->dx_co, p->x_f32), rows_of(p, g->df, g->df_cs, g->df_co, p->f_f32)};
+    const OnedcMem in[] = {rows_of(p, p->x, p->x_cs, p->x_co, p->x_f32), rows_of(p, p->f, p->f_cs, p->f_co, p->f_f32),
+                           rows_of(p, g->dy, g->dy_cs, g->dy_co, p->f_f32), rows_of(p, g->dxo, g->dxo_cs, g->dxo_co, p->x_f32)};
+    if (onedc_mem_any_shared(d, v) || onedc_mem_any_shared(d, out) || onedc_mem_any_shared(d, in) || onedc_mem_any_shared(out, v)) return false;
+    for (const OnedcMem *a = d; a != std::end(d); ++a)
+        for (const OnedcMem *b = d; b != a; ++b)
+            if (onedc_mem_shared(*a, *b)) return false;
+    return true;
+}
+
 // How rows lie in lanes, by the row's width alone.  Two pieces a lane, in as few lanes as that takes: 4.4 TB/s at 320 channels and 5.4 at
 // 640 against 4.2 / 3.0 with one piece (twice the lanes, half of them idle) and, three pieces, 4.3 / 5.0; five pieces spill.  Three where two
 // of 64 lanes end (1280 channels: 4.3 against 3.8 for one row a workgroup), but not with a ragged end, whose code takes their registers.
@@ -921,6 +954,10 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
     if (check_view(p->xo, p->xo_cs, p->xo_co, p->C) || check_view(p->y, p->y_cs, p->y_co, p->C)) return -2;
     if (!p->f != !p->xo) return -3;
     if (!p->y && (p->w || p->b || p->scale || p->shift)) return -3;
+    OnedcMem vectors[VECTORS];
+    vectors_of(p, vectors);
+    const OnedcMem out[] = {rows_of(p, p->xo, p->xo_cs, p->xo_co, p->x_f32), rows_of(p, p->y, p->y_cs, p->y_co, p->f_f32)};
+    if (onedc_mem_any_shared(out, vectors)) return ONEDC_SHARED_MEMORY;
     const onedc_block_norm_params q = joined_pictures(p);
     Plan pl;
     const Shape shape = row_shape(p->C, WIDEST, false, &pl.L);
@@ -986,6 +1023,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     if (sums && !onedc_grid_fits((int64_t)(any ? q.B : p->B) * ((p->C + 31) / 32), NT)) return -2;
     const int64_t need = onedc_block_norm_backward_ws_bytes(p, g);
     if (need && (!g->ws || g->ws_bytes < need || (uintptr_t)g->ws & 15)) return -15;
+    if (!gradients_apart(p, g, need)) return ONEDC_SHARED_MEMORY;
     if (!any) {
         if (sums) {                                  // no rows: every sum is 0
             onedc_block_norm_params none = *p;

@@ -266,3 +266,34 @@ def test_mxfp4_outputs_in_operands(fmt):
     shared(K.mxfp4_quantize, x, K.MxFp4(room[:M * k // 2].view(M, k // 2), room[64:64 + M * k // 32].view(M, k // 32), M, k))
     shared(K.mxfp4_dequantize, K.MxFp4(room[:M * k // 2].view(M, k // 2), q.scales, M, k), y)
     shared(K.mxfp4_dequantize, K.MxFp4(q.codes, room[-M * k // 32:].view(M, k // 32), M, k), y)
+
+
+def test_block_norm_outputs_in_vectors_and_gradients_in_rows(fmt):
+    B, N, Cc = 2, 6, 64
+    g = gen(52)
+    x, f, dy, dxo = (tokens(rand(g, B, N, Cc).to(F32)) for _ in range(4))
+    xo, y, dx, df = (empty(B, N, Cc, F32) for _ in range(4))
+    mod = torch.ones(B, 3 * Cc, device=DEV)
+    gate, scale, shift = mod[:, :Cc], mod[:, Cc:2 * Cc], mod[:, 2 * Cc:]
+    w, flat = torch.ones(Cc, device=DEV), torch.ones(B * N * Cc, device=DEV)
+    inside = View(flat, B, 1, N, Cc)
+    for p in (dict(gate=flat[Cc:2 * Cc]), dict(scale=flat[-Cc:]), dict(shift=flat[:B * Cc].view(B, Cc)), dict(w=flat[5:5 + Cc]),
+              dict(post=True, post_b=flat[:Cc])):
+        shared(K.block_norm, x, inside, f=f, xo=xo, **p)
+        shared(K.block_norm, x, y, f=f, xo=inside, **p)
+        shared(K.block_norm_backward, x, dy, inside, dxo=dxo, f=f, df=df, **p)
+        shared(K.block_norm_backward, x, dy, dx, dxo=dxo, f=f, df=inside, **p)
+    given = dict(dxo=dxo, f=f, df=df, gate=gate, scale=scale, shift=shift, w=w, b=w)
+    buf = torch.empty(4 * Cc, device=DEV)
+    shared(K.block_norm_backward, x, dy, dx, **given, d_w=buf[:Cc], d_b=buf[8:8 + Cc])
+    shared(K.block_norm_backward, x, dy, dx, **given, d_gate=buf[:B * Cc].view(B, Cc), d_w=buf[B * Cc - 1:(B + 1) * Cc - 1])
+    for v in (x, f, dy, dxo, dx, df):
+        shared(K.block_norm_backward, x, dy, dx, **given, d_w=v.t[-Cc:])
+        shared(K.block_norm_backward, x, dy, dx, **given, d_scale=v.t[:B * Cc].view(B, Cc))
+    shared(K.block_norm_backward, x, dy, dx, **given, d_w=w)
+    shared(K.block_norm_backward, x, dy, dx, **given, d_b=mod.view(-1)[Cc - 1:2 * Cc - 1])
+    # end to end is apart
+    K.block_norm_backward(x, dy, dx, **given, d_w=buf[:Cc], d_b=buf[Cc:2 * Cc], d_gate=buf[2 * Cc:].view(B, Cc))
+    alone = [torch.empty(Cc, device=DEV), torch.empty(Cc, device=DEV), torch.empty(B, Cc, device=DEV)]
+    K.block_norm_backward(x, dy, dx, **given, d_w=alone[0], d_b=alone[1], d_gate=alone[2])
+    assert torch.equal(buf, torch.cat([t.flatten() for t in alone]))

@@ -46,7 +46,7 @@ read = open(sys.argv[2], "a+")
 for name, args in json.load(sys.stdin):
     if name == "onedc_block_norm_backward":
         p, g = K.BlockNormParams(**args[0]), K.BlockNormGrad(**args[1])
-        g.ws, g.ws_bytes = 1 << 46, 1 << 62
+        g.ws, g.ws_bytes = 1 << 54, 1 << 62
         rc = lib.onedc_block_norm_backward(ctypes.byref(p), ctypes.byref(g), None)
     elif name in structs:
         rc = getattr(lib, name)(ctypes.byref(structs[name](**args)), None)
@@ -90,7 +90,7 @@ def inside_limits(calls, got):
             assert lds <= most <= 160 * 1024, (call, lds, most)
 
 
-FAR = 1 << 40                                             # operands far from each other
+FAR = 1 << 43                                             # operands far from each other
 
 
 def rotary(rows, qh, kh, D, pairs, x_f32=0, neighbours=0, B=1):

@@ -55,6 +55,91 @@ def test_rows_that_meet_or_do_not(tmp_path):
     assert not shared(0, 3, 8, 2, 1, 1, 8, 1)             # NULL: no operand
 
 
+# ---- block_norm -------------------------------------------------------------------------------------------------------------------
+B, TOKENS, CH = 3, 5, 24
+ROWS = dict(x=0x100000, f=0x200000, xo=0x300000, y=0x400000)
+VECTORS = dict(post_w=0x500000, post_b=0x510000, gate=0x520000, w=0x530000, b=0x540000, scale=0x550000, shift=0x560000)
+PER_PICTURE = dict(gate_rs=CH + 8, scale_rs=CH, shift_rs=3 * CH)
+
+
+def norm_params(**over):
+    p = dict(B=B, N=TOKENS, C=CH, x_cs=CH, f_cs=CH, xo_cs=CH, y_cs=CH, post=1, alpha=1.0, eps=1e-5, **ROWS, **VECTORS, **PER_PICTURE)
+    return {**p, **over}
+
+
+def norm(**over):
+    return K.lib().onedc_block_norm(C.byref(K.BlockNormParams(**norm_params(**over))), None)
+
+
+def last_of(name):
+    """The first byte of a vector's last value."""
+    return VECTORS[name] + 4 * ((CH if name in ("post_w", "post_b", "w", "b") else (B - 1) * PER_PICTURE[name + "_rs"] + CH) - 1)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("name", sorted(VECTORS))
+def test_block_norm_outputs_in_a_vector(name, f32):
+    size = B * TOKENS * CH * (4 if f32 else 2)
+    for out in ("xo", "y"):
+        for at in (VECTORS[name], last_of(name), VECTORS[name] - size + 4):
+            assert norm(**{out: at}, x_f32=f32, f_f32=f32) == SHARED, (out, hex(at))
+    # a row of the stream that has the parameters behind its channels, whatever picture's they are
+    if name == "gate":
+        assert norm(gate=ROWS["xo"] + 4 * CH - 4, gate_rs=TOKENS * 64, xo_cs=64, x_f32=1) == SHARED
+
+
+GRADS = dict(d_post_w=0x600000, d_post_b=0x610000, d_gate=0x620000, d_w=0x630000, d_b=0x640000, d_scale=0x650000, d_shift=0x660000)
+GRAD_ROWS = dict(dy=0x700000, dxo=0x710000, dx=0x720000, df=0x730000)
+
+
+def norm_back(p=None, **over):
+    g = dict(**GRADS, **GRAD_ROWS, dy_cs=CH, dxo_cs=CH, dx_cs=CH, df_cs=CH, ws=0x900000, ws_bytes=1 << 20)
+    params, grad = K.BlockNormParams(**norm_params(**(p or {}))), K.BlockNormGrad(**{**g, **over})
+    return K.lib().onedc_block_norm_backward(C.byref(params), C.byref(grad), None)
+
+
+def grad_bytes(name):
+    return 4 * CH * (B if name in ("d_gate", "d_scale", "d_shift") else 1)
+
+
+@pytest.mark.parametrize("name", sorted(GRADS))
+def test_block_norm_gradients_in_other_memory(name):
+    size = grad_bytes(name)
+    places = [v for o, v in GRADS.items() if o != name] + [v + grad_bytes(o) - 4 for o, v in GRADS.items() if o != name]
+    places += [v - size + 4 for o, v in GRADS.items() if o != name]
+    places += list(VECTORS.values()) + [last_of(v) for v in VECTORS] + [VECTORS["scale"] - size + 4]
+    places += list(GRAD_ROWS.values()) + [v + B * TOKENS * CH * 2 - 4 for v in GRAD_ROWS.values()] + [ROWS["x"], ROWS["f"] + 48, 0x900000, 0x900040]
+    for at in places:
+        assert norm_back(**{name: at}) == SHARED, hex(at)
+    # one row for all pictures: C values, not B C
+    if size > 4 * CH:
+        one = {name[2:] + "_rs": 0}
+        assert norm_back(one, **{name: GRADS["d_w"] - 4 * CH + 4}) == SHARED
+        # no rows: gradients are written all the same (zeros), and parameters are not theirs to write
+        assert norm_back(dict(N=0), **{name: VECTORS["w"]}) == SHARED
+
+
+def test_block_norm_backward_outputs_and_workspace_in_other_memory():
+    for out in ("dx", "df"):
+        for name in VECTORS:
+            assert norm_back(**{out: VECTORS[name]}) == norm_back(**{out: last_of(name) - 2}) == SHARED
+    for at in [*VECTORS.values(), *GRAD_ROWS.values(), *GRADS.values(), ROWS["x"], ROWS["f"]]:
+        assert norm_back(ws=at) == SHARED, hex(at)
+
+
+def test_what_block_norm_still_takes(launches):
+    p = norm_params()
+    g = dict(**GRADS, **GRAD_ROWS, dy_cs=CH, dxo_cs=CH, dx_cs=CH, df_cs=CH)
+    stream = 0x100000                                    # one buffer: f32 rows of 128 values, a picture one token; parameters behind the channels
+    rows = dict(B=B, N=1, x=stream, xo=stream, x_cs=128, xo_cs=128, x_f32=1, gate=stream + 4 * CH, gate_rs=128, scale=stream + 8 * CH, scale_rs=128)
+    packed = {n: 0x600000 + 4 * CH * i for i, n in enumerate(("d_w", "d_b", "d_post_w", "d_post_b"))}        # end to end
+    calls = [["onedc_block_norm", p], ["onedc_block_norm", {**p, "xo": p["x"]}], ["onedc_block_norm", {**p, **rows}],
+             ["onedc_block_norm", {**p, "scale": p["gate"], "shift": p["gate"], "scale_rs": p["gate_rs"], "shift_rs": p["gate_rs"]}],
+             ["onedc_block_norm_backward", [p, g]], ["onedc_block_norm_backward", [p, {**g, "dx": g["dxo"], "df": g["dy"]}]],
+             ["onedc_block_norm_backward", [{**p, **rows}, {**g, **packed}]], ["onedc_block_norm_backward", [{**p, "N": 0}, g]]]
+    assert [rc for rc, _ in launches(calls)] == [0] * len(calls)
+
+
 # ---- mxfp4 ------------------------------------------------------------------------------------------------------------------------
 M, N, KV = 40, 64, 200                                    # two steps of 128: 128 bytes of codes and 8 of scales a row
 AT = dict(xc=0x100000, xs=0x200000, wc=0x300000, ws=0x400000, bias=0x500000, y=0x600000)
