@@ -926,10 +926,10 @@ def block_norm(x, y=None, *, f=None, xo=None, kind=NORM_LAYER, eps=1e-5, post=Fa
         _check_apart(what, "y", sy, (sx, sf, so))
     _check_device(what, (x.t, None if f is None else f.t, None if xo is None else xo.t, None if y is None else y.t, post_w, post_b, gate, w, b,
                          scale, shift))
-    p = _block_norm_params(sx[4], sf[4] if sf else 0, so[4] if so else 0, sy[4] if sy else 0, _address(post_w), _address(post_b), _address(gate),
-                           _address(w), _address(b), _address(scale), _address(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0,
-                           f.co if sf else 0, xo.cs if so else 0, xo.co if so else 0, y.cs if sy else 0, y.co if sy else 0, gate_rs, scale_rs,
-                           shift_rs, kind, 1 if post else 0, 1 if x.t.dtype is torch.float32 else 0, 1 if (f or y).t.dtype is torch.float32 else 0,
+    p = _block_norm_params(sx[4], sf[4] if sf else 0, so[4] if so else 0, sy[4] if sy else 0,
+                           *[0 if t is None else t.data_ptr() for t in (post_w, post_b, gate, w, b, scale, shift)], x.B, x.H * x.W, x.C, x.cs, x.co,
+                           f.cs if sf else 0, f.co if sf else 0, xo.cs if so else 0, xo.co if so else 0, y.cs if sy else 0, y.co if sy else 0,
+                           gate_rs, scale_rs, shift_rs, kind, 1 if post else 0, 1 if x.t.dtype is torch.float32 else 0, 1 if (f or y).t.dtype is torch.float32 else 0,
                            alpha, eps)
     _ok(lib().onedc_block_norm(C.byref(p), stream()), "onedc_block_norm")
     return xo, y
@@ -967,18 +967,18 @@ def block_norm_backward(x, dy, dx=None, *, dxo=None, f=None, df=None, kind=NORM_
             if of is None:
                 raise KernelError(f"{what}: {name} of a parameter that the call has not")
             _check_vector(what, name, t, x.C * rows)
-    outs = [t.data_ptr() for t in (d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift) if t is not None]
-    if len(set(outs)) != len(outs) and x.B:
+    grads = [0 if t is None else t.data_ptr() for t in (d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift)]
+    outs = [a for a in grads if a]
+    if len(set(outs)) != len(outs) and x.B:          # (one that begins inside another: the entry's check)
         raise KernelError(f"{what}: two parameter gradients share memory")
     _check_device(what, [v.t for v in (x, f, dy, dxo, dx, df) if v is not None] +
                   [post_w, post_b, gate, w, b, scale, shift, d_post_w, d_post_b, d_gate, d_w, d_b, d_scale, d_shift])
     side = f or dy
-    p = _block_norm_params(sx[4], sf[4] if sf else 0, 0, 0, _address(post_w), _address(post_b), _address(gate), _address(w), _address(b),
-                           _address(scale), _address(shift), x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, 0, 0, 0, 0,
+    p = _block_norm_params(sx[4], sf[4] if sf else 0, 0, 0,
+                           *[0 if t is None else t.data_ptr() for t in (post_w, post_b, gate, w, b, scale, shift)], x.B, x.H * x.W, x.C, x.cs, x.co, f.cs if sf else 0, f.co if sf else 0, 0, 0, 0, 0,
                            gate_rs, scale_rs, shift_rs, kind, 1 if post else 0, 1 if x.t.dtype is torch.float32 else 0,
                            1 if side is not None and side.t.dtype is torch.float32 else 0, alpha, eps)
-    g = _block_norm_grad(sy[4] if sy else 0, so[4] if so else 0, sdx[4] if sdx else 0, sdf[4] if sdf else 0, _address(d_post_w),
-                         _address(d_post_b), _address(d_gate), _address(d_w), _address(d_b), _address(d_scale), _address(d_shift), 0, 0,
+    g = _block_norm_grad(sy[4] if sy else 0, so[4] if so else 0, sdx[4] if sdx else 0, sdf[4] if sdf else 0, *grads, 0, 0,
                          dy.cs if sy else 0, dy.co if sy else 0, dxo.cs if so else 0, dxo.co if so else 0, dx.cs if sdx else 0,
                          dx.co if sdx else 0, df.cs if sdf else 0, df.co if sdf else 0)
     native, at_p, at_g = lib(), C.byref(p), C.byref(g)
