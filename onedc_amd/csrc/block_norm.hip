@@ -196,9 +196,9 @@ struct Vector {
         on = on_;
         if (!on) return;
         if constexpr (SHARED) {
-            last = (p.C + 7) & ~7;
-            for (int c = threadIdx.x; c < last; c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
-            if (threadIdx.x < 8) at_lds[last + threadIdx.x] = 0.f;
+            last = ((p.C + 7) & ~7) - (WHICH == HAS_A ? 0 : 8);
+            for (int c = threadIdx.x; c < ((p.C + 7) & ~7); c += blockDim.x) at_lds[c] = c < p.C ? combined(p, WHICH, b, c) : 0.f;
+            if (WHICH == HAS_A && threadIdx.x < 8) at_lds[last + threadIdx.x] = 0.f;
             lds = at_lds;
             at_lds += last + 8;
         } else {
@@ -208,11 +208,12 @@ struct Vector {
                 for (int j = 0; j < 8; ++j) {
                     const int c = c0 + i * step + j;
                     const float q = combined(p, WHICH, b, min(c, p.C - 1));
-                    v[i][j] = c < p.C ? q : 0.f;
+                    v[i][j] = WHICH != HAS_A || c < p.C ? q : 0.f;
                 }
         }
     }
-    // eight of them from channel c on; zeros behind the row (an infinite one there would make a sum over the row no number)
+    // eight of them from channel c on; a piece behind the row gets the last ones, which multiply zeros and are not stored, but of A zeros: an
+    // infinite gate there would make a sum over the row no number
     __device__ __forceinline__ void get(int i, int c, float (&o)[8]) const {
         if constexpr (SHARED) {
             c = min(c, last);
@@ -968,7 +969,7 @@ int onedc_block_norm(const onedc_block_norm_params *p, void *stream) {
         if (!onedc_grid_fits((int64_t)q.B * pl.runs, shape.threads)) return -2;
         const int opt = !p->f || !p->y || p->post_b ? GENERIC : p->post ? JOIN_POST : JOIN;
         if (opt) pl.has = HAS_A | HAS_W | HAS_S;
-        const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)__builtin_popcount(pl.has) * (((p->C + 7) & ~7) + 8) * 4 : 0);
+        const size_t lds = shape.threads / 64 * 16 + (shape.shared ? (size_t)(__builtin_popcount(pl.has) * ((p->C + 7) & ~7) + 8) * 4 : 0);
         const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
         by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
             constexpr int NTH = decltype(nth)::value, IT = decltype(it)::value;
@@ -1042,7 +1043,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
     float *part = sums ? (float *)((char *)g->ws + pictures_bytes(q, g)) : nullptr;
     const dim3 grid((unsigned)((int64_t)q.B * pl.runs));
     if (rows) {
-        const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most with their zeros, then the sums)
+        const size_t scratch = shape.shared ? (size_t)4 * ((p->C + 7) & ~7) * 4 : 0;          // (the vectors, two at most and A's zeros, then the sums)
         const size_t lds = shape.threads / 64 * 16 + scratch;
         const int opt = !p->f || !g->dy || !g->dxo || !g->dx || !g->df ? GENERIC : p->post ? JOIN_POST : JOIN;
         by_shape(shape, p->x_f32, p->f_f32, p->C & 7, opt, [&](auto nth, auto shared, auto it, auto x32, auto f32, auto tail, auto what) {
