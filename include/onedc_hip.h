@@ -428,7 +428,7 @@ int onedc_block_norm_backward(const onedc_block_norm_params *p, const onedc_bloc
  * to 2^-53 of the position whatever its size; sine and cosine in f32).  axis: int32 [pairs], each in [0, axes).  pos: int32 or
  * (pos_f32) f32 [N][axes], pos_bs elements between pictures (0: the same for all).  x16 or (x_f32) f32 heads.  q / k may be
  * transformed in place (qo == q with the same strides); kh = 0: no keys.
- * Returns -1 for a missing pointer, -2 for sizes or strides. */
+ * Returns -1 for a missing pointer, -2 for sizes or strides, ONEDC_SHARED_MEMORY where qo or ko lies in the memory of pos, turns or axis. */
 typedef struct onedc_rotary_params {
     const void *q; void *qo; const void *k; void *ko; const void *pos; const double *turns; const int32_t *axis;
     int32_t B, N, D, pairs, axes, qh, kh;

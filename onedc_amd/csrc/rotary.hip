@@ -13,6 +13,7 @@
 // 25 us, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; one token 3.0 us in a graph, a launch's own time.
 #include <type_traits>
 
+#include "apart.h"
 #include "conv_common.h"
 #include "elem.h"
 
@@ -186,6 +187,11 @@ extern "C" int onedc_rotary_axes(const onedc_rotary_params *p, void *stream) {
     if (p->q_co < 0 || p->q_cs - cq < p->q_co || p->qo_co < 0 || p->qo_cs - cq < p->qo_co) return -2;
     if (p->kh && (p->k_co < 0 || p->k_cs - ck < p->k_co || p->ko_co < 0 || p->ko_cs - ck < p->ko_co)) return -2;
     if (!p->B || !p->N) return 0;
+    const auto rows = [&](const void *t, int64_t cs, int64_t co, int64_t c) { return onedc_mem_rows(t, (int64_t)p->B * p->N, cs, co, c, p->x_f32 ? 4 : 2); };
+    const OnedcMem out[] = {rows(p->qo, p->qo_cs, p->qo_co, cq), p->kh ? rows(p->ko, p->ko_cs, p->ko_co, ck) : OnedcMem()};
+    const OnedcMem plan[] = {onedc_mem(p->pos, ((p->B - 1) * p->pos_bs + (int64_t)p->N * p->axes) * 4), onedc_mem(p->turns, (int64_t)p->pairs * 8),
+                             onedc_mem(p->axis, (int64_t)p->pairs * 4)};
+    if (onedc_mem_any_shared(out, plan)) return ONEDC_SHARED_MEMORY;
     // the widest piece that divides a head's parts and every row's beginning: 16 bytes, 8 bytes, or single values
     const int part = p->neighbours ? 2 * p->pairs : p->pairs, size = p->x_f32 ? 4 : 2;
     int bits = part | (p->D - 2 * p->pairs) | p->D | p->q_cs | p->q_co | p->qo_cs | p->qo_co;

@@ -297,3 +297,17 @@ def test_block_norm_outputs_in_vectors_and_gradients_in_rows(fmt):
     alone = [torch.empty(Cc, device=DEV), torch.empty(Cc, device=DEV), torch.empty(B, Cc, device=DEV)]
     K.block_norm_backward(x, dy, dx, **given, d_w=alone[0], d_b=alone[1], d_gate=alone[2])
     assert torch.equal(buf, torch.cat([t.flatten() for t in alone]))
+
+
+def test_rotary_outputs_in_positions(fmt):
+    D, N = 16, 8
+    plan, q, k = RotaryAxes(D, (8, 8), device=DEV), tokens(rand(gen(53), 1, N, 2 * D).to(fmt)), tokens(rand(gen(54), 1, N, D).to(fmt))
+    buf = torch.zeros(N * 2 * D, dtype=torch.int32, device=DEV)
+    inside = View(buf.view(fmt)[:N * 2 * D], 1, 1, N, 2 * D)
+    for at in (0, N * D - 2 * N):
+        pos = buf[at:at + 2 * N].view(N, 2)
+        shared(K.rotary_axes, plan, pos, q, inside, k)
+        shared(K.rotary_axes, plan, pos, inside)
+        shared(K.rotary_axes, plan, pos, q, None, k, View(inside.t, 1, 1, N, D, 2 * D, D if at else 0))
+    K.rotary_axes(plan, buf[N * D:N * D + 2 * N].view(N, 2), q, inside)          # behind it
+    assert torch.equal(back(inside), back(q))                                    # position 0

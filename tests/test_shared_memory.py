@@ -140,6 +140,33 @@ def test_what_block_norm_still_takes(launches):
     assert [rc for rc, _ in launches(calls)] == [0] * len(calls)
 
 
+# ---- rotary -----------------------------------------------------------------------------------------------------------------------
+ROT = dict(q=0x100000, qo=0x200000, k=0x300000, ko=0x400000, pos=0x500000, turns=0x510000, axis=0x520000, B=2, N=6, D=16, pairs=7, axes=3, qh=4, kh=2,
+           q_cs=64, qo_cs=64, k_cs=32, ko_cs=32, pos_bs=18)
+
+
+def rotary(**over):
+    return K.lib().onedc_rotary_axes(C.byref(K.RotaryParams(**{**ROT, **over})), None)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_rotary_outputs_in_the_plan_or_the_positions(f32):
+    size = 4 if f32 else 2
+    for out, heads in (("qo", 4), ("ko", 2)):
+        rows = 12 * heads * 16 * size
+        for name, n in (("pos", 2 * 18 * 4), ("turns", 7 * 8), ("axis", 7 * 4)):
+            for at in (ROT[name], ROT[name] + n - size, ROT[name] - rows + size):
+                assert rotary(**{out: at}, x_f32=f32) == SHARED, (out, name, hex(at))
+    assert rotary(qo=0x500000 + 18 * 4 - size, pos_bs=0, x_f32=f32) == SHARED               # one picture's positions for all
+
+
+def test_what_rotary_still_takes(launches):
+    same = dict(ROT, qo=ROT["q"], ko=ROT["k"])
+    calls = [["onedc_rotary_axes", ROT], ["onedc_rotary_axes", same], ["onedc_rotary_axes", dict(ROT, qo=ROT["pos"] + 2 * 18 * 4, ko=ROT["axis"] + 28)],
+             ["onedc_rotary_axes", dict(ROT, pos_bs=0, qo=ROT["pos"] + 18 * 4)], ["onedc_rotary_axes", dict(ROT, kh=0, k=None, ko=None)]]
+    assert [rc for rc, _ in launches(calls)] == [0] * len(calls)
+
+
 # ---- mxfp4 ------------------------------------------------------------------------------------------------------------------------
 M, N, KV = 40, 64, 200                                    # two steps of 128: 128 bytes of codes and 8 of scales a row
 AT = dict(xc=0x100000, xs=0x200000, wc=0x300000, ws=0x400000, bias=0x500000, y=0x600000)
