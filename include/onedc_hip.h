@@ -382,7 +382,8 @@ int onedc_mxfp8_roundtrip(const void *x, void *y, int64_t pixels, int C, int x_c
  *   t  = x + alpha * gate[b] * P(f)                         P = identity, or (post) norm(f) * post_w + post_b
  *   xo = t in the stream's type                             (f, xo NULL: t = x, no join)
  *   y  = (norm(t) * w + b) * (1 + scale[b]) + shift[b]      (y NULL: no norm behind the join)
- * norm = LayerNorm (mean and variance) or RMSNorm (mean square) over the C channels, statistics and arithmetic in f32; y is taken
+ * norm = LayerNorm (mean and variance) or RMSNorm (mean square) over the C channels, statistics and arithmetic in f32 (where squares
+ * pass f32's range, an infinity under RMSNorm among them, the deviation is infinite and the row's finite values become 0); y is taken
  * from t BEFORE xo's rounding.  Every vector is f32 and may be NULL (factor 1, summand 0); gate / scale / shift hold one row per
  * picture, `*_rs` floats apart (0: one row for all pictures, e.g. a learned per-channel residual scale as the gate).
  * x and xo are 16-bit or (x_f32) f32; f, y are 16-bit or (f_f32, only with x_f32) f32.  Rows are NHWC views: channel stride *_cs,

@@ -26,9 +26,10 @@ constexpr int NT = 256;
 //   A = alpha gate post_w, Ab = alpha gate post_b (join);  W = w (1 + scale), S = b (1 + scale) + shift (norm behind it)
 // into LDS where several rows of a wave share them, into registers where a thread owns its channels.  The next row's loads are in
 // flight while a row is computed.
-// 16-bit, gated, modulated, norms on both sides: 16 x 9216 x 320 in 83 us (4.6 TB/s of 5.15 that a large copy reaches), 16 x 2304 x 640 34 us (5.5),
-// 16 x 576 x 1280 22 us (4.4), 16 x 2304 x 643 36 us (5.3), 16 x 576 x 4096 69 us (4.4); with every gradient backward 130 us (4.4), 64 us (4.4),
-// 48 us (2.9), 78 us (3.6), 113 us (4.0), of which the sums over the rows are 7 to 11.
+// 16-bit, gated, modulated, norms on both sides: 16 x 9216 x 320 in 81 us (4.7 TB/s of 5.15 that a large copy reaches), 16 x 2304 x 640 33 us (5.7),
+// 16 x 576 x 1280 21 us (4.5), 16 x 2304 x 643 36 us (5.3), 16 x 576 x 4096 63 us (4.8); with every gradient backward 131 us (4.3), 71 us (4.0),
+// 56 us (2.5: 160 pieces leave 96 of 256 lanes idle, and every sum is a barrier), 84 us (3.4), 113 us (4.0), of which the sums over the rows are 7 to 11.
+// Norm alone 36, 21 and 13 us of the first three, join alone 47, 24 and 15.
 // Outputs stored past the cache take the first to 62 us and give it all back in whoever reads them.
 
 // sum over the L neighbouring lanes of v's row, the same bits in each of them
@@ -257,8 +258,8 @@ __device__ __forceinline__ float normalise(float (&v)[IT][8], int c0, int step, 
     return r;
 }
 
-// What a call has, known to the compiler for the join between two sub-blocks in full (its branches cost the generic form a third of its
-// time); GENERIC asks the arguments.
+// What a call has, known to the compiler for the join between two sub-blocks in full; GENERIC asks the arguments (join and norm with a post_b:
+// 16 x 9216 x 320 85 us against 84 without, 16 x 2304 x 640 39 against 35, 16 x 576 x 1280 25 against 23).
 enum { GENERIC = 0, JOIN = 1, JOIN_POST = 2 };
 
 // NTH 256: rows of up to 64 lanes (SHARED), or one row a workgroup

@@ -103,6 +103,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 
 // Four neighbouring lanes hold a block, eight values each: a wave reads 1 KB (16-bit) in a row and writes 256 bytes of codes.  HBM bound: 16384 x 8192
 // bf16 to codes 59 us, 5.7 TB/s, and back 60 us, 5.6 TB/s (f32 109 us, 5.6 TB/s; back 155 us, 3.9 TB/s: 32 bytes a lane to store).
+// Rows that do not begin at whole 16 bytes are read and written as single values: 16384 x 8191 133 us, back 185 us.
 // A workgroup takes QN consecutive groups of 256 pieces of eight values, the pieces of all rows counted through.
 constexpr int QN = 4;
 template <bool F32, bool VEC>
@@ -240,7 +241,8 @@ __device__ __forceinline__ void store8(const onedc_mxfp4_params &p, int64_t m, i
 // consecutive steps of a round straight from memory, 256 bytes of every weight row and 16 bytes of its scales, all in flight at once (steps dealt
 // out in turn instead would send all waves to the same memory channels where a row is a power of two long: 8192 x 8192 against one row 11.3 us
 // that way).  The waves' sums are added through LDS in wave order.  Raw rows are quantised by the workgroup together, under the weights' loads, into LDS.
-// 8192 x 8192 against one row of codes 8.2 us (4.3 TB/s of weights), a raw row 8.7 us, sixteen 9.8 and 13.1 us.
+// 8192 x 8192 against one row of codes 9.3 us (3.8 TB/s of weights), a raw row 9.7 us, sixteen 10.7 and 14.1 us (every workgroup quantises the rows
+// for itself).
 constexpr int SKW = 16, SKU = 4, ROUND = SKW * SKU;                       // steps of a round
 constexpr int XPITCH = ROUND * 64 + 16, SPITCH = ROUND * 4 + 16;          // bytes of a row's codes and scales in LDS, off the banks' period
 
@@ -360,10 +362,11 @@ __global__ __launch_bounds__(64 * SKW) void skinny_kernel(onedc_mxfp4_params p, 
 // The DMA is written as instructions (it has no destination register): behind the builtin the compiler drains every DMA in flight
 // before each LDS read.
 // 32x32x64 in place of 16x16x128: 6.4 against 5.2 - 5.9 PFLOP/s from registers on random codes, where power bounds it (9.7 on zeros).
-// 16384 x 8192 x 8192, 256 x 256: 550 - 572 us, 3.8 - 4.0 PFLOP/s.  Without the DMA it takes 465, without the LDS reads 524, without both
-// 373, without the stores 507, the products alone 337: the feeding and the power limit bound it together.  Stages of one step in rings of
-// three and four, 2 x 4 waves, other spacings of the DMA and outputs stored from registers (605 us) gained nothing.  4096^3 40 us, 3.4 PFLOP/s;
-// 8655 x 10240 x 1280 gated 96 - 115 us, 2.0 - 2.3 PFLOP/s: ten steps a tile, its GELU costs as much as its products.
+// 16384 x 8192 x 8192, 256 x 256: 544 - 572 us, 3.8 - 4.0 PFLOP/s.  Without the DMA it takes 465, without the LDS reads 524, without both
+// 373, without the stores 507, the products alone 337: the feeding and the power limit bound it together; the matrix pipe is busy 0.44 of the
+// time, and of the LDS reads' cycles 0.48 are conflicts.  Stages of one step in rings of three and four, 2 x 4 waves, other spacings of the DMA and
+// outputs stored from registers (605 us) gained nothing.  4096^3 40 us, 3.4 PFLOP/s; 8655 x 10240 x 1280 gated 103 - 115 us, 2.0 - 2.2 PFLOP/s: ten
+// steps a tile, its GELU costs as much as its products.
 #define MX_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -718,18 +721,20 @@ int onedc_mxfp4_linear(const onedc_mxfp4_params *p, void *stream) {
     }
     // (the tiles' scale reads need 16 bytes in all)
     if (p->M <= ONEDC_MXFP4_ROWS_RAW || (int64_t)p->N * steps < 4) return launch_skinny<0, true>(p, steps, whole, stream);
-    // Tiles, by how many of them there are for 256 CUs (measured on grids of M 64 .. 36864, N 320 .. 10240, K 320 .. 8192):
-    //   256 x 256, eight waves, two stages: the fewest bytes into LDS a product.  From 160 tiles on, where it pads no tenth more than 128 x 128;
-    //     gated layers only from 32 steps on (8192 x 4096 x 5120: 95 us against 110; gated 8655 x 10240 x 1280: 117 against 100, there
-    //     the epilogue counts, and nothing else runs on the CU meanwhile)
+    // Tiles, by how many of them there are for 256 CUs.  One card, the shapes in turn (f16, gated ones with a bias and operands that no cache holds):
+    //   256 x 256, eight waves, two stages: the fewest bytes into LDS a product.  From 160 tiles on, where it pads no tenth more than 128 x 128
+    //     (8192 x 4096 x 5120: 94 us against 109; 16384 x 8192 x 8192: 544 against 626); gated layers, whose epilogue runs under nothing else on
+    //     the CU, only from 32 steps on (8192 x 10240 x 4096: 203 us against 207 of 128 x 256; with 30 steps 228 against 231, with 20 175 against
+    //     173, with 10 121 against 110, with 5 190 against 173)
     //   64 x 64, two teams of four waves that halve a long K, while there is no second workgroup for a CU: one team waits where the other
-    //     multiplies (300 x 520 x 8192: 9.8 us against 12.4, 1024 x 1024 x 8192: 12.0 against 14.1; with 10 steps 9.8 against 5.9, three or four
-    //     teams 10.2 and 10.5 in the first case)
-    //   64 x 64, three stages, while they fit the CUs' first four each (2048 x 1280 x 5120: 17 us against 19; 4096 x 1280 x 5120: 28 against 26)
+    //     multiplies (300 x 520 x 8192: 11.5 us against 14.2, 1024 x 1024 x 8192: 13.0 against 15.6; with 10 steps 9.8 against 5.9, three or four
+    //     teams 10.2 and 10.5 in the first case where two took 9.8)
+    //   64 x 64, three stages, while they fit the CUs' first four each (2048 x 1280 x 5120: 18 us against 21; 4096 x 1280 x 5120: 29 against 27)
     //   128 x 128: one stage and three workgroups a CU that load and multiply in turn; two stages where there are less than two a CU
-    //     (4096 x 1280 x 5120: 26 us against 28; 8192 x 4096 x 5120: 112 against 110)
-    //   128 x 256, four waves, one stage, two workgroups a CU: gated layers of very many tiles, whose epilogue weighs most (8655 x 10240 x 1280: 115.5 us
-    //     against 120, 36864 x 5120 x 640: 171.5 against 175; linear 36864 x 640 x 640 28 against 25)
+    //     (4096 x 1280 x 5120: 27 us against 30; 8192 x 4096 x 5120: 112 against 109)
+    //   128 x 256, four waves, one stage, two workgroups a CU: gated layers of very many tiles, the more the longer their K (9216 x 10240 x 3840: 231 us
+    //     against 240, 16384 x 10240 x 1280: 191 against 197; 8655 x 10240 x 1280 110 both, 36864 x 5120 x 640 173 against 172; linear
+    //     36864 x 640 x 640 28 against 25.5)
     const auto tiles = [&](int64_t t) { return ((p->N + t - 1) / t) * ((p->M + t - 1) / t); };
     const bool gated = p->epi == ONEDC_EPI_GEGLU;
     if (tiles(256) >= 160 && tiles(256) * 40 <= tiles(128) * 11 && (!gated || steps >= 32)) return launch_tiles<4, 2, 2, 4, 2, 2, 1>(p, steps, whole, stream);

@@ -10,7 +10,7 @@
 // lanes hold neighbouring heads, so most of a wave's LDS reads are one address).  Pieces of 16 bytes where the sizes allow it, two or four of a
 // thread in flight.  16-bit heads: 49152 tokens x 32 x 80 in 101 us, 5.0 TB/s (a copy of 1 GB reaches 5.15; with the angles computed at every element
 // 328 us), 36864 x 16 x 80 40 - 44 us, or, held by the last-level cache, 31 - 33; pairs of which only four share a piece (16384 x 32 x 72, held too)
-// 25 us, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; one token 3.0 us in a graph, a launch's own time.
+// 26 us, single values (32000 x 16 x 42) 26 us, 3.3 TB/s; f32 heads (16384 x 32 x 72) 58 us, 5.2 TB/s; one token 3.0 us in a graph, a launch's own time.
 #include <type_traits>
 
 #include "apart.h"

@@ -311,3 +311,59 @@ def test_rotary_outputs_in_positions(fmt):
         shared(K.rotary_axes, plan, pos, q, None, k, View(inside.t, 1, 1, N, D, 2 * D, D if at else 0))
     K.rotary_axes(plan, buf[N * D:N * D + 2 * N].view(N, 2), q, inside)          # behind it
     assert torch.equal(back(inside), back(q))                                    # position 0
+
+
+def test_two_threads_in_their_own_format_and_stream():
+    """Calls of two threads at once, each on a stream of its own, one with either format's library: workspaces are the calls' own, the format and the
+    current stream the threads'."""
+    import threading
+    B, N, Cc = 2, 700, 320
+    turns, plan = 30, RotaryAxes(40, (20, 20), device=DEV)
+    pos = torch.randint(0, 100, (N, 2), dtype=torch.int32, device=DEV)
+
+    def work(name):
+        t = FORMATS[name]
+        g = torch.Generator(device=DEV).manual_seed(60)
+        x, f, dy, dxo = (torch.randn(B * N * Cc, generator=g, device=DEV).to(t) for _ in range(4))
+        gate, scale, w = torch.randn(B, Cc, generator=g, device=DEV), torch.randn(B, Cc, generator=g, device=DEV), torch.randn(Cc, Cc, generator=g, device=DEV)
+        held = K.mxfp4_quantize(View(w, 1, 1, Cc, Cc))
+
+        def v(buf):
+            return View(buf, B, 1, N, Cc)
+
+        def once():
+            xo, y, z, dx, df = (torch.empty_like(x) for _ in range(5))
+            dg, ds = torch.empty_like(gate), torch.empty_like(scale)
+            K.block_norm(v(x), v(y), f=v(f), xo=v(xo), post=True, gate=gate, scale=scale)
+            K.mxfp4_linear(v(y), held, None, v(z))
+            K.rotary_axes(plan, pos, v(z))
+            K.block_norm_backward(v(xo), v(dy), v(dx), dxo=v(dxo), f=v(f), df=v(df), post=True, gate=gate, scale=scale, d_gate=dg, d_scale=ds)
+            return [xo, z, dx, df, dg, ds]
+        return once
+    fns, want, got, failed = {}, {}, {"f16": [], "bf16": []}, []
+    for name in FORMATS:
+        with K.act_format(name):
+            fns[name] = work(name)
+            want[name] = fns[name]()
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+
+    def run(name):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream), K.act_format(name):
+                start.wait(30)
+                for _ in range(turns):
+                    got[name].append(fns[name]())
+                stream.synchronize()
+        except Exception as e:                           # noqa: BLE001 (shown by the thread that waits)
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(name,)) for name in FORMATS]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for name in FORMATS:
+        assert len(got[name]) == turns and all(torch.equal(a, b) for r in got[name] for a, b in zip(r, want[name])), name
