@@ -10,8 +10,8 @@ pytestmark = pytest.mark.gpu
 
 from onedc_amd import kernels as K
 from onedc_amd.kernels import KernelError, RotaryAxes, View
-from test_gpu_token_ops import (CASES, DEV, EPS32, F32, FORMATS, back, empty, gen, grads64, half_step, held64, in64, join64, norm64, on_gpu,
-                                options, rand, rows_view, tiny, tokens)
+from test_gpu_token_ops import (CASES, DEV, EPS32, F32, FORMATS, back, block_setup, empty, gen, grads64, half_step, held64, in64, join64, linear64,
+                                norm64, on_gpu, options, rand, rotary64, rows_view, run_block, tiny, tokens, tol_rot, tol_y, within)
 
 
 @pytest.fixture(params=["f16", "bf16"])
@@ -367,3 +367,56 @@ def test_two_threads_in_their_own_format_and_stream():
     assert not failed, failed
     for name in FORMATS:
         assert len(got[name]) == turns and all(torch.equal(a, b) for r in got[name] for a, b in zip(r, want[name])), name
+
+
+def test_every_operator_of_a_block_on_the_inputs_it_got(fmt, monkeypatch):
+    """The block of test_gpu_token_ops, each of its operators compared with its definition in 64 bits on what the run itself handed it, to that
+    operator's own tolerance: a small wrong term has nowhere to hide behind the block's other roundings."""
+    B, H, W, heads, D, sections, wts, dev, pos, x, plan = block_setup(fmt)
+    calls, real = [], {n: getattr(K, n) for n in ("block_norm", "mxfp4_linear", "rotary_axes", "mxfp4_quantize")}
+
+    def values(v):                                        # what rows of a View or codes stand for, [rows, K] in 64 bits
+        if isinstance(v, K.MxFp4):
+            y = torch.empty(v.rows, v.K, device=DEV)
+            K.mxfp4_dequantize(v, View(y, 1, 1, v.rows, v.K))
+            return y.cpu().double()
+        return held64(back(v).flatten(0, 1))[2]
+
+    def block_norm(xv, y=None, f=None, xo=None, **a):
+        given, branch = back(xv).double(), back(f).double() if f is not None else None
+        real["block_norm"](xv, y, f=f, xo=xo, **a)
+        a = {k: v.cpu().double() if isinstance(v, torch.Tensor) else v for k, v in {"kind": K.NORM_LAYER, **a}.items()}
+        t, ref = join64(given, branch, a, 1e-5)
+        if xo is not None:
+            step = (t - given).abs() + given.abs()
+            within(back(xo), t, half_step(fmt) * t.abs() + tiny(fmt) + 64 * EPS32 * step.amax(-1, keepdim=True), "xo")
+        if y is not None:
+            within(back(y), ref, tol_y(t, ref, a, fmt), "y")
+        calls.append("block_norm")
+
+    def mxfp4_linear(xv, w, bias, y, epi=K.EPI_LINEAR):
+        ref, err = linear64(values(xv), values(w), None, epi, 1.0, 0.0, None)
+        real["mxfp4_linear"](xv, w, bias, y, epi=epi)
+        within(back(y).flatten(0, 1), ref, half_step(fmt) * ref.abs() + tiny(fmt) + err, "linear")
+        calls.append("mxfp4_linear")
+
+    def rotary_axes(p, at, q, k=None):
+        given = [back(v) for v in (q, k)]
+        real["rotary_axes"](p, at, q, k=k)
+        for v, was in zip((q, k), given):
+            ref = rotary64(was.double(), heads, D, sections, at.cpu(), 10000.0, False, False, False)
+            within(back(v), ref, tol_rot(was, ref, heads, D, fmt), "rotary")
+        calls.append("rotary_axes")
+
+    def mxfp4_quantize(v, q=None):
+        q = real["mxfp4_quantize"](v, q)
+        codes, scales, _ = held64(back(v).flatten(0, 1))
+        assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+        calls.append("mxfp4_quantize")
+        return q
+    for fn in (block_norm, mxfp4_linear, rotary_axes, mxfp4_quantize):
+        monkeypatch.setattr(K, fn.__name__, fn)
+    out = run_block(tokens(x), dev, plan, pos.to(DEV), B, H, W, heads, D)
+    assert sorted(calls) == ["block_norm"] * 3 + ["mxfp4_linear"] * (4 + B) + ["mxfp4_quantize", "rotary_axes"]
+    monkeypatch.undo()
+    assert torch.equal(back(out), back(run_block(tokens(x), dev, plan, pos.to(DEV), B, H, W, heads, D)))
